@@ -222,4 +222,49 @@ unsafe extern "C" {
         message_capacity: usize,
     ) -> Tk100Status;
     pub fn tk100_fp8_projection_static_status(stream: Tk100Stream, word: *mut u32) -> Tk100Status;
+
+    pub fn tk100_page_plan(
+        ctx: *mut Tk100Ctx, stream: Tk100Stream, requests: c_int, table_rows: c_int,
+        max_pages: c_int, page_tokens: c_int, max_tokens: c_int, free_capacity: c_int,
+        request_rows: *const i32, new_tokens: *const i32, lengths: *const i32,
+        lengths_output: *mut i32, block_table: *mut i32, free_pages: *const i32,
+        free_count: *const i32, free_count_output: *mut i32, starts: *mut i32,
+        kv_lengths: *mut i32, positions: *mut i32, slots: *mut i64,
+    ) -> Tk100Status;
+    pub fn tk100_page_release(
+        ctx: *mut Tk100Ctx, stream: Tk100Stream, requests: c_int, table_rows: c_int,
+        max_pages: c_int, page_tokens: c_int, free_capacity: c_int, request_rows: *const i32,
+        lengths: *const i32, lengths_output: *mut i32, block_table: *const i32,
+        free_pages: *mut i32, free_count: *const i32, free_count_output: *mut i32,
+    ) -> Tk100Status;
+    pub fn tk100_rotary_cache(
+        ctx: *mut Tk100Ctx, stream: Tk100Stream, tokens: c_int, q_heads: c_int,
+        kv_heads: c_int, head_dim: c_int, rotary_dim: c_int, axes: c_int,
+        frequencies: *const f64, pair_axes: *const u8, positions: *const i32,
+        query: *const u16, query_token_stride: c_int, query_head_stride: c_int,
+        key: *const u16, value: *const u16, kv_token_stride: c_int, kv_head_stride: c_int,
+        query_norm: *const u16, key_norm: *const u16, query_output: *mut u16,
+        key_output: *mut u16, key_cache: *mut u16, value_cache: *mut u16, pages: c_int,
+        page_tokens: c_int, page_stride: c_int, cache_token_stride: c_int,
+        cache_head_stride: c_int, slots: *const i64,
+    ) -> Tk100Status;
+    pub fn tk100_attention_workspace_bytes(
+        ctx: *const Tk100Ctx, head_dim: c_int,
+    ) -> usize;
+    pub fn tk100_paged_attention(
+        ctx: *mut Tk100Ctx, stream: Tk100Stream, sequences: c_int, tokens: c_int,
+        q_heads: c_int, kv_heads: c_int, head_dim: c_int, starts: *const i32,
+        kv_lengths: *const i32, query: *const u16, gate: *const u16, query_token_stride: c_int,
+        query_head_stride: c_int, key_cache: *const u16, value_cache: *const u16, pages: c_int,
+        page_tokens: c_int, page_stride: c_int, cache_token_stride: c_int,
+        cache_head_stride: c_int, block_table: *const i32, table_rows: c_int, max_pages: c_int,
+        request_rows: *const i32, scale: f32, workspace: *mut c_void, output: *mut u16,
+    ) -> Tk100Status;
+    pub fn tk100_prompt_attention(
+        ctx: *mut Tk100Ctx, stream: Tk100Stream, sequences: c_int, tokens: c_int,
+        q_heads: c_int, kv_heads: c_int, head_dim: c_int, starts: *const i32,
+        query: *const u16, gate: *const u16, query_token_stride: c_int,
+        query_head_stride: c_int, key: *const u16, value: *const u16, kv_token_stride: c_int,
+        kv_head_stride: c_int, scale: f32, workspace: *mut c_void, output: *mut u16,
+    ) -> Tk100Status;
 }

@@ -20,6 +20,10 @@ const SOURCES: &[&str] = &[
     "pair_gemm.cu",
     "peer_reduce.cu",
     "sampler.cu",
+    "paging.cu",
+    "rotary.cu",
+    "attention.cu",
+    "attention_ops.cu",
     "ops.cu",
     "static_entry.cu",
 ];

@@ -460,6 +460,106 @@ TK100_API tk100_status tk100_fp8_projection_static(
  * static launches used, after them. */
 TK100_API tk100_status tk100_fp8_projection_static_status(tk100_stream stream, uint32_t* word);
 
+/* ---------------------------------------------------------------- full attention
+ * The step between the fused QKV projection and the output projection.  The reference has none (its
+ * full-attention layer ends at that projection), so names and layouts here are this library's own:
+ *
+ *   - a request has a row of the block table, int32 [table_rows, max_pages]: page of its tokens
+ *     [k * page_tokens, (k + 1) * page_tokens).  page_tokens is a power of two from 16 to 2^20;
+ *   - key and value cache planes are BF16 with element (page, token, head, d) at
+ *     page * page_stride + token * cache_token_stride + head * cache_head_stride + d, so that
+ *     [pages, tokens, heads, d], [pages, heads, tokens, d] and planes that hold both in turn all fit;
+ *   - a slot is page * page_tokens + place in the page, -1 for a row that is not stored;
+ *   - head_dim is 128 or 256; query head h belongs to key/value head h / (q_heads / kv_heads), at most
+ *     128 query heads to one;
+ *   - strides count BF16 values and are multiples of 8; planes start on 16 bytes.
+ * The context's device is made current during the call. */
+
+/* One step's block table rows, slots, positions and lengths.  Request r (row request_rows[r], or r when
+ * that is NULL; rows differ) appends new_tokens[r] >= 0 tokens to lengths[row]; pages it lacks come off
+ * the top of the stack free_pages[0 .. free_count), in request order, and are entered in its row.
+ *   starts        [requests + 1]  first token row of each request, and the sum
+ *   kv_lengths    [requests]      lengths with the new tokens
+ *   positions     [max_tokens]    position of every token row (0 behind the last)
+ *   slots         [max_tokens]    its place in the cache (-1 behind the last)
+ *   lengths_output, free_count_output: the new values; may be the planes they were read from.
+ * A step that does not fit -- a row out of range or given twice, too few free pages, more than max_tokens
+ * tokens, more tokens than max_pages hold -- changes nothing: starts and kv_lengths are zero, slots -1,
+ * and the status word says TK100_DEVICE_BAD_ARGUMENT.  requests <= 4096, table_rows <= 262144,
+ * max_pages * page_tokens <= 2^30; free_capacity = entries of the stack. */
+TK100_API tk100_status tk100_page_plan(tk100_ctx* ctx, tk100_stream stream, int requests, int table_rows,
+                                       int max_pages, int page_tokens, int max_tokens, int free_capacity,
+                                       const int32_t* request_rows, const int32_t* new_tokens,
+                                       const int32_t* lengths, int32_t* lengths_output, int32_t* block_table,
+                                       const int32_t* free_pages, const int32_t* free_count,
+                                       int32_t* free_count_output, int32_t* starts, int32_t* kv_lengths,
+                                       int32_t* positions, int64_t* slots);
+
+/* Gives the pages of requests that ended back: pushed onto the stack in request order, a request's in the
+ * order of its row, whose entries stay as they are; the requests' lengths become 0.  Refused as above
+ * where a row is out of range or given twice, or the stack has no room. */
+TK100_API tk100_status tk100_page_release(tk100_ctx* ctx, tk100_stream stream, int requests, int table_rows,
+                                          int max_pages, int page_tokens, int free_capacity,
+                                          const int32_t* request_rows, const int32_t* lengths,
+                                          int32_t* lengths_output, const int32_t* block_table,
+                                          int32_t* free_pages, const int32_t* free_count,
+                                          int32_t* free_count_output);
+
+/* Rotary positions with several axes on queries and keys, with what surrounds them, in one launch.  A head
+ * is normalised when its norm weight w [head_dim] is given, y = x / sqrt(mean(x^2) + eps) * (1 + w) with the
+ * context's eps; then the pairs (y_i, y_{i + rotary_dim / 2}) turn by positions[pair_axes[i]][token] *
+ * frequencies[i], i < rotary_dim / 2; the other values pass.  positions is int32 [axes, tokens]; frequencies
+ * are doubles in radians per position (angles are formed in 64 bits); pair_axes NULL = axis 0 for all.
+ * rotary_dim is a multiple of 16 up to head_dim, axes 1 to 8.
+ * Queries go to query_output [tokens, q_heads, head_dim]; keys to key_output [tokens, kv_heads, head_dim]
+ * (may be NULL when there is a cache) and, with the untouched values, to slots[token] of the cache (both
+ * planes NULL = no cache; a negative slot is skipped, one behind the last page is skipped and reported).
+ * No two tokens have the same slot.  An output may be the plane it is computed from where that has its
+ * layout; other overlaps are refused. */
+TK100_API tk100_status tk100_rotary_cache(tk100_ctx* ctx, tk100_stream stream, int tokens, int q_heads,
+                                          int kv_heads, int head_dim, int rotary_dim, int axes,
+                                          const double* frequencies, const uint8_t* pair_axes,
+                                          const int32_t* positions, const uint16_t* query,
+                                          int query_token_stride, int query_head_stride, const uint16_t* key,
+                                          const uint16_t* value, int kv_token_stride, int kv_head_stride,
+                                          const uint16_t* query_norm, const uint16_t* key_norm,
+                                          uint16_t* query_output, uint16_t* key_output, uint16_t* key_cache,
+                                          uint16_t* value_cache, int pages, int page_tokens, int page_stride,
+                                          int cache_token_stride, int cache_head_stride, const int64_t* slots);
+
+/* Bytes of the workspace of one attention launch: zeroed once by the caller, left as it was by every launch
+ * (zero it again after a wait that ran out).  Launches that may run at the same time -- on two streams, in
+ * two captured graphs -- need a workspace each. */
+TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_dim);
+
+/* Causal attention of new tokens over a paged cache, from one token per sequence (decode) to whole chunks.
+ * Sequence s has token rows starts[s] .. starts[s + 1] of `tokens`, its keys are the first kv_lengths[s] of
+ * its block table row (request_rows[s], or s when that is NULL), the new tokens' own included; with q new
+ * tokens over k keys token i sees keys 0 .. k - q + i.  A token that sees none gets zeros.
+ *   output[token][head] = softmax(scale * q . K) V, times sigmoid(gate[token][head]) when gate is given
+ * (the queries' strides).  output is [tokens, q_heads, head_dim]; rows outside the sequences are left as
+ * they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
+ * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used. */
+TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
+                                             int q_heads, int kv_heads, int head_dim, const int32_t* starts,
+                                             const int32_t* kv_lengths, const uint16_t* query,
+                                             const uint16_t* gate, int query_token_stride,
+                                             int query_head_stride, const uint16_t* key_cache,
+                                             const uint16_t* value_cache, int pages, int page_tokens,
+                                             int page_stride, int cache_token_stride, int cache_head_stride,
+                                             const int32_t* block_table, int table_rows, int max_pages,
+                                             const int32_t* request_rows, float scale, void* workspace,
+                                             uint16_t* output);
+
+/* The same over whole prompts packed one behind the other: keys and values are rows of the same tokens. */
+TK100_API tk100_status tk100_prompt_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
+                                              int q_heads, int kv_heads, int head_dim, const int32_t* starts,
+                                              const uint16_t* query, const uint16_t* gate,
+                                              int query_token_stride, int query_head_stride,
+                                              const uint16_t* key, const uint16_t* value, int kv_token_stride,
+                                              int kv_head_stride, float scale, void* workspace,
+                                              uint16_t* output);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

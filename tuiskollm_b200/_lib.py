@@ -88,6 +88,15 @@ SIGNATURES = {
     "tk100_peer_sum_bytes": (C.c_size_t, [C.c_size_t, _i]),
     "tk100_peer_sum_bf16": (_i, [_vp, _vp, C.c_size_t, C.c_size_t, _i, _i, _vp,
                                  C.POINTER(C.c_uint64), _vp]),
+    "tk100_page_plan": (_i, [_vp, _vp] + [_i] * 6 + [_vp] * 12),
+    "tk100_page_release": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 7),
+    "tk100_rotary_cache": (_i, [_vp, _vp] + [_i] * 6 + [_vp] * 4 + [_i] * 2 + [_vp] * 2 + [_i] * 2 + [_vp] * 6
+                           + [_i] * 5 + [_vp]),
+    "tk100_attention_workspace_bytes": (C.c_size_t, [_vp, _i]),
+    "tk100_paged_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 4 + [_i] * 2 + [_vp] * 2 + [_i] * 5
+                              + [_vp, _i, _i, _vp, C.c_float, _vp, _vp]),
+    "tk100_prompt_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 3 + [_i] * 2 + [_vp] * 2 + [_i] * 2
+                               + [C.c_float, _vp, _vp]),
     "tk100_fp8_projection_static": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, C.c_char_p,
                                          C.c_size_t]),
     "tk100_fp8_projection_static_status": (_i, [_vp, C.POINTER(C.c_uint32)]),

@@ -1,0 +1,768 @@
+// Causal attention with grouped heads over a paged key/value cache or over packed prompt rows.
+//
+// Sequence s has q new tokens and k keys (k = q for a prompt); its token i sees keys 0 .. k - q + i:
+//     o_i = sum_j softmax_j(scale * q_i . k_j) v_j,   optionally times sigmoid(gate_i);
+// a token that sees nothing (k - q + i < 0) gets zeros.
+//
+// Tiles.  The G query heads that share a key/value head are rows of one tile: row r = token r / G, head
+// r % G, floor(128 / G) whole tokens, so a decoded token's heads read the cache once and a prompt's diagonal
+// tile wastes 128 / G keys instead of 128.  A tile walks over its keys 128 at a time:
+//     S = Q K^T (tcgen05, both from shared memory) -> TMEM, two buffers
+//     P = exp2(scale log2e (S - m)) -> BF16 into the first half of S's columns
+//     O += P V (tcgen05, P from TMEM, V from shared memory) -> TMEM
+// m is the row's reference maximum: it follows the running maximum only when that has grown by more than 2^8,
+// so O is rescaled in TMEM a few times per row, not per tile, and P stays below 2^8, where BF16 and the
+// fp32 sum of P lose nothing.  P is rounded to BF16 (half a step 2^-9 each, the tensor core's operand type);
+// sums, maxima, O and the join of split rows are fp32.
+//
+// Roles, ten warps: TMA producer; MMA issuer; four softmax warps (thread = row); four epilogue warps, which
+// read O, normalise, gate and store while the softmax warps are on the next tile.  S of tile j + 1 is issued
+// before P V of tile j, so that the tensor pipe works during the softmax of j.  K arrives in units of 128 keys x
+// 64 values and V in units of 8192 values (32 or 64 keys), 16 KB each, one ring for both; a unit is read where
+// the page of the block table says, page by page.
+//
+// Work split.  All tiles of a launch in order (sequence, key/value head, tile) form one line of 128-key
+// steps, and each CTA (one per SM) takes an equal stretch of the line, wherever tiles begin and end.  A tile
+// whose steps lie in several CTAs is joined: each leaves its fp32 O, m and sum in the workspace, takes the
+// tile's ticket, and the CTA that draws the last one adds the parts in order of their keys (the same
+// bits whoever is last) and stores.  The lengths stay on the device: every CTA sums the tile counts up for
+// itself, so a captured launch follows them.
+#include "common.cuh"
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace tk100 {
+namespace {
+
+constexpr int kRows = 128;   // rows of a tile
+constexpr int kKeys = 128;   // keys of a step
+constexpr int kThreads = 320;
+constexpr int kUnit = 16384;  // bytes of a ring stage
+
+template <int D>
+struct Shape {
+  static constexpr int CHUNKS = D / 64;                    // 128-byte columns of a row
+  static constexpr int V_KEYS = kUnit / (2 * D);           // keys of a V unit: 32 or 64
+  static constexpr int V_UNITS = kKeys / V_KEYS;
+  static constexpr int STAGES = D == 256 ? 10 : 12;
+  static constexpr int SHARED = kRows * 2 * D + STAGES * kUnit + 1024;
+};
+
+// ---------------------------------------------------------------- the line of steps
+
+// Sum over k < n of floor((a k + b) / m): the lattice points under a line, by the Euclidean algorithm on (a, m).
+__device__ __forceinline__ long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  long long sum = 0;
+  while (n > 0) {
+    if (a >= m) {
+      sum += static_cast<long long>(n) * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += static_cast<long long>(n) * (b / m);
+      b %= m;
+    }
+    const unsigned top = a * n + b;  // below the number of keys
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+struct Sequence {
+  int start, q, kv;  // first token row, new tokens, keys
+};
+
+__device__ __forceinline__ Sequence read_sequence(const AttentionParams& p, int s) {
+  Sequence r;
+  r.start = min(max(p.starts[s], 0), p.tokens);
+  r.q = min(max(p.starts[s + 1], r.start), p.tokens) - r.start;
+  r.kv = r.q;
+  if (p.kv_lengths) r.kv = min(max(p.kv_lengths[s], 0), p.key_capacity);
+  return r;
+}
+
+// Steps of tile i: at least one, so that a tile which sees nothing still stores its zeros.
+__device__ __forceinline__ int tile_limit(const AttentionParams& p, const Sequence& s, int i) {
+  return max(s.kv - s.q + min((i + 1) * p.tile_tokens, s.q), 0);  // keys its last token sees
+}
+__device__ __forceinline__ int tile_steps(const AttentionParams& p, const Sequence& s, int i) {
+  return max((tile_limit(p, s, i) + kKeys - 1) / kKeys, 1);
+}
+__device__ __forceinline__ int tile_count(const AttentionParams& p, const Sequence& s) {
+  return (s.q + p.tile_tokens - 1) / p.tile_tokens;
+}
+
+// Steps of the first i tiles of one key/value head.
+__device__ __forceinline__ long long steps_before(const AttentionParams& p, const Sequence& s, int i) {
+  const int tiles = tile_count(p, s);
+  long long sum = 0;
+  int full = i;  // tiles that end at their own (i + 1) tile_tokens
+  if (i == tiles && i > 0) {
+    sum = tile_steps(p, s, i - 1);
+    --full;
+  }
+  const int ahead = s.kv - s.q;  // keys in front of the first new token
+  // tiles of one step: ahead + (j + 1) tile_tokens <= 128
+  const int ones = min(max(ahead > kKeys ? 0 : (kKeys - ahead) / p.tile_tokens, 0), full);
+  sum += ones;
+  if (full > ones) {
+    const int b = ahead + (ones + 1) * p.tile_tokens + kKeys - 1;  // > 2 * 128 - 1
+    sum += floor_sum(static_cast<unsigned>(full - ones), kKeys, static_cast<unsigned>(p.tile_tokens), static_cast<unsigned>(b));
+  }
+  return sum;
+}
+
+struct Start {
+  int sequence, head, tile, step;  // where this CTA's stretch begins
+  int ctas;                        // CTAs that have work
+  long long total, first, last;    // steps of the launch; this CTA's [first, last)
+};
+
+__device__ __forceinline__ long long cta_first(long long total, int ctas, int c) { return c * total / ctas; }
+// CTA whose stretch holds step u.
+__device__ __forceinline__ int cta_of(long long total, int ctas, long long u) {
+  return static_cast<int>(((u + 1) * ctas - 1) / total);
+}
+
+// One tile, or the part of it that this CTA works on.
+struct Item {
+  Sequence seq;
+  int sequence, head, tile;
+  int first, last, steps;  // its steps [first, last) of `steps`
+  int limit;               // keys its last token sees
+  int tokens;              // tokens of the tile
+  long long line;          // place of its step 0 in the line
+};
+
+struct Walk {
+  int sequence, head, tile, step;
+  long long at, end;
+  Sequence seq;
+  int tiles;
+
+  __device__ __forceinline__ Walk(const AttentionParams& p, const Start& s)
+      : sequence(s.sequence), head(s.head), tile(s.tile), step(s.step), at(s.first), end(s.last) {
+    seq = {0, 0, 0};
+    tiles = 0;
+    if (at < end) {
+      seq = read_sequence(p, sequence);
+      tiles = tile_count(p, seq);
+    }
+  }
+  __device__ __forceinline__ bool next(const AttentionParams& p, Item* it) {
+    if (at >= end) return false;
+    while (tile >= tiles) {  // the next head, or the next sequence that has tokens
+      tile = 0;
+      if (tiles == 0 || ++head == p.kv_heads) {
+        head = 0;
+        if (++sequence >= p.sequences) return false;
+        seq = read_sequence(p, sequence);
+        tiles = tile_count(p, seq);
+      }
+    }
+    it->seq = seq;
+    it->sequence = sequence;
+    it->head = head;
+    it->tile = tile;
+    it->steps = tile_steps(p, seq, tile);
+    it->limit = tile_limit(p, seq, tile);
+    it->tokens = min(p.tile_tokens, seq.q - tile * p.tile_tokens);
+    it->first = step;
+    it->last = static_cast<int>(min(static_cast<long long>(it->steps), step + (end - at)));
+    it->line = at - step;
+    at += it->last - it->first;
+    step = 0;
+    ++tile;
+    return true;
+  }
+};
+
+struct Scratch {
+  long long warp_sums[kThreads / 32];
+  Start start;
+};
+
+__device__ __forceinline__ void find_start(const AttentionParams& p, Scratch& sh) {
+  const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
+  const int run = (p.sequences + kThreads - 1) / kThreads;
+  const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Sequence q = read_sequence(p, s);
+    mine += steps_before(p, q, tile_count(p, q)) * p.kv_heads;
+    if (blockIdx.x == 0 && (q.start != p.starts[s] || q.start + q.q != p.starts[s + 1] || (p.kv_lengths && q.kv != p.kv_lengths[s])))
+      atomicOr(p.status, STATUS_BAD_ARGUMENT);  // lengths outside the planes are cut to them
+  }
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 31) sh.warp_sums[warp] = sum;
+  if (t == 0) sh.start = {};
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sh.warp_sums[w];
+    total += sh.warp_sums[w];
+  }
+  before += sum - mine;
+  if (total == 0) return;
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + p.min_steps - 1) / p.min_steps));
+  const int c = static_cast<int>(blockIdx.x);
+  if (c < ctas) {
+    const long long first = cta_first(total, ctas, c), last = cta_first(total, ctas, c + 1);
+    if (before <= first && first < before + mine) {
+      long long rest = first - before;
+      int s = s0;
+      Sequence q = read_sequence(p, s);
+      long long steps = steps_before(p, q, tile_count(p, q));
+      while (rest >= steps * p.kv_heads) {
+        rest -= steps * p.kv_heads;
+        q = read_sequence(p, ++s);
+        steps = steps_before(p, q, tile_count(p, q));
+      }
+      Start r;
+      r.sequence = s;
+      r.head = static_cast<int>(rest / steps);
+      rest -= r.head * steps;
+      int low = 0, high = tile_count(p, q);  // steps_before(low) <= rest < steps_before(high)
+      while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (steps_before(p, q, middle) <= rest) {
+          low = middle;
+        } else {
+          high = middle;
+        }
+      }
+      r.tile = low;
+      r.step = static_cast<int>(rest - steps_before(p, q, low));
+      r.ctas = ctas;
+      r.total = total;
+      r.first = first;
+      r.last = last;
+      sh.start = r;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// One row of S; keys it does not see read as -infinity.
+__device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int seen, uint32_t (&s)[kKeys]) {
+#pragma unroll
+  for (int k = 0; k < kKeys; k += 32) tmem_ld32(taddr + k, s + k);
+  tmem_ld_wait();
+  if (masked) {
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) s[k] = k < seen ? s[k] : 0xff800000u;
+  }
+}
+
+// ------------------------------------------------------------------------- the kernel
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q1,
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ AttentionParams p) {
+  using S = Shape<D>;
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ uint8_t dynamic[];
+  uint8_t* smem_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = smem_q + kRows * 2 * D;
+
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done, o_full, o_free, stats_full, drained;
+  __shared__ uint32_t tmem_base;
+  __shared__ float row_max[kRows], row_sum[kRows];
+  __shared__ int last_part;
+  __shared__ Scratch scratch;
+
+  const int warp = warp_index(), lane = static_cast<int>(threadIdx.x) & 31;
+
+  if (warp == 0 && elect_one()) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(&pv_done, 1);
+    mbar_init(&o_full, 1);
+    mbar_init(&o_free, 4);
+    mbar_init(&stats_full, 4);
+    mbar_init(&drained, 1);
+    fence_mbar_init();
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_trigger();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const uint32_t tmem_o = tmem + 2 * kKeys;
+
+  find_start(p, scratch);
+  const Start start = scratch.start;
+  Walk walk(p, start);
+  Item it;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    int stage = 0, item = 0;
+    uint32_t phase = 1;  // parity to wait for on `empty`: a fresh barrier's earlier phase
+    bool ok = true;
+    auto advance = [&]() {
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    };
+    while (ok && walk.next(p, &it)) {
+      if (item > 0) ok = mbar_wait(&q_empty, (item - 1) & 1, p.status);
+      if (!ok) break;
+      const int token = it.seq.start + it.tile * p.tile_tokens;
+      if (elect_one()) {
+        const bool one = it.tokens == 1;
+        const uint32_t bytes = static_cast<uint32_t>(p.group * (one ? 1 : p.tile_tokens) * 128);
+        mbar_arrive_expect_tx(&q_full, bytes * S::CHUNKS);
+        for (int c = 0; c < S::CHUNKS; ++c) {
+          tma_load_4d(smem_q + c * kRows * 128, one ? &map_q1 : &map_q, &q_full, 64 * c, 0, it.head, token);
+        }
+      }
+      __syncwarp();
+      ++item;
+
+      const int row = p.block_table ? (p.table_rows ? p.table_rows[it.sequence] : it.sequence) : 0;
+      const bool row_ok = row >= 0 && row < p.table_row_count;
+      const int per_step = p.block_table ? max(kKeys >> p.page_shift, 1) : 0;  // pages of a step
+      // lane l holds the page of keys [l * page tokens, ...) of the step
+      auto pages_of = [&](int j) -> int {
+        int id = -1;
+        if (lane < per_step) {
+          const int index = p.page_shift >= 7 ? j >> (p.page_shift - 7) : j * per_step + lane;
+          const bool needed = j * kKeys + (lane << p.page_shift) < it.limit;
+          if (needed) {
+            if (row_ok && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
+            if (id < 0 || id >= p.pages) {
+              id = -1;  // outside the plane: TMA fills zeros
+              atomicOr(p.status, STATUS_BAD_ARGUMENT);
+            }
+          }
+        }
+        return id;
+      };
+      // one unit: `rows` keys from key `key` of step j on, `chunks` 64-value columns from `chunk` on
+      auto load_unit = [&](const CUtensorMap* map, int ids, int j, int key, int rows, int chunk, int chunks) {
+        const int keys = min(rows, it.limit - j * kKeys - key);  // of these `keys` exist
+        const int box = p.block_table ? min(rows, 1 << p.page_shift) : rows;
+        const int boxes = max((keys + box - 1) / box, 1);
+        uint8_t* to = ring + stage * kUnit;
+        if (elect_one()) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * box * chunks * 128));
+        __syncwarp();
+        for (int b = 0; b < boxes; ++b) {
+          const int at = key + b * box;  // within the step
+          int page = 0, within;
+          if (p.block_table) {
+            page = __shfl_sync(0xffffffffu, ids, p.page_shift >= 7 ? 0 : at >> p.page_shift);
+            within = (j * kKeys + at) & ((1 << p.page_shift) - 1);
+          } else {
+            within = it.seq.start + j * kKeys + at;
+          }
+          if (elect_one()) {
+            for (int c = 0; c < chunks; ++c) {
+              tma_load_4d(to + c * rows * 128 + b * box * 128, map, &full[stage], 64 * (chunk + c), within, it.head, page);
+            }
+          }
+          __syncwarp();
+        }
+      };
+      int ids = pages_of(it.first), ids_before = 0;
+      // K of step j, then V of step j - 1: the order in which the MMA warp asks for them
+      for (int j = it.first; ok && j <= it.last; ++j) {
+        if (j < it.last) {
+          for (int c = 0; ok && c < S::CHUNKS; ++c) {
+            ok = mbar_wait(&empty[stage], phase, p.status);
+            if (ok) {
+              load_unit(&map_k, ids, j, 0, kKeys, c, 1);
+              advance();
+            }
+          }
+        }
+        if (j > it.first) {
+          const int v = j - 1;
+          const int keys = it.limit - v * kKeys;
+          for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
+            ok = mbar_wait(&empty[stage], phase, p.status);
+            if (ok) {
+              load_unit(&map_v, ids_before, v, u * S::V_KEYS, S::V_KEYS, 0, S::CHUNKS);
+              advance();
+            }
+          }
+        }
+        ids_before = ids;
+        if (j + 1 < it.last) ids = pages_of(j + 1);
+      }
+    }
+    if (!ok) {
+      // what was asked for lands before the CTA's shared memory is somebody else's
+      for (int n = 0; item > 0 && n < 200000 && !mbar_try_wait(&q_full, (item - 1) & 1); ++n) {
+      }
+      for (int i = 0; i < STAGES; ++i) {
+        for (int n = 0; n < 200000 && !mbar_try_wait(&full[stage], phase); ++n) {
+        }
+        advance();
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------- MMA
+    constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys, false);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, D, true);
+    int stage = 0, item = 0;
+    uint32_t phase = 0;
+    int n = 0;  // steps so far
+    bool ok = true;
+    auto advance = [&]() {
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    };
+    const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
+    auto scores = [&](int buffer) {  // S[buffer] = Q K^T
+      for (int c = 0; ok && c < S::CHUNKS; ++c) {
+        ok = mbar_wait(&full[stage], phase, p.status);
+        if (!ok) return;
+        if (elect_one()) {
+          const uint64_t a = umma_desc_sw128(q_addr + c * kRows * 128), b = umma_desc_sw128(ring_addr + stage * kUnit);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem + buffer * kKeys, a + 2 * k, b + 2 * k, idesc_s, c > 0 || k > 0);
+          umma_commit(&empty[stage]);
+        }
+        __syncwarp();
+        advance();
+      }
+      if (elect_one()) umma_commit(&s_full[buffer]);
+      __syncwarp();
+    };
+    while (ok && walk.next(p, &it)) {
+      ok = mbar_wait(&q_full, item & 1, p.status);
+      if (!ok) break;
+      scores(n & 1);
+      for (int j = it.first; ok && j < it.last; ++j, ++n) {
+        const int buffer = n & 1;
+        if (j + 1 < it.last) {
+          scores(buffer ^ 1);
+          if (!ok) break;
+        }
+        if (j + 1 >= it.last) {
+          if (elect_one()) umma_commit(&q_empty);  // every product with Q is issued
+          __syncwarp();
+        }
+        if (j == it.first && item > 0) ok = mbar_wait(&o_free, (item - 1) & 1, p.status);
+        if (ok) ok = mbar_wait(&p_full[buffer], (n >> 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int keys = it.limit - j * kKeys;
+        for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
+          ok = mbar_wait(&full[stage], phase, p.status);
+          if (!ok) break;
+          uint8_t* unit = ring + stage * kUnit;
+          const int mine = min(max(keys - u * S::V_KEYS, 0), S::V_KEYS);  // keys of this unit that count
+          const int slices = max((mine + 15) / 16, 1);
+          if (mine < slices * 16) {
+            // P is zero for the keys behind the last, but what lies there may be no number: zeros
+            for (int i = lane; i < (slices * 16 - mine) * S::CHUNKS * 8; i += 32) {
+              const int r = mine + i / (S::CHUNKS * 8), c = (i / 8) % S::CHUNKS, piece = i % 8;
+              *reinterpret_cast<uint4*>(unit + c * S::V_KEYS * 128 + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (elect_one()) {
+            const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * kUnit, S::V_KEYS * 128);
+            for (int k = 0; k < slices; ++k) {
+              umma_bf16_ta(tmem_o, tmem + buffer * kKeys + u * (S::V_KEYS / 2) + 8 * k, b + (2048 >> 4) * k, idesc_o,
+                           j > it.first || u > 0 || k > 0);
+            }
+            umma_commit(&empty[stage]);
+          }
+          __syncwarp();
+          advance();
+        }
+        if (ok && elect_one()) {
+          umma_commit(&pv_done);
+          if (j + 1 >= it.last) umma_commit(&o_full);
+        }
+        __syncwarp();
+      }
+      ++item;
+    }
+    if (!ok) {
+      if (elect_one()) umma_commit(&drained);
+      __syncwarp();
+      for (int i = 0; i < 200000 && !mbar_try_wait(&drained, 0); ++i) {
+      }
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ----------------------------------------------------------------- softmax
+    const int quadrant = warp & 3;  // the TMEM lanes this warp may touch
+    const int r = quadrant * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+    const float c = p.scale_log2;
+    int n = 0, item = 0;
+    bool ok = true;
+    while (ok && walk.next(p, &it)) {
+      const int rows = it.tokens * p.group;
+      const bool active = quadrant * 32 < rows;
+      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens;
+      const int limit = ahead + r / p.group + 1;  // keys this row sees
+      float reference = -INFINITY, sum = 0.0f;
+      for (int j = it.first; j < it.last; ++j, ++n) {
+        const int buffer = n & 1;
+        ok = mbar_wait(&s_full[buffer], (n >> 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (active) {
+          uint32_t s[kKeys];
+          const uint32_t at = tmem + buffer * kKeys + lanes;
+          const int seen = limit - j * kKeys;
+          const bool masked = __any_sync(0xffffffffu, seen < kKeys);
+          load_scores(at, masked, seen, s);
+          float top = __uint_as_float(s[0]);
+#pragma unroll
+          for (int k = 1; k < kKeys; ++k) top = fmaxf(top, __uint_as_float(s[k]));
+          if (j == it.first) {
+            reference = top;
+          } else {
+            const bool grown = (top - reference) * c > 8.0f;
+            if (__any_sync(0xffffffffu, grown)) {
+              // O of the steps before this one is complete, and none is added until P of this one is
+              ok = mbar_wait(&pv_done, (n - 1) & 1, p.status);
+              if (!ok) break;
+              tc_fence_after_sync();
+              const float alpha = grown ? exp2_approx((reference - top) * c) : 1.0f;
+              if (grown) reference = top;
+              sum *= alpha;
+#pragma unroll 1
+              for (int k = 0; k < D; k += 32) {
+                uint32_t o[32];
+                tmem_ld32(tmem_o + lanes + k, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st32(tmem_o + lanes + k, o);
+              }
+              tmem_st_wait();
+              load_scores(at, masked, seen, s);  // rather than 128 registers kept over the wait
+            }
+          }
+          const float shift = reference == -INFINITY ? 0.0f : reference * c;
+          float part = 0.0f;
+#pragma unroll
+          for (int k = 0; k < kKeys; k += 2) {
+            const float a = exp2_approx(fmaf(__uint_as_float(s[k]), c, -shift));
+            const float b = exp2_approx(fmaf(__uint_as_float(s[k + 1]), c, -shift));
+            part += a + b;
+            s[k / 2] = pack_bf16x2(a, b);
+          }
+          sum += part;
+          tmem_st32(at, s);
+          tmem_st32(at + 32, s + 32);
+          tmem_st_wait();
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buffer]);
+      }
+      if (!ok) break;
+      if (item > 0) ok = mbar_wait(&o_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
+      if (!ok) break;
+      row_max[r] = reference == -INFINITY ? -INFINITY : reference * c;
+      row_sum[r] = sum;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stats_full);
+      ++item;
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 192;
+    const int r = quadrant * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+    int item = 0;
+    bool ok = true;  // a warp whose wait ran out still takes part in the barriers of the four
+    while (walk.next(p, &it)) {
+      ok = ok && mbar_wait(&stats_full, item & 1, p.status) && mbar_wait(&o_full, item & 1, p.status);
+      tc_fence_after_sync();
+      const float m = row_max[r], sum = row_sum[r];
+      const int rows = it.tokens * p.group;
+      const int tile_token = it.seq.start + it.tile * p.tile_tokens;  // first token row
+      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens;
+      auto gate_row = [&](int row) {
+        return p.gate + static_cast<size_t>(tile_token + row / p.group) * p.query_token_stride +
+               static_cast<size_t>(it.head * p.group + row % p.group) * p.query_head_stride;
+      };
+      auto output_row = [&](int row) {
+        return p.output + (static_cast<size_t>(tile_token + row / p.group) * p.q_heads + it.head * p.group + row % p.group) * D;
+      };
+      const bool whole = it.first == 0 && it.last == it.steps;
+      if (whole) {
+        const bool blind = ahead + r / p.group < 0;  // sees no key
+        const float scale = blind ? 0.0f : 1.0f / sum;
+        if (ok && quadrant * 32 < rows) {
+#pragma unroll 1
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + lanes + k, o);
+            tmem_ld_wait();
+            if (r < rows) {
+              uint16_t* out = output_row(r) + k;
+              const uint16_t* gate = p.gate ? gate_row(r) + k : nullptr;
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = blind ? 0.0f : __uint_as_float(o[e + i]) * scale;
+                if (gate) {
+                  const uint4 g = *reinterpret_cast<const uint4*>(gate + e);
+                  const uint32_t w[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = __fdividef(v[2 * i], 1.0f + exp2_approx(bf16x2_lo(w[i]) * -1.4426950408889634f));
+                    v[2 * i + 1] = __fdividef(v[2 * i + 1], 1.0f + exp2_approx(bf16x2_hi(w[i]) * -1.4426950408889634f));
+                  }
+                }
+                *reinterpret_cast<uint4*>(out + e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                                pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+              }
+            }
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free);
+      } else {
+        const int c0 = cta_of(start.total, start.ctas, it.line), c1 = cta_of(start.total, start.ctas, it.line + it.steps - 1);
+        // a CTA's first item goes to its slot 0, a later one (then its last) to slot 1
+        const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (item == 0 ? 0 : 1);
+        float* part = p.parts + slot * kRows * D;
+        if (ok && quadrant * 32 < rows) {
+#pragma unroll 1
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + lanes + k, o);
+            tmem_ld_wait();
+            if (r < rows) {
+              float* to = part + static_cast<size_t>(r) * D + k;
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<uint4*>(to + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+          if (r < rows) p.part_stats[slot * kRows + r] = make_float2(m, sum);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free);
+        __threadfence();
+        named_barrier(1, 128);
+        if (thread == 0) last_part = atomicAdd(&p.tickets[c0], 1u) == static_cast<unsigned>(c1 - c0);
+        named_barrier(1, 128);
+        if (last_part) {
+          __threadfence();
+          const size_t slot0 = 2 * static_cast<size_t>(c0) + (cta_first(start.total, start.ctas, c0) == it.line ? 0 : 1);
+          for (int i = thread; i < rows * (D / 4); i += 128) {
+            const int row = i / (D / 4), column = i % (D / 4) * 4;
+            float top = -INFINITY;
+            for (int k = c0; k <= c1; ++k) {
+              const size_t at = k == c0 ? slot0 : 2 * static_cast<size_t>(k);
+              top = fmaxf(top, __ldcg(&p.part_stats[at * kRows + row]).x);
+            }
+            float total = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k = c0; k <= c1; ++k) {
+              const size_t at = k == c0 ? slot0 : 2 * static_cast<size_t>(k);
+              const float2 stats = __ldcg(&p.part_stats[at * kRows + row]);
+              // a part without a key of this row has nothing to add, whatever its O holds
+              if (stats.x == -INFINITY && stats.y == 0.0f) continue;
+              const float w = exp2_approx(stats.x - top);
+              const float4 o = __ldcg(reinterpret_cast<const float4*>(p.parts + (at * kRows + row) * D + column));
+              total = fmaf(stats.y, w, total);
+              acc.x = fmaf(o.x, w, acc.x);
+              acc.y = fmaf(o.y, w, acc.y);
+              acc.z = fmaf(o.z, w, acc.z);
+              acc.w = fmaf(o.w, w, acc.w);
+            }
+            const bool blind = ahead + row / p.group < 0;
+            const float scale = 1.0f / total;
+            float v[4] = {acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale};
+            if (p.gate) {
+              const uint2 g = *reinterpret_cast<const uint2*>(gate_row(row) + column);
+              v[0] = __fdividef(v[0], 1.0f + exp2_approx(bf16x2_lo(g.x) * -1.4426950408889634f));
+              v[1] = __fdividef(v[1], 1.0f + exp2_approx(bf16x2_hi(g.x) * -1.4426950408889634f));
+              v[2] = __fdividef(v[2], 1.0f + exp2_approx(bf16x2_lo(g.y) * -1.4426950408889634f));
+              v[3] = __fdividef(v[3], 1.0f + exp2_approx(bf16x2_hi(g.y) * -1.4426950408889634f));
+            }
+            if (blind) v[0] = v[1] = v[2] = v[3] = 0.0f;
+            *reinterpret_cast<uint2*>(output_row(row) + column) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+          }
+          if (thread == 0) p.tickets[c0] = 0u;
+        }
+        named_barrier(1, 128);  // `last_part` is written again
+      }
+      ++item;
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+cudaError_t attention_prepare() {
+  cudaError_t e = cudaFuncSetAttribute(attention_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<256>::SHARED);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<128>::SHARED);
+}
+
+int attention_value_box(int dim) { return kUnit / (2 * dim); }
+
+cudaError_t launch_attention(cudaStream_t stream, int dim, int ctas, const CUtensorMap& map_q, const CUtensorMap& map_q1,
+                             const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p) {
+  if (dim == 256) {
+    return launch_kernel(attention_kernel<256>, dim3(ctas), dim3(kThreads), Shape<256>::SHARED, stream, map_q, map_q1, map_k, map_v, p);
+  }
+  return launch_kernel(attention_kernel<128>, dim3(ctas), dim3(kThreads), Shape<128>::SHARED, stream, map_q, map_q1, map_k, map_v, p);
+}
+
+}  // namespace tk100

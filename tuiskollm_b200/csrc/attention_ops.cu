@@ -1,0 +1,327 @@
+// Operator layer of the full-attention step: page plans, rotary positions with cache stores, attention.
+#include "ops.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace tk100 {
+
+namespace {
+
+#define TK100_TRY(expr)                  \
+  do {                                   \
+    Status _s = (expr);                  \
+    if (_s != TK100_OK) return _s;       \
+  } while (0)
+
+constexpr int kMaxTokens = 1 << 24;          // rows of one launch
+constexpr int kMaxSequences = 1 << 20;
+constexpr long long kMaxKeys = 1ll << 30;    // keys of one sequence
+constexpr int kAttentionRows = 128;          // rows of a tile (attention.cu)
+constexpr size_t kTicketBytes = 4096;
+
+// The caller's current device is the context's during a launch, whatever it was.
+class DeviceScope {
+ public:
+  DeviceScope(Context& ctx) : ctx_(ctx) {
+    status_ = cudaGetDevice(&before_);
+    if (status_ == cudaSuccess && before_ != ctx.config().device) {
+      status_ = cudaSetDevice(ctx.config().device);
+      moved_ = status_ == cudaSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  Status status() { return ctx_.check(status_, "making the context's device current"); }
+
+ private:
+  Context& ctx_;
+  cudaError_t status_;
+  int before_ = 0;
+  bool moved_ = false;
+};
+
+Status refuse(Context& ctx, const char* what, const std::string& message) {
+  return ctx.fail(TK100_ERR_LAUNCH, std::string("[gpu.launch] ") + what + ": " + message);
+}
+
+Status plane(Context& ctx, const char* what, const char* name, const void* p, size_t alignment) {
+  if (p == nullptr) return refuse(ctx, what, std::string(name) + " plane is null");
+  if ((reinterpret_cast<uintptr_t>(p) & (alignment - 1)) != 0)
+    return refuse(ctx, what, std::string(name) + " plane is not " + std::to_string(alignment) + "-byte aligned");
+  return TK100_OK;
+}
+
+Status range(Context& ctx, const char* what, const char* name, long long v, long long low, long long high) {
+  if (v >= low && v <= high) return TK100_OK;
+  return refuse(ctx, what, std::string(name) + " " + std::to_string(v) + " is outside the admitted range " +
+                               std::to_string(low) + "..=" + std::to_string(high));
+}
+
+// Rows are read 16 bytes at a time: strides in whole groups of eight values.
+Status stride(Context& ctx, const char* what, const char* name, int v, int least) {
+  if (v >= least && v % 8 == 0) return TK100_OK;
+  return refuse(ctx, what, std::string(name) + " stride " + std::to_string(v) + " is not a multiple of 8 of at least " +
+                               std::to_string(least));
+}
+
+Status heads(Context& ctx, const char* what, int q_heads, int kv_heads, int head_dim) {
+  if (head_dim != 128 && head_dim != 256)
+    return refuse(ctx, what, "heads of " + std::to_string(head_dim) + " values are not admitted (128 or 256)");
+  TK100_TRY(range(ctx, what, "key/value head count", kv_heads, 1, 1024));
+  if (q_heads < kv_heads || q_heads % kv_heads != 0 || q_heads / kv_heads > kAttentionRows)
+    return refuse(ctx, what, std::to_string(q_heads) + " query heads do not share " + std::to_string(kv_heads) +
+                                 " key/value heads evenly, at most 128 each");
+  return TK100_OK;
+}
+
+Status cache_geometry(Context& ctx, const char* what, const CacheGeometry& g, int head_dim) {
+  TK100_TRY(range(ctx, what, "page count", g.pages, 1, 1 << 30));
+  if (g.page_tokens < 16 || g.page_tokens > (1 << 20) || (g.page_tokens & (g.page_tokens - 1)) != 0)
+    return refuse(ctx, what, "pages of " + std::to_string(g.page_tokens) + " tokens are not admitted (a power of two, 16 to 2^20)");
+  TK100_TRY(stride(ctx, what, "cache page", g.page_stride, head_dim));
+  TK100_TRY(stride(ctx, what, "cache token", g.token_stride, head_dim));
+  return stride(ctx, what, "cache head", g.head_stride, head_dim);
+}
+
+int log2_of(int power) {
+  int s = 0;
+  while ((1 << s) < power) ++s;
+  return s;
+}
+
+// [first, last) bytes that `tokens` rows of `heads` heads touch
+struct Span {
+  uintptr_t first, last;
+  Span(const uint16_t* p, long long tokens, long long token_stride, long long heads, long long head_stride, int dim)
+      : first(reinterpret_cast<uintptr_t>(p)),
+        last(first + 2 * static_cast<uintptr_t>((tokens - 1) * token_stride + (heads - 1) * head_stride + dim)) {}
+  bool meets(const Span& o) const { return first < o.last && o.first < last; }
+};
+
+}  // namespace
+
+// ---------------------------------------------------------------------- PagePlanOp
+
+Status PagePlanOp::check(const char* what, const PageParams& p) {
+  TK100_TRY(range(ctx_, what, "request count", p.requests, 1, kPageMaxRequests));
+  TK100_TRY(range(ctx_, what, "block table row count", p.table_rows, 1, kPageMaxRows));
+  TK100_TRY(range(ctx_, what, "pages per row", p.max_pages, 1, 1 << 30));
+  if (p.page_tokens < 16 || p.page_tokens > (1 << 20) || (p.page_tokens & (p.page_tokens - 1)) != 0)
+    return refuse(ctx_, what, "pages of " + std::to_string(p.page_tokens) + " tokens are not admitted (a power of two, 16 to 2^20)");
+  // more pages than that hold more keys than a sequence may have
+  if (static_cast<long long>(p.max_pages) * p.page_tokens > kMaxKeys)
+    return refuse(ctx_, what, "a block table row of " + std::to_string(p.max_pages) + " pages exceeds 2^30 tokens");
+  TK100_TRY(range(ctx_, what, "free page capacity", p.free_capacity, 1, 1 << 30));
+  TK100_TRY(plane(ctx_, what, "length", p.lengths, 4));
+  TK100_TRY(plane(ctx_, what, "length output", p.lengths_output, 4));
+  TK100_TRY(plane(ctx_, what, "block table", p.block_table, 4));
+  TK100_TRY(plane(ctx_, what, "free page", p.free_pages, 4));
+  TK100_TRY(plane(ctx_, what, "free count", p.free_count, 4));
+  return plane(ctx_, what, "free count output", p.free_count_output, 4);
+}
+
+Status PagePlanOp::launch(cudaStream_t stream, PageParams p) {
+  const char* what = "page plan";
+  TK100_TRY(check(what, p));
+  TK100_TRY(range(ctx_, what, "token capacity", p.max_tokens, 1, kMaxTokens));
+  TK100_TRY(plane(ctx_, what, "new token", p.new_tokens, 4));
+  TK100_TRY(plane(ctx_, what, "start", p.starts, 4));
+  TK100_TRY(plane(ctx_, what, "key length", p.kv_lengths, 4));
+  TK100_TRY(plane(ctx_, what, "position", p.positions, 4));
+  TK100_TRY(plane(ctx_, what, "slot", p.slots, 8));
+  p.status = ctx_.status_word();
+  DeviceScope device(ctx_);
+  TK100_TRY(device.status());
+  ctx_.count_launch();
+  return ctx_.check(launch_page(stream, p, false), "launching the page plan");
+}
+
+Status PagePlanOp::release(cudaStream_t stream, PageParams p) {
+  const char* what = "page release";
+  TK100_TRY(check(what, p));
+  p.status = ctx_.status_word();
+  p.max_tokens = p.requests;  // sets the CTA count only
+  DeviceScope device(ctx_);
+  TK100_TRY(device.status());
+  ctx_.count_launch();
+  return ctx_.check(launch_page(stream, p, true), "launching the page release");
+}
+
+// ------------------------------------------------------------------- RotaryCacheOp
+
+Status RotaryCacheOp::launch(cudaStream_t stream, int head_dim, RotaryParams p, const CacheGeometry& cache) {
+  const char* what = "rotary";
+  TK100_TRY(heads(ctx_, what, p.q_heads, p.kv_heads, head_dim));
+  TK100_TRY(range(ctx_, what, "token count", p.tokens, 1, kMaxTokens));
+  if (p.half < 8 || p.half % 8 != 0 || 2 * p.half > head_dim)
+    return refuse(ctx_, what, std::to_string(2 * p.half) + " rotated values are not admitted (a multiple of 16 up to the head's)");
+  TK100_TRY(range(ctx_, what, "position axis count", p.axes, 1, 8));
+  TK100_TRY(plane(ctx_, what, "frequency", p.frequencies, 8));
+  TK100_TRY(plane(ctx_, what, "position", p.positions, 4));
+  TK100_TRY(plane(ctx_, what, "query", p.query, 16));
+  TK100_TRY(plane(ctx_, what, "key", p.key, 16));
+  TK100_TRY(plane(ctx_, what, "query output", p.query_output, 16));
+  TK100_TRY(stride(ctx_, what, "query token", p.query_token_stride, head_dim));
+  TK100_TRY(stride(ctx_, what, "query head", p.query_head_stride, head_dim));
+  TK100_TRY(stride(ctx_, what, "key/value token", p.kv_token_stride, head_dim));
+  TK100_TRY(stride(ctx_, what, "key/value head", p.kv_head_stride, head_dim));
+  if (p.query_norm) TK100_TRY(plane(ctx_, what, "query norm", p.query_norm, 16));
+  if (p.key_norm) TK100_TRY(plane(ctx_, what, "key norm", p.key_norm, 16));
+  if (p.key_output) TK100_TRY(plane(ctx_, what, "key output", p.key_output, 16));
+  if (p.key_cache || p.value_cache) {
+    TK100_TRY(cache_geometry(ctx_, what, cache, head_dim));
+    TK100_TRY(plane(ctx_, what, "key cache", p.key_cache, 16));
+    TK100_TRY(plane(ctx_, what, "value cache", p.value_cache, 16));
+    TK100_TRY(plane(ctx_, what, "value", p.value, 16));
+    TK100_TRY(plane(ctx_, what, "slot", p.slots, 8));
+    p.pages = cache.pages;
+    p.page_shift = log2_of(cache.page_tokens);
+    p.page_stride = cache.page_stride;
+    p.cache_token_stride = cache.token_stride;
+    p.cache_head_stride = cache.head_stride;
+  } else if (!p.key_output) {
+    return refuse(ctx_, what, "rotated keys go nowhere: neither a key output nor a cache");
+  }
+  // An output may be the plane it is computed from, element for element; any other overlap would have one
+  // CTA write what another still reads.
+  const Span query(p.query, p.tokens, p.query_token_stride, p.q_heads, p.query_head_stride, head_dim);
+  const Span key(p.key, p.tokens, p.kv_token_stride, p.kv_heads, p.kv_head_stride, head_dim);
+  const Span q_out(p.query_output, p.tokens, static_cast<long long>(p.q_heads) * head_dim, p.q_heads, head_dim, head_dim);
+  const bool q_same = p.query_output == p.query && p.query_head_stride == head_dim &&
+                      p.query_token_stride == p.q_heads * head_dim;
+  if (q_out.meets(query) && !q_same) return refuse(ctx_, what, "the query output overlaps the queries");
+  if (q_out.meets(key)) return refuse(ctx_, what, "the query output overlaps the keys");
+  if (p.key_output) {
+    const Span k_out(p.key_output, p.tokens, static_cast<long long>(p.kv_heads) * head_dim, p.kv_heads, head_dim, head_dim);
+    const bool k_same = p.key_output == p.key && p.kv_head_stride == head_dim && p.kv_token_stride == p.kv_heads * head_dim;
+    if (k_out.meets(key) && !k_same) return refuse(ctx_, what, "the key output overlaps the keys");
+    if (k_out.meets(query) || k_out.meets(q_out)) return refuse(ctx_, what, "the key output overlaps the queries or their output");
+  }
+  if (p.key_cache) {
+    const Span value(p.value, p.tokens, p.kv_token_stride, p.kv_heads, p.kv_head_stride, head_dim);
+    if (q_out.meets(value)) return refuse(ctx_, what, "the query output overlaps the values");
+    if (p.key_output) {
+      const Span k_out(p.key_output, p.tokens, static_cast<long long>(p.kv_heads) * head_dim, p.kv_heads, head_dim, head_dim);
+      if (k_out.meets(value)) return refuse(ctx_, what, "the key output overlaps the values");
+    }
+  }
+  p.epsilon = ctx_.config().rms_norm_epsilon;
+  p.status = ctx_.status_word();
+  DeviceScope device(ctx_);
+  TK100_TRY(device.status());
+  ctx_.count_launch();
+  return ctx_.check(launch_rotary(stream, head_dim, p), "launching the rotary positions");
+}
+
+// --------------------------------------------------------------------- AttentionOp
+
+size_t AttentionOp::workspace_bytes(int sms, int head_dim) {
+  const size_t rows = 2 * static_cast<size_t>(sms) * kAttentionRows;
+  return kTicketBytes + rows * sizeof(float2) + rows * head_dim * sizeof(float);
+}
+
+Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, const uint16_t* query, const uint16_t* key,
+                            const uint16_t* value, float scale, void* workspace) {
+  TK100_TRY(heads(ctx_, what, p->q_heads, p->kv_heads, head_dim));
+  TK100_TRY(range(ctx_, what, "token count", p->tokens, 1, kMaxTokens));
+  TK100_TRY(range(ctx_, what, "sequence count", p->sequences, 1, kMaxSequences));
+  TK100_TRY(plane(ctx_, what, "start", p->starts, 4));
+  TK100_TRY(plane(ctx_, what, "query", query, 16));
+  TK100_TRY(plane(ctx_, what, "key", key, 16));
+  TK100_TRY(plane(ctx_, what, "value", value, 16));
+  TK100_TRY(plane(ctx_, what, "output", p->output, 16));
+  TK100_TRY(plane(ctx_, what, "workspace", workspace, 16));
+  if (p->gate) TK100_TRY(plane(ctx_, what, "gate", p->gate, 16));
+  TK100_TRY(stride(ctx_, what, "query token", p->query_token_stride, head_dim));
+  TK100_TRY(stride(ctx_, what, "query head", p->query_head_stride, head_dim));
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse(ctx_, what, "the scale must be positive and finite");
+  const Span out(p->output, p->tokens, static_cast<long long>(p->q_heads) * head_dim, p->q_heads, head_dim, head_dim);
+  const Span in(query, p->tokens, p->query_token_stride, p->q_heads, p->query_head_stride, head_dim);
+  if (out.meets(in)) return refuse(ctx_, what, "the output overlaps the queries");
+  if (p->gate) {
+    const Span gate(p->gate, p->tokens, p->query_token_stride, p->q_heads, p->query_head_stride, head_dim);
+    if (out.meets(gate)) return refuse(ctx_, what, "the output overlaps the gate");
+  }
+  p->group = p->q_heads / p->kv_heads;
+  p->tile_tokens = kAttentionRows / p->group;
+  p->scale_log2 = scale * 1.4426950408889634f;
+  p->min_steps = 1;
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  const size_t rows = 2 * static_cast<size_t>(ctx_.sm_count()) * kAttentionRows;
+  p->tickets = reinterpret_cast<unsigned int*>(w);
+  p->part_stats = reinterpret_cast<float2*>(w + kTicketBytes);
+  p->parts = reinterpret_cast<float*>(w + kTicketBytes + rows * sizeof(float2));
+  p->status = ctx_.status_word();
+  return TK100_OK;
+}
+
+Status AttentionOp::launch(cudaStream_t stream, const char* what, int head_dim, const AttentionParams& p,
+                           const uint16_t* query, const CUtensorMap& map_k, const CUtensorMap& map_v) {
+  CUtensorMap map_q, map_q1;
+  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(p.group),
+                            static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.tokens)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(p.query_head_stride),
+                               static_cast<uint64_t>(p.query_head_stride) * p.group,
+                               static_cast<uint64_t>(p.query_token_stride)};
+  const uint32_t group = static_cast<uint32_t>(p.group);
+  TK100_TRY(ctx_.bf16_map(query, dims, strides, {64u, group, 1u, static_cast<uint32_t>(p.tile_tokens)}, &map_q));
+  TK100_TRY(ctx_.bf16_map(query, dims, strides, {64u, group, 1u, 1u}, &map_q1));
+  DeviceScope device(ctx_);
+  TK100_TRY(device.status());
+  ctx_.count_launch();
+  return ctx_.check(launch_attention(stream, head_dim, ctx_.sm_count(), map_q, map_q1, map_k, map_v, p),
+                    (std::string("launching the ") + what).c_str());
+}
+
+Status AttentionOp::paged(cudaStream_t stream, int head_dim, AttentionParams p, const uint16_t* query,
+                          const uint16_t* key_cache, const uint16_t* value_cache, const CacheGeometry& cache, float scale,
+                          void* workspace) {
+  const char* what = "paged attention";
+  TK100_TRY(prepare(what, head_dim, &p, query, key_cache, value_cache, scale, workspace));
+  TK100_TRY(cache_geometry(ctx_, what, cache, head_dim));
+  TK100_TRY(plane(ctx_, what, "key length", p.kv_lengths, 4));
+  TK100_TRY(plane(ctx_, what, "block table", p.block_table, 4));
+  TK100_TRY(range(ctx_, what, "block table row count", p.table_row_count, 1, 1 << 30));
+  TK100_TRY(range(ctx_, what, "pages per row", p.max_pages, 1, 1 << 30));
+  if (!p.table_rows && p.sequences > p.table_row_count)
+    return refuse(ctx_, what, "the block table has fewer rows than there are sequences");
+  p.page_shift = log2_of(cache.page_tokens);
+  p.pages = cache.pages;
+  p.key_capacity = static_cast<int>(std::min(kMaxKeys, static_cast<long long>(p.max_pages) << p.page_shift));
+  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(cache.page_tokens),
+                            static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(cache.pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(cache.token_stride), static_cast<uint64_t>(cache.head_stride),
+                               static_cast<uint64_t>(cache.page_stride)};
+  const uint32_t k_box = static_cast<uint32_t>(std::min(128, cache.page_tokens));
+  const uint32_t v_box = static_cast<uint32_t>(std::min(attention_value_box(head_dim), cache.page_tokens));
+  CUtensorMap map_k, map_v;
+  TK100_TRY(ctx_.bf16_map(key_cache, dims, strides, {64u, k_box, 1u, 1u}, &map_k));
+  TK100_TRY(ctx_.bf16_map(value_cache, dims, strides, {64u, v_box, 1u, 1u}, &map_v));
+  return launch(stream, what, head_dim, p, query, map_k, map_v);
+}
+
+Status AttentionOp::prompt(cudaStream_t stream, int head_dim, AttentionParams p, const uint16_t* query, const uint16_t* key,
+                           const uint16_t* value, int kv_token_stride, int kv_head_stride, float scale, void* workspace) {
+  const char* what = "prompt attention";
+  TK100_TRY(prepare(what, head_dim, &p, query, key, value, scale, workspace));
+  TK100_TRY(stride(ctx_, what, "key/value token", kv_token_stride, head_dim));
+  TK100_TRY(stride(ctx_, what, "key/value head", kv_head_stride, head_dim));
+  const Span out(p.output, p.tokens, static_cast<long long>(p.q_heads) * head_dim, p.q_heads, head_dim, head_dim);
+  if (out.meets(Span(key, p.tokens, kv_token_stride, p.kv_heads, kv_head_stride, head_dim)) ||
+      out.meets(Span(value, p.tokens, kv_token_stride, p.kv_heads, kv_head_stride, head_dim)))
+    return refuse(ctx_, what, "the output overlaps the keys or values");
+  p.kv_lengths = nullptr;
+  p.block_table = nullptr;
+  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(p.tokens),
+                            static_cast<uint64_t>(p.kv_heads), 1u};
+  const uint64_t strides[3] = {static_cast<uint64_t>(kv_token_stride), static_cast<uint64_t>(kv_head_stride),
+                               static_cast<uint64_t>(kv_token_stride)};
+  CUtensorMap map_k, map_v;
+  TK100_TRY(ctx_.bf16_map(key, dims, strides, {64u, 128u, 1u, 1u}, &map_k));
+  TK100_TRY(ctx_.bf16_map(value, dims, strides, {64u, static_cast<uint32_t>(attention_value_box(head_dim)), 1u, 1u}, &map_v));
+  return launch(stream, what, head_dim, p, query, map_k, map_v);
+}
+
+}  // namespace tk100

@@ -152,7 +152,12 @@ PyObject* invoke(const char* name, tk100_status (*fn)(tk100_ctx*, tk100_stream, 
   X(tk100_nvfp4_gate_up_swiglu)              \
   X(tk100_nvfp4_gate_up_swiglu_quantize)     \
   X(tk100_nvfp4_down)                        \
-  X(tk100_nvfp4_down_partial)
+  X(tk100_nvfp4_down_partial)                \
+  X(tk100_page_plan)                         \
+  X(tk100_page_release)                      \
+  X(tk100_rotary_cache)                      \
+  X(tk100_paged_attention)                   \
+  X(tk100_prompt_attention)
 
 #define TK100_WRAPPER(name)                                                              \
   decltype(&::name) g_##name = nullptr;                                                  \

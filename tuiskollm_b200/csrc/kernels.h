@@ -390,4 +390,68 @@ cudaError_t launch_f32_to_bf16(cudaStream_t stream, long long n, const float* in
 cudaError_t launch_nvfp4_quantize(cudaStream_t stream, int rows, int k, const uint16_t* x,
                                   float divisor, uint8_t* codes, uint8_t* scales);
 
+// ------------------------------------------------------------ paging.cu, rotary.cu, attention.cu
+
+constexpr int kPageMaxRequests = 4096;  // requests of one plan: 16 bytes of shared memory each
+constexpr int kPageMaxRows = 262144;    // rows of a block table: a bit of shared memory each
+
+struct PageParams {
+  int requests, table_rows, max_pages, page_tokens, max_tokens, free_capacity;
+  const int32_t* request_rows;  // null: request i has row i
+  const int32_t* new_tokens;
+  const int32_t* lengths;
+  int32_t* lengths_output;
+  int32_t* block_table;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* free_count_output;
+  int32_t* starts;
+  int32_t* kv_lengths;
+  int32_t* positions;
+  long long* slots;
+  uint32_t* status;
+};
+cudaError_t page_prepare();
+cudaError_t launch_page(cudaStream_t stream, const PageParams& p, bool release);
+
+struct RotaryParams {
+  int tokens, q_heads, kv_heads, half, axes;
+  const double* frequencies;
+  const uint8_t* pair_axes;  // null: axis 0
+  const int32_t* positions;  // [axes, tokens]
+  const uint16_t *query, *key, *value;
+  int query_token_stride, query_head_stride, kv_token_stride, kv_head_stride;
+  const uint16_t *query_norm, *key_norm;  // null: no norm
+  float epsilon;
+  uint16_t *query_output, *key_output;  // key_output may be null
+  uint16_t *key_cache, *value_cache;    // both or neither
+  int pages, page_shift, page_stride, cache_token_stride, cache_head_stride;
+  const int64_t* slots;
+  uint32_t* status;
+};
+cudaError_t launch_rotary(cudaStream_t stream, int dim, const RotaryParams& p);
+
+struct AttentionParams {
+  int sequences, tokens, q_heads, kv_heads, group, tile_tokens;
+  int min_steps;               // 128-key steps that a CTA takes at least
+  const int32_t* starts;       // [sequences + 1]
+  const int32_t* kv_lengths;   // null: as many keys as new tokens
+  int key_capacity;            // keys that the block table has room for
+  const int32_t* block_table;  // null: keys and values are packed rows
+  const int32_t* table_rows;   // null: sequence s has row s
+  int table_row_count, max_pages, page_shift, pages;
+  float scale_log2;  // scale * log2(e)
+  const uint16_t* gate;
+  int query_token_stride, query_head_stride;
+  uint16_t* output;
+  float* parts;        // [2 per CTA][128 rows][head_dim]
+  float2* part_stats;  // [2 per CTA][128 rows]
+  unsigned int* tickets;
+  uint32_t* status;
+};
+cudaError_t attention_prepare();
+int attention_value_box(int dim);  // keys of a box of the value map
+cudaError_t launch_attention(cudaStream_t stream, int dim, int ctas, const CUtensorMap& map_q, const CUtensorMap& map_q1,
+                             const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p);
+
 }  // namespace tk100

@@ -162,6 +162,11 @@ Status Context::create(const tk100_config& in, Context** out, std::string* error
     delete ctx;
     return TK100_ERR_MODULE;
   }
+  if ((e = page_prepare()) != cudaSuccess || (e = attention_prepare()) != cudaSuccess) {
+    *error = std::string("[gpu.module] preparing the attention routes: ") + cudaGetErrorString(e);
+    delete ctx;
+    return TK100_ERR_MODULE;
+  }
   if ((e = nvfp4_prepare()) != cudaSuccess) {
     *error = std::string("[gpu.module] preparing the NVFP4 projection routes: ") +
              cudaGetErrorString(e);
@@ -300,6 +305,23 @@ Status Context::scale_map(const void* base, uint64_t chunks, CUtensorMap* out) {
   if (maps_.size() > 4096) maps_.clear();
   maps_.emplace(key, map);
   *out = map;
+  return TK100_OK;
+}
+
+Status Context::bf16_map(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                         const uint32_t (&box)[4], CUtensorMap* out) {
+  auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode_fn_);
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t bytes[3] = {2 * strides[0], 2 * strides[1], 2 * strides[2]};
+  const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
+  const cuuint32_t elem[4] = {1u, 1u, 1u, 1u};
+  CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, bytes, b, elem,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(TK100_ERR_DRIVER, "[gpu.driver] cuTensorMapEncodeTiled (BF16 heads) failed with CUresult " +
+                                      std::to_string(static_cast<int>(r)));
+  }
   return TK100_OK;
 }
 
@@ -1928,6 +1950,147 @@ tk100_status tk100_f32_to_bf16(tk100_ctx* ctx, tk100_stream stream, size_t count
   return ctx->impl->check(tk100::launch_f32_to_bf16(static_cast<cudaStream_t>(stream),
                                                     static_cast<long long>(count), input, output),
                           "launching fp32 -> BF16");
+}
+
+tk100_status tk100_page_plan(tk100_ctx* ctx, tk100_stream stream, int requests, int table_rows, int max_pages,
+                             int page_tokens, int max_tokens, int free_capacity, const int32_t* request_rows,
+                             const int32_t* new_tokens, const int32_t* lengths, int32_t* lengths_output,
+                             int32_t* block_table, const int32_t* free_pages, const int32_t* free_count,
+                             int32_t* free_count_output, int32_t* starts, int32_t* kv_lengths, int32_t* positions,
+                             int64_t* slots) {
+  if (!ctx) return TK100_ERR_CONTEXT;
+  tk100::PageParams p{};
+  p.requests = requests;
+  p.table_rows = table_rows;
+  p.max_pages = max_pages;
+  p.page_tokens = page_tokens;
+  p.max_tokens = max_tokens;
+  p.free_capacity = free_capacity;
+  p.request_rows = request_rows;
+  p.new_tokens = new_tokens;
+  p.lengths = lengths;
+  p.lengths_output = lengths_output;
+  p.block_table = block_table;
+  p.free_pages = const_cast<int32_t*>(free_pages);  // only the release writes it
+  p.free_count = free_count;
+  p.free_count_output = free_count_output;
+  p.starts = starts;
+  p.kv_lengths = kv_lengths;
+  p.positions = positions;
+  p.slots = reinterpret_cast<long long*>(slots);
+  return tk100::PagePlanOp(*ctx->impl).launch(static_cast<cudaStream_t>(stream), p);
+}
+
+tk100_status tk100_page_release(tk100_ctx* ctx, tk100_stream stream, int requests, int table_rows, int max_pages,
+                                int page_tokens, int free_capacity, const int32_t* request_rows,
+                                const int32_t* lengths, int32_t* lengths_output, const int32_t* block_table,
+                                int32_t* free_pages, const int32_t* free_count, int32_t* free_count_output) {
+  if (!ctx) return TK100_ERR_CONTEXT;
+  tk100::PageParams p{};
+  p.requests = requests;
+  p.table_rows = table_rows;
+  p.max_pages = max_pages;
+  p.page_tokens = page_tokens;
+  p.free_capacity = free_capacity;
+  p.request_rows = request_rows;
+  p.lengths = lengths;
+  p.lengths_output = lengths_output;
+  p.block_table = const_cast<int32_t*>(block_table);  // only the plan writes it
+  p.free_pages = free_pages;
+  p.free_count = free_count;
+  p.free_count_output = free_count_output;
+  return tk100::PagePlanOp(*ctx->impl).release(static_cast<cudaStream_t>(stream), p);
+}
+
+tk100_status tk100_rotary_cache(tk100_ctx* ctx, tk100_stream stream, int tokens, int q_heads, int kv_heads,
+                                int head_dim, int rotary_dim, int axes, const double* frequencies,
+                                const uint8_t* pair_axes, const int32_t* positions, const uint16_t* query,
+                                int query_token_stride, int query_head_stride, const uint16_t* key,
+                                const uint16_t* value, int kv_token_stride, int kv_head_stride,
+                                const uint16_t* query_norm, const uint16_t* key_norm, uint16_t* query_output,
+                                uint16_t* key_output, uint16_t* key_cache, uint16_t* value_cache, int pages,
+                                int page_tokens, int page_stride, int cache_token_stride, int cache_head_stride,
+                                const int64_t* slots) {
+  if (!ctx) return TK100_ERR_CONTEXT;
+  tk100::RotaryParams p{};
+  p.tokens = tokens;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.half = rotary_dim % 2 == 0 ? rotary_dim / 2 : 0;
+  p.axes = axes;
+  p.frequencies = frequencies;
+  p.pair_axes = pair_axes;
+  p.positions = positions;
+  p.query = query;
+  p.key = key;
+  p.value = value;
+  p.query_token_stride = query_token_stride;
+  p.query_head_stride = query_head_stride;
+  p.kv_token_stride = kv_token_stride;
+  p.kv_head_stride = kv_head_stride;
+  p.query_norm = query_norm;
+  p.key_norm = key_norm;
+  p.query_output = query_output;
+  p.key_output = key_output;
+  p.key_cache = key_cache;
+  p.value_cache = value_cache;
+  p.slots = slots;
+  return tk100::RotaryCacheOp(*ctx->impl)
+      .launch(static_cast<cudaStream_t>(stream), head_dim, p,
+              {pages, page_tokens, page_stride, cache_token_stride, cache_head_stride});
+}
+
+size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_dim) {
+  return ctx && head_dim > 0 ? tk100::AttentionOp::workspace_bytes(ctx->impl->sm_count(), head_dim) : 0;
+}
+
+tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens, int q_heads,
+                                   int kv_heads, int head_dim, const int32_t* starts, const int32_t* kv_lengths,
+                                   const uint16_t* query, const uint16_t* gate, int query_token_stride,
+                                   int query_head_stride, const uint16_t* key_cache, const uint16_t* value_cache,
+                                   int pages, int page_tokens, int page_stride, int cache_token_stride,
+                                   int cache_head_stride, const int32_t* block_table, int table_rows, int max_pages,
+                                   const int32_t* request_rows, float scale, void* workspace, uint16_t* output) {
+  if (!ctx) return TK100_ERR_CONTEXT;
+  tk100::AttentionParams p{};
+  p.sequences = sequences;
+  p.tokens = tokens;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.starts = starts;
+  p.kv_lengths = kv_lengths;
+  p.block_table = block_table;
+  p.table_rows = request_rows;
+  p.table_row_count = table_rows;
+  p.max_pages = max_pages;
+  p.gate = gate;
+  p.query_token_stride = query_token_stride;
+  p.query_head_stride = query_head_stride;
+  p.output = output;
+  return tk100::AttentionOp(*ctx->impl)
+      .paged(static_cast<cudaStream_t>(stream), head_dim, p, query, key_cache, value_cache,
+             {pages, page_tokens, page_stride, cache_token_stride, cache_head_stride}, scale, workspace);
+}
+
+tk100_status tk100_prompt_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens, int q_heads,
+                                    int kv_heads, int head_dim, const int32_t* starts, const uint16_t* query,
+                                    const uint16_t* gate, int query_token_stride, int query_head_stride,
+                                    const uint16_t* key, const uint16_t* value, int kv_token_stride,
+                                    int kv_head_stride, float scale, void* workspace, uint16_t* output) {
+  if (!ctx) return TK100_ERR_CONTEXT;
+  tk100::AttentionParams p{};
+  p.sequences = sequences;
+  p.tokens = tokens;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.starts = starts;
+  p.gate = gate;
+  p.query_token_stride = query_token_stride;
+  p.query_head_stride = query_head_stride;
+  p.output = output;
+  return tk100::AttentionOp(*ctx->impl)
+      .prompt(static_cast<cudaStream_t>(stream), head_dim, p, query, key, value, kv_token_stride, kv_head_stride, scale,
+              workspace);
 }
 
 }  // extern "C"

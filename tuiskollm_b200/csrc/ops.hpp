@@ -86,6 +86,11 @@ class Context {
   Status swiglu_map(const void* base, uint64_t outputs, uint64_t row_bytes, CUtensorMap* out);
   Status swiglu_scale_map(const void* base, uint64_t outputs, uint64_t chunks_per_tile, CUtensorMap* out);
 
+  // BF16 tensor of four dimensions (innermost first; strides of the outer three in elements), read in boxes of
+  // box[0] = 64 values with the 128-byte swizzle.  Encoded anew at each launch: activation planes move.
+  Status bf16_map(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4],
+                  CUtensorMap* out);
+
   const tk100_config& config() const { return config_; }
   int sm_count() const { return sm_count_; }
   // Clusters of `splits` CTA pairs (pair_gemm.cu) that fit the device at once.
@@ -330,6 +335,54 @@ class Nvfp4MlpOp {
                 float* output_f32 = nullptr, const Nvfp4NextQuant* next = nullptr);
 
  private:
+  Context& ctx_;
+};
+
+// What follows has no counterpart in the reference, whose full-attention layer ends at the QKV projection.
+
+// Geometry of a paged cache plane pair: element (page, token, head, d) of either at
+// page * page_stride + token * token_stride + head * head_stride + d.
+struct CacheGeometry {
+  int pages, page_tokens, page_stride, token_stride, head_stride;
+};
+
+// Block tables, slot maps and lengths of a step, built on the device (paging.cu).
+class PagePlanOp {
+ public:
+  explicit PagePlanOp(Context& ctx) : ctx_(ctx) {}
+  Status launch(cudaStream_t stream, PageParams p);
+  Status release(cudaStream_t stream, PageParams p);
+
+ private:
+  Status check(const char* what, const PageParams& p);
+  Context& ctx_;
+};
+
+// Head norms, rotary positions with several axes and the stores into the cache, one launch (rotary.cu).
+class RotaryCacheOp {
+ public:
+  explicit RotaryCacheOp(Context& ctx) : ctx_(ctx) {}
+  Status launch(cudaStream_t stream, int head_dim, RotaryParams p, const CacheGeometry& cache);
+
+ private:
+  Context& ctx_;
+};
+
+// Causal attention over a paged cache or over packed prompt rows (attention.cu).
+class AttentionOp {
+ public:
+  explicit AttentionOp(Context& ctx) : ctx_(ctx) {}
+  static size_t workspace_bytes(int sms, int head_dim);
+  Status paged(cudaStream_t stream, int head_dim, AttentionParams p, const uint16_t* query, const uint16_t* key_cache,
+               const uint16_t* value_cache, const CacheGeometry& cache, float scale, void* workspace);
+  Status prompt(cudaStream_t stream, int head_dim, AttentionParams p, const uint16_t* query, const uint16_t* key,
+                const uint16_t* value, int kv_token_stride, int kv_head_stride, float scale, void* workspace);
+
+ private:
+  Status prepare(const char* what, int head_dim, AttentionParams* p, const uint16_t* query, const uint16_t* key,
+                 const uint16_t* value, float scale, void* workspace);
+  Status launch(cudaStream_t stream, const char* what, int head_dim, const AttentionParams& p, const uint16_t* query,
+                const CUtensorMap& map_k, const CUtensorMap& map_v);
   Context& ctx_;
 };
 

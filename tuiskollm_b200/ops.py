@@ -360,6 +360,231 @@ class GdnRecurrenceOp:
                                        state_rows, state, output)
 
 
+def _plane(context: Context, t, name, dtype, least):
+    """Address of a contiguous plane of at least `least` values of one type on the context's device."""
+    if t.dtype != dtype or t.device.type != "cuda" or t.device.index != context.device:
+        raise GpuError(5, f"[gpu.launch] {name}: a {dtype} plane on the context's device is required, got {t.dtype} "
+                          f"on {t.device}")
+    if t.numel() < least or not t.is_contiguous():
+        raise GpuError(5, f"[gpu.launch] {name}: a contiguous plane of at least {least} values is required, got "
+                          f"shape {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _heads(context: Context, t, name, shape):
+    """(address, strides) of a BF16 plane of the given shape (None: any extent) whose last dimension is dense."""
+    if t.dtype != torch.bfloat16 or t.device.type != "cuda" or t.device.index != context.device:
+        raise GpuError(5, f"[gpu.launch] {name}: a torch.bfloat16 plane on the context's device is required, got "
+                          f"{t.dtype} on {t.device}")
+    if t.dim() != len(shape) or any(b is not None and a != b for a, b in zip(t.shape, shape)):
+        raise GpuError(5, f"[gpu.launch] {name}: shape {tuple(t.shape)} is not {shape}")
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] > 1:
+        raise GpuError(5, f"[gpu.launch] {name}: the values of a head are not next to each other")
+    return t.data_ptr(), strides
+
+
+def _cache(context: Context, key_cache, value_cache, kv_heads, head_dim):
+    """(addresses, pages, page tokens, strides) of a cache pair ``[pages, page tokens, heads, head_dim]``."""
+    key, strides = _heads(context, key_cache, "key cache", (None, None, kv_heads, head_dim))
+    value, others = _heads(context, value_cache, "value cache", key_cache.shape)
+    if strides != others:
+        raise GpuError(5, f"[gpu.launch] key and value cache have different strides {strides} and {others}")
+    return key, value, key_cache.shape[0], key_cache.shape[1], strides
+
+
+class PagePlanOp:
+    """Block tables, slot maps, positions and lengths of a step, built on the device from the requests' lengths
+    (``tk100_page_plan``), and pages taken back (``tk100_page_release``).  Nothing of it passes the host, so a
+    captured step can be replayed while requests grow.
+
+    ``block_table`` is int32 ``[rows, pages per row]``, ``lengths`` int32 ``[rows]``, ``free_pages`` the int32 stack of
+    free page ids with its count in ``free_count[0]``; ``request_rows`` (or None: request i has row i) and
+    ``new_tokens`` are int32 ``[requests]``.  Outputs: ``starts`` int32 ``[requests + 1]``, ``kv_lengths`` int32
+    ``[requests]``, ``positions`` int32 and ``slots`` int64, whose length is the step's token capacity.  A step that
+    does not fit changes nothing and is reported in :meth:`Context.device_status`."""
+
+    def __init__(self, context: Context, page_tokens: int):
+        self.ctx = context
+        self.page_tokens = page_tokens
+
+    def _state(self, requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count,
+               free_count_output):
+        c = self.ctx
+        if block_table.dim() != 2:
+            raise GpuError(5, f"[gpu.launch] block table: shape {tuple(block_table.shape)} is not [rows, pages]")
+        rows, pages = block_table.shape
+        i32 = torch.int32
+        return (rows, pages, free_pages.numel(),
+                None if request_rows is None else _plane(c, request_rows, "request rows", i32, requests),
+                _plane(c, lengths, "lengths", i32, rows), _plane(c, lengths_output, "length output", i32, rows),
+                _plane(c, block_table, "block table", i32, 1), _plane(c, free_pages, "free pages", i32, 1),
+                _plane(c, free_count, "free count", i32, 1), _plane(c, free_count_output, "free count output", i32, 1))
+
+    def launch(self, stream, requests, request_rows, new_tokens, lengths, lengths_output, block_table, free_pages,
+               free_count, free_count_output, starts, kv_lengths, positions, slots):
+        c = self.ctx
+        rows, pages, capacity, chosen, old, new, table, stack, count, left = self._state(
+            requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count, free_count_output)
+        tokens = slots.numel()
+        c._native.tk100_page_plan(
+            c, stream, requests, rows, pages, self.page_tokens, tokens, capacity, chosen,
+            _plane(c, new_tokens, "new tokens", torch.int32, requests), old, new, table, stack, count, left,
+            _plane(c, starts, "starts", torch.int32, requests + 1),
+            _plane(c, kv_lengths, "key lengths", torch.int32, requests),
+            _plane(c, positions, "positions", torch.int32, tokens), _plane(c, slots, "slots", torch.int64, 1))
+
+    def release(self, stream, requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count,
+                free_count_output):
+        c = self.ctx
+        rows, pages, capacity, chosen, old, new, table, stack, count, left = self._state(
+            requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count, free_count_output)
+        c._native.tk100_page_release(c, stream, requests, rows, pages, self.page_tokens, capacity, chosen, old, new,
+                                     table, stack, count, left)
+
+
+def rotary_frequencies(rotary_dim: int, theta: float, device="cuda"):
+    """``theta ** (-2 i / rotary_dim)`` radians per position, float64 ``[rotary_dim / 2]``."""
+    return (theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)).to(device)
+
+
+def rotary_pair_axes(sections, interleaved: bool = False, device="cuda"):
+    """The axis that turns each pair, uint8 ``[sum(sections)]``: ``sections[a]`` pairs for axis a (time, height,
+    width), one section behind the other or, interleaved, the axes in turn while they have pairs left, the rest
+    to axis 0."""
+    if not interleaved:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    else:
+        axes, count = [0] * sum(sections), len(sections)
+        for a in range(1, count):
+            places = range(a, sum(sections), count)
+            if len(places) < sections[a]:
+                raise ValueError(f"axis {a} has {sections[a]} pairs, but only {len(places)} places in turn")
+            for place in places[:sections[a]]:
+                axes[place] = a
+    return torch.tensor(axes, dtype=torch.uint8, device=device)
+
+
+class RotaryCacheOp:
+    """Head norms (optional), rotary positions with one or several axes, and the stores into the paged cache
+    (``tk100_rotary_cache``), one launch behind the QKV projection.
+
+    ``frequencies`` is float64 ``[rotary_dim / 2]`` (:func:`rotary_frequencies`, or any scaled set), ``pair_axes``
+    uint8 of the same length (:func:`rotary_pair_axes`; None: one axis)."""
+
+    def __init__(self, context: Context, q_heads: int, kv_heads: int, head_dim: int, frequencies, pair_axes=None):
+        self.ctx, self.q_heads, self.kv_heads, self.head_dim = context, q_heads, kv_heads, head_dim
+        self.rotary_dim = 2 * frequencies.numel()
+        self.frequencies, self.pair_axes = frequencies, pair_axes
+        self._frequencies = _plane(context, frequencies, "frequencies", torch.float64, 1)
+        self._pair_axes = None if pair_axes is None else _plane(context, pair_axes, "pair axes", torch.uint8,
+                                                                frequencies.numel())
+
+    def launch(self, stream, tokens, positions, query, key, value, query_norm, key_norm, query_output, key_output,
+               key_cache, value_cache, slots):
+        """``query`` ``[>= tokens, q_heads, head_dim]``, ``key`` and ``value`` ``[>= tokens, kv_heads, head_dim]`` with any
+        token and head strides (views of the projection's rows); ``positions`` int32 ``[axes, tokens]`` or
+        ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output`` dense or None; caches
+        ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
+        c, dim = self.ctx, self.head_dim
+        q, qs = _heads(c, query, "query", (None, self.q_heads, dim))
+        k, ks = _heads(c, key, "key", (None, self.kv_heads, dim))
+        v = None
+        if value is not None:
+            v, vs = _heads(c, value, "value", (None, self.kv_heads, dim))
+            if vs != ks:
+                raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
+        if min(query.shape[0], key.shape[0], key.shape[0] if value is None else value.shape[0]) < tokens:
+            raise GpuError(5, f"[gpu.launch] rotary: planes have fewer than {tokens} rows")
+        axes = 1 if positions.dim() == 1 else positions.shape[0]
+        if positions.shape[-1] != tokens:
+            raise GpuError(5, f"[gpu.launch] positions: shape {tuple(positions.shape)} is not [axes, {tokens}]")
+        bf16 = torch.bfloat16
+        kc = vc = at = None
+        pages = page_tokens = 0
+        cs = (0, 0, 0)
+        if key_cache is not None or value_cache is not None:
+            if key_cache is None or value_cache is None or value is None or slots is None:
+                raise GpuError(5, "[gpu.launch] rotary: a key cache, a value cache, values and slots go together")
+            kc, vc, pages, page_tokens, cs = _cache(c, key_cache, value_cache, self.kv_heads, dim)
+            at = _plane(c, slots, "slots", torch.int64, tokens)
+        c._native.tk100_rotary_cache(
+            c, stream, tokens, self.q_heads, self.kv_heads, dim, self.rotary_dim, axes, self._frequencies,
+            self._pair_axes, _plane(c, positions, "positions", torch.int32, axes * tokens), q, qs[0], qs[1], k, v,
+            ks[0], ks[1], None if query_norm is None else _plane(c, query_norm, "query norm", bf16, dim),
+            None if key_norm is None else _plane(c, key_norm, "key norm", bf16, dim),
+            _plane(c, query_output, "query output", bf16, tokens * self.q_heads * dim),
+            None if key_output is None else _plane(c, key_output, "key output", bf16, tokens * self.kv_heads * dim),
+            kc, vc, pages, page_tokens, cs[0], cs[1], cs[2], at)
+
+
+class _AttentionOp:
+    def __init__(self, context: Context, q_heads: int, kv_heads: int, head_dim: int, scale: Optional[float] = None):
+        self.ctx, self.q_heads, self.kv_heads, self.head_dim = context, q_heads, kv_heads, head_dim
+        self.scale = float(scale if scale is not None else head_dim ** -0.5)
+
+    def workspace(self):
+        """A zeroed workspace.  Launches one behind the other share one; launches that may overlap (two streams,
+        two captured graphs) need one each."""
+        nbytes = int(self.ctx._lib.tk100_attention_workspace_bytes(self.ctx.handle, self.head_dim))
+        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", self.ctx.device))
+
+    def _rows(self, sequences, starts, query, gate, workspace, output):
+        c, dim = self.ctx, self.head_dim
+        q, qs = _heads(c, query, "query", (None, self.q_heads, dim))
+        g = None
+        if gate is not None:
+            g, gs = _heads(c, gate, "gate", query.shape)
+            if gs != qs:
+                raise GpuError(5, f"[gpu.launch] query and gate have different strides {qs} and {gs}")
+        tokens = query.shape[0]
+        need = int(c._lib.tk100_attention_workspace_bytes(c.handle, dim))
+        return (tokens, q, g, qs, _plane(c, starts, "starts", torch.int32, sequences + 1),
+                _plane(c, workspace, "workspace", torch.uint8, need),
+                _plane(c, output, "output", torch.bfloat16, tokens * self.q_heads * dim))
+
+
+class PagedAttentionOp(_AttentionOp):
+    """Causal attention of new tokens over the paged cache (``tk100_paged_attention``): decode steps, chunks of a
+    prompt, and both in one launch.  24 query heads over 4 key/value heads of 256 values are the model's;
+    heads of 128 and up to 128 query heads per key/value head are admitted.
+
+    ``launch``: ``starts`` int32 ``[sequences + 1]`` rows of ``query`` ``[tokens, q_heads, head_dim]``; ``kv_lengths`` int32
+    ``[sequences]`` keys of each, its new ones included; ``gate`` None or a plane with the query's strides whose sigmoid
+    multiplies the output; ``block_table`` int32 ``[rows, pages per row]`` with row ``request_rows[s]`` (None: s)."""
+
+    def launch(self, stream, sequences, starts, kv_lengths, query, gate, key_cache, value_cache, block_table,
+               request_rows, workspace, output):
+        c = self.ctx
+        tokens, q, g, qs, at, work, out = self._rows(sequences, starts, query, gate, workspace, output)
+        key, value, pages, page_tokens, cs = _cache(c, key_cache, value_cache, self.kv_heads, self.head_dim)
+        if block_table.dim() != 2:
+            raise GpuError(5, f"[gpu.launch] block table: shape {tuple(block_table.shape)} is not [rows, pages]")
+        c._native.tk100_paged_attention(
+            c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,
+            _plane(c, kv_lengths, "key lengths", torch.int32, sequences), q, g, qs[0], qs[1], key, value, pages,
+            page_tokens, cs[0], cs[1], cs[2], _plane(c, block_table, "block table", torch.int32, 1),
+            block_table.shape[0], block_table.shape[1],
+            None if request_rows is None else _plane(c, request_rows, "request rows", torch.int32, sequences),
+            self.scale, work, out)
+
+
+class PromptAttentionOp(_AttentionOp):
+    """Causal attention over whole prompts packed one behind the other (``tk100_prompt_attention``); ``key`` and
+    ``value`` are ``[tokens, kv_heads, head_dim]`` with the rows of ``query`` and any token and head strides."""
+
+    def launch(self, stream, sequences, starts, query, gate, key, value, workspace, output):
+        c = self.ctx
+        tokens, q, g, qs, at, work, out = self._rows(sequences, starts, query, gate, workspace, output)
+        shape = (tokens, self.kv_heads, self.head_dim)
+        k, ks = _heads(c, key, "key", shape)
+        v, vs = _heads(c, value, "value", shape)
+        if vs != ks:
+            raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
+        c._native.tk100_prompt_attention(c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,
+                                         q, g, qs[0], qs[1], k, v, ks[0], ks[1], self.scale, work, out)
+
+
 class LmHeadOp:
     """tuisko-kernels-sm120/src/fp8/projection.rs:704-793 plus the fused greedy argmax.
 

@@ -37,14 +37,15 @@ namespace {
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kKeys = 128;   // keys of a step
 constexpr int kThreads = 320;
-constexpr int kUnit = 16384;  // bytes of a ring stage
+constexpr int kUnit = 32768;  // bytes of a ring stage
 
 template <int D>
 struct Shape {
-  static constexpr int CHUNKS = D / 64;                    // 128-byte columns of a row
-  static constexpr int V_KEYS = kUnit / (2 * D);           // keys of a V unit: 32 or 64
+  static constexpr int CHUNKS = D / 64;           // 128-byte columns of a row
+  static constexpr int K_UNITS = CHUNKS / 2;      // a K unit is 128 keys x 2 chunks
+  static constexpr int V_KEYS = kUnit / (2 * D);  // a V unit is 64 or 128 keys x all chunks
   static constexpr int V_UNITS = kKeys / V_KEYS;
-  static constexpr int STAGES = D == 256 ? 10 : 12;
+  static constexpr int STAGES = D == 256 ? 5 : 6;
   static constexpr int SHARED = kRows * 2 * D + STAGES * kUnit + 1024;
 };
 
@@ -117,17 +118,28 @@ __device__ __forceinline__ long long steps_before(const AttentionParams& p, cons
   return sum;
 }
 
-struct Start {
-  int sequence, head, tile, step;  // where this CTA's stretch begins
-  int ctas;                        // CTAs that have work
-  long long total, first, last;    // steps of the launch; this CTA's [first, last)
+// A place in the line: step `step` of a tile, whose step 0 is at `line`.
+struct Place {
+  int sequence, head, tile, step;
+  long long line;
 };
 
-__device__ __forceinline__ long long cta_first(long long total, int ctas, int c) { return c * total / ctas; }
-// CTA whose stretch holds step u.
+// This CTA's stretch [first, last) of the `total` steps that `ctas` CTAs share, and the places of its ends.
+struct Stretch {
+  long long total, first, last;
+  int ctas;
+  Place from, to;  // `to` is of use where it lies inside a tile (step > 0)
+};
+
+// Even cuts of the line.
+__device__ __forceinline__ long long cut(long long total, int ctas, int c) { return c * total / ctas; }
+// CTA whose even stretch holds step u.
 __device__ __forceinline__ int cta_of(long long total, int ctas, long long u) {
   return static_cast<int>(((u + 1) * ctas - 1) / total);
 }
+// A cut closer than this to an end of the tile it falls into moves there: joining the parts of a tile of 128 rows
+// costs as much as some four steps (their fp32 rows through L2 and back), of a decoded token's as one.
+__device__ __forceinline__ int cut_margin(int rows) { return 1 + rows / 32; }
 
 // One tile, or the part of it that this CTA works on.
 struct Item {
@@ -139,22 +151,46 @@ struct Item {
   long long line;          // place of its step 0 in the line
 };
 
+__device__ __forceinline__ void describe(const AttentionParams& p, const Sequence& seq, int sequence, int head, int tile,
+                                         Item* it) {
+  it->seq = seq;
+  it->sequence = sequence;
+  it->head = head;
+  it->tile = tile;
+  it->steps = tile_steps(p, seq, tile);
+  it->limit = tile_limit(p, seq, tile);
+  it->tokens = min(p.tile_tokens, seq.q - tile * p.tile_tokens);
+}
+
+// The CTA's items.  A tile that it begins and another CTA goes on with comes first: with the tile that it goes on
+// with itself, parts are there early and are joined while the whole tiles run.
 struct Walk {
-  int sequence, head, tile, step;
+  int sequence, head, tile, step, tiles;
   long long at, end;
   Sequence seq;
-  int tiles;
+  Place tail;
+  bool has_tail;
 
-  __device__ __forceinline__ Walk(const AttentionParams& p, const Start& s)
-      : sequence(s.sequence), head(s.head), tile(s.tile), step(s.step), at(s.first), end(s.last) {
+  __device__ __forceinline__ Walk(const AttentionParams& p, const Stretch& s)
+      : sequence(s.from.sequence), head(s.from.head), tile(s.from.tile), step(s.from.step), tiles(0), at(s.first),
+        end(s.last), tail(s.to) {
     seq = {0, 0, 0};
-    tiles = 0;
+    has_tail = at < end && tail.step > 0 && tail.line >= at;
+    if (has_tail) end = tail.line;
     if (at < end) {
       seq = read_sequence(p, sequence);
       tiles = tile_count(p, seq);
     }
   }
   __device__ __forceinline__ bool next(const AttentionParams& p, Item* it) {
+    if (has_tail) {
+      has_tail = false;
+      describe(p, read_sequence(p, tail.sequence), tail.sequence, tail.head, tail.tile, it);
+      it->first = 0;
+      it->last = tail.step;
+      it->line = tail.line;
+      return true;
+    }
     if (at >= end) return false;
     while (tile >= tiles) {  // the next head, or the next sequence that has tokens
       tile = 0;
@@ -165,13 +201,7 @@ struct Walk {
         tiles = tile_count(p, seq);
       }
     }
-    it->seq = seq;
-    it->sequence = sequence;
-    it->head = head;
-    it->tile = tile;
-    it->steps = tile_steps(p, seq, tile);
-    it->limit = tile_limit(p, seq, tile);
-    it->tokens = min(p.tile_tokens, seq.q - tile * p.tile_tokens);
+    describe(p, seq, sequence, head, tile, it);
     it->first = step;
     it->last = static_cast<int>(min(static_cast<long long>(it->steps), step + (end - at)));
     it->line = at - step;
@@ -182,12 +212,36 @@ struct Walk {
   }
 };
 
-struct Scratch {
-  long long warp_sums[kThreads / 32];
-  Start start;
+// The items' steps one behind the other.
+struct Steps {
+  Walk walk;
+  Item it;
+  int j, item;
+
+  __device__ __forceinline__ Steps(const AttentionParams& p, const Stretch& s) : walk(p, s), j(0), item(-1) {
+    it.first = it.last = 0;
+  }
+  __device__ __forceinline__ bool next(const AttentionParams& p) {
+    if (++j < it.last) return true;
+    if (!walk.next(p, &it)) return false;
+    j = it.first;
+    ++item;
+    return true;
+  }
+  __device__ __forceinline__ bool opens() const { return j == it.first; }
+  __device__ __forceinline__ bool closes() const { return j + 1 == it.last; }
 };
 
-__device__ __forceinline__ void find_start(const AttentionParams& p, Scratch& sh) {
+struct Scratch {
+  long long warp_sums[kThreads / 32];
+  int sequence[2];
+  long long rest[2];
+  Stretch stretch;
+};
+
+// Finds the CTA's stretch.  All threads sum up the sequences' steps; the thread that passes a cut names the
+// sequence, and one warp per cut finds head and tile in it.
+__device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh) {
   const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
   const int run = (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
@@ -205,7 +259,7 @@ __device__ __forceinline__ void find_start(const AttentionParams& p, Scratch& sh
     if (lane >= o) sum += x;
   }
   if (lane == 31) sh.warp_sums[warp] = sum;
-  if (t == 0) sh.start = {};
+  if (t == 0) sh.stretch = {};
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -217,38 +271,69 @@ __device__ __forceinline__ void find_start(const AttentionParams& p, Scratch& sh
   if (total == 0) return;
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + p.min_steps - 1) / p.min_steps));
   const int c = static_cast<int>(blockIdx.x);
-  if (c < ctas) {
-    const long long first = cta_first(total, ctas, c), last = cta_first(total, ctas, c + 1);
-    if (before <= first && first < before + mine) {
-      long long rest = first - before;
+  if (c >= ctas) return;
+  const long long cuts[2] = {cut(total, ctas, c), cut(total, ctas, c + 1)};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (before <= cuts[k] && cuts[k] < before + mine) {
+      long long rest = cuts[k] - before;
       int s = s0;
-      Sequence q = read_sequence(p, s);
-      long long steps = steps_before(p, q, tile_count(p, q));
-      while (rest >= steps * p.kv_heads) {
-        rest -= steps * p.kv_heads;
-        q = read_sequence(p, ++s);
-        steps = steps_before(p, q, tile_count(p, q));
+      for (;; ++s) {
+        const Sequence q = read_sequence(p, s);
+        const long long steps = steps_before(p, q, tile_count(p, q)) * p.kv_heads;
+        if (rest < steps) break;
+        rest -= steps;
       }
-      Start r;
-      r.sequence = s;
-      r.head = static_cast<int>(rest / steps);
-      rest -= r.head * steps;
-      int low = 0, high = tile_count(p, q);  // steps_before(low) <= rest < steps_before(high)
+      sh.sequence[k] = s;
+      sh.rest[k] = rest;
+    }
+  }
+  __syncthreads();
+  if (warp < 2) {
+    long long u = cuts[0];
+    Place at = {};
+    if (warp == 1) u = cuts[1];
+    if (u < total) {
+      at.sequence = sh.sequence[warp];
+      const Sequence q = read_sequence(p, at.sequence);
+      const int tiles = tile_count(p, q);
+      long long rest = sh.rest[warp];
+      const long long per_head = steps_before(p, q, tiles);
+      at.head = static_cast<int>(rest / per_head);
+      rest -= at.head * per_head;
+      int low = 0, high = tiles;  // steps_before(low) <= rest < steps_before(high)
       while (high - low > 1) {
-        const int middle = (low + high) >> 1;
-        if (steps_before(p, q, middle) <= rest) {
-          low = middle;
-        } else {
-          high = middle;
-        }
+        const int width = (high - low + 31) / 32, probe = low + (lane + 1) * width;
+        const bool behind = probe < high && steps_before(p, q, probe) <= rest;
+        low += __popc(__ballot_sync(0xffffffffu, behind)) * width;
+        high = min(high, low + width);
       }
-      r.tile = low;
-      r.step = static_cast<int>(rest - steps_before(p, q, low));
-      r.ctas = ctas;
-      r.total = total;
-      r.first = first;
-      r.last = last;
-      sh.start = r;
+      at.tile = low;
+      rest -= steps_before(p, q, low);
+      at.step = static_cast<int>(rest);
+      at.line = u - rest;
+      const int steps = tile_steps(p, q, at.tile);
+      const int margin = cut_margin(min(p.tile_tokens, q.q - at.tile * p.tile_tokens) * p.group);
+      if (at.step < margin) {
+        at.step = 0;
+        u = at.line;
+      } else if (steps - at.step < margin) {
+        at.step = 0;
+        ++at.tile;
+        u = at.line + steps;
+        at.line = u;
+      }
+    }
+    if (lane == 0) {
+      if (warp == 0) {
+        sh.stretch.from = at;
+        sh.stretch.first = u;
+        sh.stretch.total = total;
+        sh.stretch.ctas = ctas;
+      } else {
+        sh.stretch.to = at;
+        sh.stretch.last = u;
+      }
     }
   }
   __syncthreads();
@@ -272,6 +357,99 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int see
   if (masked) {
 #pragma unroll
     for (int k = 0; k < kKeys; ++k) s[k] = k < seen ? s[k] : 0xff800000u;
+  }
+}
+
+// A bounded wait of a whole warp, with one verdict.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+}
+
+// Rows of a tile whose first token row is `token`.
+__device__ __forceinline__ const uint16_t* gate_row(const AttentionParams& p, int token, int head, int row) {
+  return p.gate + static_cast<size_t>(token + row / p.group) * p.query_token_stride +
+         static_cast<size_t>(head * p.group + row % p.group) * p.query_head_stride;
+}
+template <int D>
+__device__ __forceinline__ uint16_t* output_row(const AttentionParams& p, int token, int head, int row) {
+  return p.output + (static_cast<size_t>(token + row / p.group) * p.q_heads + head * p.group + row % p.group) * D;
+}
+__device__ __forceinline__ float gated(float v, float gate) {
+  return __fdividef(v, 1.0f + exp2_approx(gate * -1.4426950408889634f));
+}
+
+// Joins the parts of a tile that CTAs c0 .. c1 left, in the order of their keys: a thread has four of a row's values
+// at a time, and of four such places and four parts all loads are under way together.
+template <int D>
+__device__ __forceinline__ void join(const AttentionParams& p, int c0, int c1, int rows, int thread, int ahead, int token,
+                                     int head) {
+  constexpr int PLACES = 4, PARTS = 4;
+  auto slot_of = [&](int k) { return 2 * static_cast<size_t>(k) + (k == c0 ? 1 : 0); };
+  const int places = rows * (D / 4);
+  for (int base = thread; base < places; base += 128 * PLACES) {
+    float top[PLACES], total[PLACES];
+    float4 acc[PLACES];
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      top[i] = -INFINITY;
+      total[i] = 0.0f;
+      acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int k = c0; k <= c1; k += PARTS) {
+#pragma unroll
+      for (int i = 0; i < PLACES; ++i) {
+        const int at = min(base + 128 * i, places - 1), row = at / (D / 4), column = at % (D / 4) * 4;
+        float2 stats[PARTS];
+        float4 o[PARTS];
+#pragma unroll
+        for (int e = 0; e < PARTS; ++e) {
+          const size_t line = slot_of(min(k + e, c1)) * kRows + row;
+          stats[e] = __ldcg(&p.part_stats[line]);
+          o[e] = __ldcg(reinterpret_cast<const float4*>(p.parts + line * D + column));
+        }
+        float most = top[i];
+#pragma unroll
+        for (int e = 0; e < PARTS; ++e) {
+          // a part without a key of this row has nothing to add, whatever its O holds
+          if (k + e > c1 || (stats[e].x == -INFINITY && stats[e].y == 0.0f)) {
+            stats[e] = make_float2(-INFINITY, 0.0f);
+            o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+          most = fmaxf(most, stats[e].x);
+        }
+        const float shift = most == -INFINITY ? 0.0f : most;
+        const float before = exp2_approx(top[i] - shift);
+        top[i] = most;
+        total[i] *= before;
+        acc[i] = make_float4(acc[i].x * before, acc[i].y * before, acc[i].z * before, acc[i].w * before);
+#pragma unroll
+        for (int e = 0; e < PARTS; ++e) {
+          const float w = exp2_approx(stats[e].x - shift);
+          total[i] = fmaf(stats[e].y, w, total[i]);
+          acc[i].x = fmaf(o[e].x, w, acc[i].x);
+          acc[i].y = fmaf(o[e].y, w, acc[i].y);
+          acc[i].z = fmaf(o[e].z, w, acc[i].z);
+          acc[i].w = fmaf(o[e].w, w, acc[i].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = base + 128 * i, row = at / (D / 4), column = at % (D / 4) * 4;
+      if (at >= places) break;
+      const float scale = 1.0f / total[i];
+      float v[4] = {acc[i].x * scale, acc[i].y * scale, acc[i].z * scale, acc[i].w * scale};
+      if (p.gate) {
+        const uint2 g = *reinterpret_cast<const uint2*>(gate_row(p, token, head, row) + column);
+        v[0] = gated(v[0], bf16x2_lo(g.x));
+        v[1] = gated(v[1], bf16x2_hi(g.x));
+        v[2] = gated(v[2], bf16x2_lo(g.y));
+        v[3] = gated(v[3], bf16x2_hi(g.y));
+      }
+      if (ahead + row / p.group < 0) v[0] = v[1] = v[2] = v[3] = 0.0f;  // sees no key
+      *reinterpret_cast<uint2*>(output_row<D>(p, token, head, row) + column) =
+          make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
   }
 }
 
@@ -330,111 +508,110 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base;
   const uint32_t tmem_o = tmem + 2 * kKeys;
 
-  find_start(p, scratch);
-  const Start start = scratch.start;
-  Walk walk(p, start);
-  Item it;
+  find_stretch(p, scratch);
+  const Stretch& stretch = scratch.stretch;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
-    int stage = 0, item = 0;
+    int stage = 0;
     uint32_t phase = 1;  // parity to wait for on `empty`: a fresh barrier's earlier phase
     bool ok = true;
+    int items = 0;
     auto advance = [&]() {
       if (++stage == STAGES) {
         stage = 0;
         phase ^= 1;
       }
     };
-    while (ok && walk.next(p, &it)) {
-      if (item > 0) ok = mbar_wait(&q_empty, (item - 1) & 1, p.status);
-      if (!ok) break;
-      const int token = it.seq.start + it.tile * p.tile_tokens;
-      if (elect_one()) {
-        const bool one = it.tokens == 1;
-        const uint32_t bytes = static_cast<uint32_t>(p.group * (one ? 1 : p.tile_tokens) * 128);
-        mbar_arrive_expect_tx(&q_full, bytes * S::CHUNKS);
-        for (int c = 0; c < S::CHUNKS; ++c) {
-          tma_load_4d(smem_q + c * kRows * 128, one ? &map_q1 : &map_q, &q_full, 64 * c, 0, it.head, token);
+    const int per_step = p.block_table ? max(kKeys >> p.page_shift, 1) : 0;  // pages of a step
+    // lane l holds the page of keys [l * page tokens, ...) of the step
+    auto pages_of = [&](int row, int limit, int j) -> int {
+      int id = -1;
+      if (lane < per_step && j * kKeys + (lane << p.page_shift) < limit) {
+        const int index = p.page_shift >= 7 ? j >> (p.page_shift - 7) : j * per_step + lane;
+        if (row >= 0 && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
+        if (id < 0 || id >= p.pages) {
+          id = -1;  // outside the plane: TMA fills zeros
+          atomicOr(p.status, STATUS_BAD_ARGUMENT);
         }
       }
+      return id;
+    };
+    // One unit: `rows` keys from key `key` of step j, of which those in front of `limit` are fetched, in boxes of
+    // `box` keys x `chunks_box` chunks, `chunks` from `chunk` on; each lane asks for a box.
+    auto load_unit = [&](const CUtensorMap* map, int ids, int start, int head, int limit, int j, int key, int rows, int box,
+                         int chunk, int chunks, int chunks_box, int chunk_bytes) {
+      ok = warp_wait(&empty[stage], phase, p.status);
+      if (!ok) return;
+      const int keys = min(rows, limit - j * kKeys - key);
+      const int boxes = max((keys + box - 1) / box, 1), across = chunks / chunks_box;
+      const int b = lane / across, c = lane % across;
+      const int at = key + b * box;  // within the step
+      int page = 0, within = start + j * kKeys + at;
+      if (p.block_table) {
+        page = __shfl_sync(0xffffffffu, ids, p.page_shift >= 7 ? 0 : (at >> p.page_shift) & 31);
+        within = (j * kKeys + at) & ((1 << p.page_shift) - 1);
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * box * chunks * 128));
       __syncwarp();
-      ++item;
-
-      const int row = p.block_table ? (p.table_rows ? p.table_rows[it.sequence] : it.sequence) : 0;
-      const bool row_ok = row >= 0 && row < p.table_row_count;
-      const int per_step = p.block_table ? max(kKeys >> p.page_shift, 1) : 0;  // pages of a step
-      // lane l holds the page of keys [l * page tokens, ...) of the step
-      auto pages_of = [&](int j) -> int {
-        int id = -1;
-        if (lane < per_step) {
-          const int index = p.page_shift >= 7 ? j >> (p.page_shift - 7) : j * per_step + lane;
-          const bool needed = j * kKeys + (lane << p.page_shift) < it.limit;
-          if (needed) {
-            if (row_ok && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
-            if (id < 0 || id >= p.pages) {
-              id = -1;  // outside the plane: TMA fills zeros
-              atomicOr(p.status, STATUS_BAD_ARGUMENT);
-            }
-          }
-        }
-        return id;
-      };
-      // one unit: `rows` keys from key `key` of step j on, `chunks` 64-value columns from `chunk` on
-      auto load_unit = [&](const CUtensorMap* map, int ids, int j, int key, int rows, int chunk, int chunks) {
-        const int keys = min(rows, it.limit - j * kKeys - key);  // of these `keys` exist
-        const int box = p.block_table ? min(rows, 1 << p.page_shift) : rows;
-        const int boxes = max((keys + box - 1) / box, 1);
-        uint8_t* to = ring + stage * kUnit;
-        if (elect_one()) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * box * chunks * 128));
-        __syncwarp();
-        for (int b = 0; b < boxes; ++b) {
-          const int at = key + b * box;  // within the step
-          int page = 0, within;
-          if (p.block_table) {
-            page = __shfl_sync(0xffffffffu, ids, p.page_shift >= 7 ? 0 : at >> p.page_shift);
-            within = (j * kKeys + at) & ((1 << p.page_shift) - 1);
-          } else {
-            within = it.seq.start + j * kKeys + at;
-          }
-          if (elect_one()) {
-            for (int c = 0; c < chunks; ++c) {
-              tma_load_4d(to + c * rows * 128 + b * box * 128, map, &full[stage], 64 * (chunk + c), within, it.head, page);
-            }
+      if (b < boxes) {
+        tma_load_5d(ring + stage * kUnit + c * chunks_box * chunk_bytes + b * box * (chunks_box > 1 ? chunks * 128 : 128), map,
+                    &full[stage], 0, within, chunk + c * chunks_box, head, page);
+      }
+      __syncwarp();
+      advance();
+    };
+    Steps now(p, stretch);
+    int ids = 0, row = 0, ids_before = 0, j_before = 0, limit_before = 0, head_before = 0, start_before = 0;
+    bool more = now.next(p), loaded = false;
+    // K of a step, then V of the step before it: the order in which the MMA warp asks for them
+    while (ok && (more || loaded)) {
+      if (more) {
+        const Item& it = now.it;
+        if (now.opens()) {
+          if (now.item > 0) ok = warp_wait(&q_empty, (now.item - 1) & 1, p.status);
+          if (!ok) break;
+          if (lane < S::CHUNKS) {
+            const bool one = it.tokens == 1;
+            if (lane == 0) mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.group * (one ? 1 : p.tile_tokens) * 128 * S::CHUNKS));
+            __syncwarp((1u << S::CHUNKS) - 1u);
+            tma_load_4d(smem_q + lane * kRows * 128, one ? &map_q1 : &map_q, &q_full, 64 * lane, 0, it.head,
+                        it.seq.start + it.tile * p.tile_tokens);
           }
           __syncwarp();
-        }
-      };
-      int ids = pages_of(it.first), ids_before = 0;
-      // K of step j, then V of step j - 1: the order in which the MMA warp asks for them
-      for (int j = it.first; ok && j <= it.last; ++j) {
-        if (j < it.last) {
-          for (int c = 0; ok && c < S::CHUNKS; ++c) {
-            ok = mbar_wait(&empty[stage], phase, p.status);
-            if (ok) {
-              load_unit(&map_k, ids, j, 0, kKeys, c, 1);
-              advance();
-            }
+          ++items;
+          if (p.block_table) {
+            row = p.table_rows ? p.table_rows[it.sequence] : it.sequence;
+            if (row >= p.table_row_count) row = -1;
+            ids = pages_of(row, it.limit, now.j);
           }
         }
-        if (j > it.first) {
-          const int v = j - 1;
-          const int keys = it.limit - v * kKeys;
-          for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
-            ok = mbar_wait(&empty[stage], phase, p.status);
-            if (ok) {
-              load_unit(&map_v, ids_before, v, u * S::V_KEYS, S::V_KEYS, 0, S::CHUNKS);
-              advance();
-            }
-          }
+        const int k_box = p.block_table ? min(kKeys, 1 << p.page_shift) : kKeys;
+        for (int u = 0; ok && u < S::K_UNITS; ++u) {
+          load_unit(&map_k, ids, it.seq.start, it.head, it.limit, now.j, 0, kKeys, k_box, 2 * u, 2, k_box < kKeys ? 1 : 2, kKeys * 128);
         }
+      }
+      if (loaded) {
+        const int v_box = p.block_table ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
+        for (int u = 0; ok && u < S::V_UNITS && (u == 0 || j_before * kKeys + u * S::V_KEYS < limit_before); ++u) {
+          load_unit(&map_v, ids_before, start_before, head_before, limit_before, j_before, u * S::V_KEYS, S::V_KEYS, v_box, 0,
+                    S::CHUNKS, S::CHUNKS, 0);
+        }
+      }
+      loaded = more;
+      if (more) {
         ids_before = ids;
-        if (j + 1 < it.last) ids = pages_of(j + 1);
+        j_before = now.j;
+        limit_before = now.it.limit;
+        head_before = now.it.head;
+        start_before = now.it.seq.start;
+        more = now.next(p);
+        if (more && !now.opens() && p.block_table) ids = pages_of(row, now.it.limit, now.j);
       }
     }
     if (!ok) {
       // what was asked for lands before the CTA's shared memory is somebody else's
-      for (int n = 0; item > 0 && n < 200000 && !mbar_try_wait(&q_full, (item - 1) & 1); ++n) {
+      for (int n = 0; items > 0 && n < 200000 && !mbar_try_wait(&q_full, (items - 1) & 1); ++n) {
       }
       for (int i = 0; i < STAGES; ++i) {
         for (int n = 0; n < 200000 && !mbar_try_wait(&full[stage], phase); ++n) {
@@ -446,9 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------- MMA
     constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys, false);
     constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, D, true);
-    int stage = 0, item = 0;
+    int stage = 0, n = 0;  // n: steps so far
     uint32_t phase = 0;
-    int n = 0;  // steps so far
     bool ok = true;
     auto advance = [&]() {
       if (++stage == STAGES) {
@@ -457,74 +633,78 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
-    auto scores = [&](int buffer) {  // S[buffer] = Q K^T
-      for (int c = 0; ok && c < S::CHUNKS; ++c) {
-        ok = mbar_wait(&full[stage], phase, p.status);
+    const int v_box = p.block_table ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
+    Steps ahead(p, stretch);
+    // S[buffer] = Q K^T of step `ahead`
+    auto scores = [&](int buffer) {
+      if (ahead.opens()) ok = warp_wait(&q_full, ahead.item & 1, p.status);
+      for (int u = 0; ok && u < S::K_UNITS; ++u) {
+        ok = warp_wait(&full[stage], phase, p.status);
         if (!ok) return;
         if (elect_one()) {
-          const uint64_t a = umma_desc_sw128(q_addr + c * kRows * 128), b = umma_desc_sw128(ring_addr + stage * kUnit);
+          const uint64_t a = umma_desc_sw128(q_addr + u * 2 * kRows * 128), b = umma_desc_sw128(ring_addr + stage * kUnit);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + buffer * kKeys, a + 2 * k, b + 2 * k, idesc_s, c > 0 || k > 0);
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t step = (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3);
+            umma_bf16(tmem + buffer * kKeys, a + step, b + step, idesc_s, u > 0 || k > 0);
+          }
+          umma_commit(&empty[stage]);
+          if (u == S::K_UNITS - 1) {
+            umma_commit(&s_full[buffer]);
+            if (ahead.closes()) umma_commit(&q_empty);
+          }
+        }
+        __syncwarp();
+        advance();
+      }
+    };
+    bool more = ahead.next(p);
+    if (more) scores(0);
+    while (ok && more) {
+      const int buffer = n & 1, keys = ahead.it.limit - ahead.j * kKeys, item = ahead.item;
+      const bool opens = ahead.opens(), closes = ahead.closes();
+      more = ahead.next(p);
+      if (more) scores(buffer ^ 1);
+      if (ok && opens && item > 0) ok = warp_wait(&o_free, (item - 1) & 1, p.status);
+      if (ok) ok = warp_wait(&p_full[buffer], (n >> 1) & 1, p.status);
+      if (!ok) break;
+      tc_fence_after_sync();
+      for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
+        ok = warp_wait(&full[stage], phase, p.status);
+        if (!ok) break;
+        uint8_t* unit = ring + stage * kUnit;
+        const int mine = min(max(keys - u * S::V_KEYS, 0), S::V_KEYS);  // keys of this unit that count
+        const int slices = max((mine + 15) / 16, 1);
+        // key r of the unit: box r / v_box of [chunk][v_box keys][128 bytes]
+        if (mine < slices * 16) {
+          // P is zero for the keys behind the last, but what lies there may be no number: zeros
+          for (int i = lane; i < (slices * 16 - mine) * S::CHUNKS * 8; i += 32) {
+            const int r = mine + i / (S::CHUNKS * 8), c = (i / 8) % S::CHUNKS, piece = i % 8;
+            *reinterpret_cast<uint4*>(unit + (r / v_box * S::CHUNKS + c) * v_box * 128 + r % v_box * 128 + piece * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * kUnit, v_box * 128);
+          for (int k = 0; k < slices; ++k) {
+            const uint32_t r = 16 * k;
+            const uint32_t offset = (r & ~(v_box - 1u)) * S::CHUNKS * 128 + (r & (v_box - 1u)) * 128;
+            umma_bf16_ta(tmem_o, tmem + buffer * kKeys + u * (S::V_KEYS / 2) + 8 * k, b + (offset >> 4), idesc_o,
+                         !opens || u > 0 || k > 0);
+          }
           umma_commit(&empty[stage]);
         }
         __syncwarp();
         advance();
       }
-      if (elect_one()) umma_commit(&s_full[buffer]);
-      __syncwarp();
-    };
-    while (ok && walk.next(p, &it)) {
-      ok = mbar_wait(&q_full, item & 1, p.status);
-      if (!ok) break;
-      scores(n & 1);
-      for (int j = it.first; ok && j < it.last; ++j, ++n) {
-        const int buffer = n & 1;
-        if (j + 1 < it.last) {
-          scores(buffer ^ 1);
-          if (!ok) break;
-        }
-        if (j + 1 >= it.last) {
-          if (elect_one()) umma_commit(&q_empty);  // every product with Q is issued
-          __syncwarp();
-        }
-        if (j == it.first && item > 0) ok = mbar_wait(&o_free, (item - 1) & 1, p.status);
-        if (ok) ok = mbar_wait(&p_full[buffer], (n >> 1) & 1, p.status);
-        if (!ok) break;
-        tc_fence_after_sync();
-        const int keys = it.limit - j * kKeys;
-        for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
-          ok = mbar_wait(&full[stage], phase, p.status);
-          if (!ok) break;
-          uint8_t* unit = ring + stage * kUnit;
-          const int mine = min(max(keys - u * S::V_KEYS, 0), S::V_KEYS);  // keys of this unit that count
-          const int slices = max((mine + 15) / 16, 1);
-          if (mine < slices * 16) {
-            // P is zero for the keys behind the last, but what lies there may be no number: zeros
-            for (int i = lane; i < (slices * 16 - mine) * S::CHUNKS * 8; i += 32) {
-              const int r = mine + i / (S::CHUNKS * 8), c = (i / 8) % S::CHUNKS, piece = i % 8;
-              *reinterpret_cast<uint4*>(unit + c * S::V_KEYS * 128 + r * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          if (elect_one()) {
-            const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * kUnit, S::V_KEYS * 128);
-            for (int k = 0; k < slices; ++k) {
-              umma_bf16_ta(tmem_o, tmem + buffer * kKeys + u * (S::V_KEYS / 2) + 8 * k, b + (2048 >> 4) * k, idesc_o,
-                           j > it.first || u > 0 || k > 0);
-            }
-            umma_commit(&empty[stage]);
-          }
-          __syncwarp();
-          advance();
-        }
-        if (ok && elect_one()) {
-          umma_commit(&pv_done);
-          if (j + 1 >= it.last) umma_commit(&o_full);
-        }
-        __syncwarp();
+      if (ok && elect_one()) {
+        umma_commit(&pv_done);
+        if (closes) umma_commit(&o_full);
       }
-      ++item;
+      __syncwarp();
+      ++n;
     }
     if (!ok) {
       if (elect_one()) umma_commit(&drained);
@@ -540,6 +720,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c = p.scale_log2;
     int n = 0, item = 0;
     bool ok = true;
+    Walk walk(p, stretch);
+    Item it;
     while (ok && walk.next(p, &it)) {
       const int rows = it.tokens * p.group;
       const bool active = quadrant * 32 < rows;
@@ -548,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float reference = -INFINITY, sum = 0.0f;
       for (int j = it.first; j < it.last; ++j, ++n) {
         const int buffer = n & 1;
-        ok = mbar_wait(&s_full[buffer], (n >> 1) & 1, p.status);
+        ok = warp_wait(&s_full[buffer], (n >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after_sync();
         if (active) {
@@ -557,16 +739,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int seen = limit - j * kKeys;
           const bool masked = __any_sync(0xffffffffu, seen < kKeys);
           load_scores(at, masked, seen, s);
-          float top = __uint_as_float(s[0]);
+          float tops[4];
 #pragma unroll
-          for (int k = 1; k < kKeys; ++k) top = fmaxf(top, __uint_as_float(s[k]));
+          for (int k = 0; k < 4; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
+#pragma unroll
+          for (int k = 8; k < kKeys; k += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 4])));
+          }
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           if (j == it.first) {
             reference = top;
           } else {
             const bool grown = (top - reference) * c > 8.0f;
             if (__any_sync(0xffffffffu, grown)) {
               // O of the steps before this one is complete, and none is added until P of this one is
-              ok = mbar_wait(&pv_done, (n - 1) & 1, p.status);
+              ok = warp_wait(&pv_done, (n - 1) & 1, p.status);
               if (!ok) break;
               tc_fence_after_sync();
               const float alpha = grown ? exp2_approx((reference - top) * c) : 1.0f;
@@ -586,15 +775,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float shift = reference == -INFINITY ? 0.0f : reference * c;
-          float part = 0.0f;
+          const F32x2 scale2 = f32x2_splat(c), shift2 = f32x2_splat(-shift);
+          F32x2 sums[2] = {f32x2_splat(0.0f), f32x2_splat(0.0f)};
 #pragma unroll
           for (int k = 0; k < kKeys; k += 2) {
-            const float a = exp2_approx(fmaf(__uint_as_float(s[k]), c, -shift));
-            const float b = exp2_approx(fmaf(__uint_as_float(s[k + 1]), c, -shift));
-            part += a + b;
+            const float2 e = f32x2_parts(fma2(f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale2, shift2));
+            const float a = exp2_approx(e.x), b = exp2_approx(e.y);
+            sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], f32x2(a, b));
             s[k / 2] = pack_bf16x2(a, b);
           }
-          sum += part;
+          const float2 part = f32x2_parts(add2(sums[0], sums[1]));
+          sum += part.x + part.y;
           tmem_st32(at, s);
           tmem_st32(at + 32, s + 32);
           tmem_st_wait();
@@ -604,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[buffer]);
       }
       if (!ok) break;
-      if (item > 0) ok = mbar_wait(&o_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
+      if (item > 0) ok = warp_wait(&o_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
       if (!ok) break;
       row_max[r] = reference == -INFINITY ? -INFINITY : reference * c;
       row_sum[r] = sum;
@@ -618,21 +809,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     int item = 0;
+    Walk walk(p, stretch);
+    Item it;
     bool ok = true;  // a warp whose wait ran out still takes part in the barriers of the four
     while (walk.next(p, &it)) {
-      ok = ok && mbar_wait(&stats_full, item & 1, p.status) && mbar_wait(&o_full, item & 1, p.status);
+      ok = ok && warp_wait(&stats_full, item & 1, p.status) && warp_wait(&o_full, item & 1, p.status);
       tc_fence_after_sync();
       const float m = row_max[r], sum = row_sum[r];
       const int rows = it.tokens * p.group;
       const int tile_token = it.seq.start + it.tile * p.tile_tokens;  // first token row
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens;
-      auto gate_row = [&](int row) {
-        return p.gate + static_cast<size_t>(tile_token + row / p.group) * p.query_token_stride +
-               static_cast<size_t>(it.head * p.group + row % p.group) * p.query_head_stride;
-      };
-      auto output_row = [&](int row) {
-        return p.output + (static_cast<size_t>(tile_token + row / p.group) * p.q_heads + it.head * p.group + row % p.group) * D;
-      };
       const bool whole = it.first == 0 && it.last == it.steps;
       if (whole) {
         const bool blind = ahead + r / p.group < 0;  // sees no key
@@ -644,8 +830,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(tmem_o + lanes + k, o);
             tmem_ld_wait();
             if (r < rows) {
-              uint16_t* out = output_row(r) + k;
-              const uint16_t* gate = p.gate ? gate_row(r) + k : nullptr;
+              uint16_t* out = output_row<D>(p, tile_token, it.head, r) + k;
+              const uint16_t* gate = p.gate ? gate_row(p, tile_token, it.head, r) + k : nullptr;
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
                 float v[8];
@@ -656,8 +842,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const uint32_t w[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = __fdividef(v[2 * i], 1.0f + exp2_approx(bf16x2_lo(w[i]) * -1.4426950408889634f));
-                    v[2 * i + 1] = __fdividef(v[2 * i + 1], 1.0f + exp2_approx(bf16x2_hi(w[i]) * -1.4426950408889634f));
+                    v[2 * i] = gated(v[2 * i], bf16x2_lo(w[i]));
+                    v[2 * i + 1] = gated(v[2 * i + 1], bf16x2_hi(w[i]));
                   }
                 }
                 *reinterpret_cast<uint4*>(out + e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
@@ -670,9 +856,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free);
       } else {
-        const int c0 = cta_of(start.total, start.ctas, it.line), c1 = cta_of(start.total, start.ctas, it.line + it.steps - 1);
-        // a CTA's first item goes to its slot 0, a later one (then its last) to slot 1
-        const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (item == 0 ? 0 : 1);
+        // the CTA that the tile begins in, and the last one that it reaches, with the cuts where they moved to
+        const int margin = cut_margin(rows);
+        const long long inner = it.line + min(margin, it.steps) - 1;
+        const int c0 = cta_of(stretch.total, stretch.ctas, inner);
+        const int c1 = cta_of(stretch.total, stretch.ctas, max(inner, it.line + it.steps - margin));
+        // the part that begins a tile goes to the CTA's slot 1, one that goes on with a tile to slot 0
+        const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (it.first == 0 ? 1 : 0);
         float* part = p.parts + slot * kRows * D;
         if (ok && quadrant * 32 < rows) {
 #pragma unroll 1
@@ -698,42 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_barrier(1, 128);
         if (last_part) {
           __threadfence();
-          const size_t slot0 = 2 * static_cast<size_t>(c0) + (cta_first(start.total, start.ctas, c0) == it.line ? 0 : 1);
-          for (int i = thread; i < rows * (D / 4); i += 128) {
-            const int row = i / (D / 4), column = i % (D / 4) * 4;
-            float top = -INFINITY;
-            for (int k = c0; k <= c1; ++k) {
-              const size_t at = k == c0 ? slot0 : 2 * static_cast<size_t>(k);
-              top = fmaxf(top, __ldcg(&p.part_stats[at * kRows + row]).x);
-            }
-            float total = 0.0f;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int k = c0; k <= c1; ++k) {
-              const size_t at = k == c0 ? slot0 : 2 * static_cast<size_t>(k);
-              const float2 stats = __ldcg(&p.part_stats[at * kRows + row]);
-              // a part without a key of this row has nothing to add, whatever its O holds
-              if (stats.x == -INFINITY && stats.y == 0.0f) continue;
-              const float w = exp2_approx(stats.x - top);
-              const float4 o = __ldcg(reinterpret_cast<const float4*>(p.parts + (at * kRows + row) * D + column));
-              total = fmaf(stats.y, w, total);
-              acc.x = fmaf(o.x, w, acc.x);
-              acc.y = fmaf(o.y, w, acc.y);
-              acc.z = fmaf(o.z, w, acc.z);
-              acc.w = fmaf(o.w, w, acc.w);
-            }
-            const bool blind = ahead + row / p.group < 0;
-            const float scale = 1.0f / total;
-            float v[4] = {acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale};
-            if (p.gate) {
-              const uint2 g = *reinterpret_cast<const uint2*>(gate_row(row) + column);
-              v[0] = __fdividef(v[0], 1.0f + exp2_approx(bf16x2_lo(g.x) * -1.4426950408889634f));
-              v[1] = __fdividef(v[1], 1.0f + exp2_approx(bf16x2_hi(g.x) * -1.4426950408889634f));
-              v[2] = __fdividef(v[2], 1.0f + exp2_approx(bf16x2_lo(g.y) * -1.4426950408889634f));
-              v[3] = __fdividef(v[3], 1.0f + exp2_approx(bf16x2_hi(g.y) * -1.4426950408889634f));
-            }
-            if (blind) v[0] = v[1] = v[2] = v[3] = 0.0f;
-            *reinterpret_cast<uint2*>(output_row(row) + column) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-          }
+          join<D>(p, c0, c1, rows, thread, ahead, tile_token, it.head);
           if (thread == 0) p.tickets[c0] = 0u;
         }
         named_barrier(1, 128);  // `last_part` is written again

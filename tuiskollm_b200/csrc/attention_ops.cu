@@ -266,13 +266,28 @@ Status AttentionOp::launch(cudaStream_t stream, const char* what, int head_dim, 
                                static_cast<uint64_t>(p.query_head_stride) * p.group,
                                static_cast<uint64_t>(p.query_token_stride)};
   const uint32_t group = static_cast<uint32_t>(p.group);
-  TK100_TRY(ctx_.bf16_map(query, dims, strides, {64u, group, 1u, static_cast<uint32_t>(p.tile_tokens)}, &map_q));
-  TK100_TRY(ctx_.bf16_map(query, dims, strides, {64u, group, 1u, 1u}, &map_q1));
+  const uint32_t box[4] = {64u, group, 1u, static_cast<uint32_t>(p.tile_tokens)}, box1[4] = {64u, group, 1u, 1u};
+  TK100_TRY(ctx_.bf16_map(query, 4, dims, strides, box, &map_q));
+  TK100_TRY(ctx_.bf16_map(query, 4, dims, strides, box1, &map_q1));
   DeviceScope device(ctx_);
   TK100_TRY(device.status());
   ctx_.count_launch();
   return ctx_.check(launch_attention(stream, head_dim, ctx_.sm_count(), map_q, map_q1, map_k, map_v, p),
                     (std::string("launching the ") + what).c_str());
+}
+
+// Keys in boxes of up to 128 tokens x 2 chunks of 64 values, one chunk where a page ends inside the 128 (a chunk's
+// 128 keys lie next to each other in shared memory); values in boxes of up to one unit's tokens x the whole head.
+Status AttentionOp::kv_map(const uint16_t* plane, int head_dim, int kv_heads, const CacheGeometry& g, int most_rows,
+                           bool keys, CUtensorMap* out) {
+  const int rows = std::min(most_rows, keys ? 128 : attention_value_box(head_dim));
+  const uint64_t dims[5] = {64u, static_cast<uint64_t>(g.page_tokens), static_cast<uint64_t>(head_dim / 64),
+                            static_cast<uint64_t>(kv_heads), static_cast<uint64_t>(g.pages)};
+  const uint64_t strides[4] = {static_cast<uint64_t>(g.token_stride), 64u, static_cast<uint64_t>(g.head_stride),
+                               static_cast<uint64_t>(g.page_stride)};
+  const uint32_t box[5] = {64u, static_cast<uint32_t>(rows),
+                           static_cast<uint32_t>(!keys ? head_dim / 64 : rows < 128 ? 1 : 2), 1u, 1u};
+  return ctx_.bf16_map(plane, 5, dims, strides, box, out);
 }
 
 Status AttentionOp::paged(cudaStream_t stream, int head_dim, AttentionParams p, const uint16_t* query,
@@ -290,15 +305,9 @@ Status AttentionOp::paged(cudaStream_t stream, int head_dim, AttentionParams p, 
   p.page_shift = log2_of(cache.page_tokens);
   p.pages = cache.pages;
   p.key_capacity = static_cast<int>(std::min(kMaxKeys, static_cast<long long>(p.max_pages) << p.page_shift));
-  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(cache.page_tokens),
-                            static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(cache.pages)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(cache.token_stride), static_cast<uint64_t>(cache.head_stride),
-                               static_cast<uint64_t>(cache.page_stride)};
-  const uint32_t k_box = static_cast<uint32_t>(std::min(128, cache.page_tokens));
-  const uint32_t v_box = static_cast<uint32_t>(std::min(attention_value_box(head_dim), cache.page_tokens));
   CUtensorMap map_k, map_v;
-  TK100_TRY(ctx_.bf16_map(key_cache, dims, strides, {64u, k_box, 1u, 1u}, &map_k));
-  TK100_TRY(ctx_.bf16_map(value_cache, dims, strides, {64u, v_box, 1u, 1u}, &map_v));
+  TK100_TRY(kv_map(key_cache, head_dim, p.kv_heads, cache, cache.page_tokens, true, &map_k));
+  TK100_TRY(kv_map(value_cache, head_dim, p.kv_heads, cache, cache.page_tokens, false, &map_v));
   return launch(stream, what, head_dim, p, query, map_k, map_v);
 }
 
@@ -314,13 +323,10 @@ Status AttentionOp::prompt(cudaStream_t stream, int head_dim, AttentionParams p,
     return refuse(ctx_, what, "the output overlaps the keys or values");
   p.kv_lengths = nullptr;
   p.block_table = nullptr;
-  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(p.tokens),
-                            static_cast<uint64_t>(p.kv_heads), 1u};
-  const uint64_t strides[3] = {static_cast<uint64_t>(kv_token_stride), static_cast<uint64_t>(kv_head_stride),
-                               static_cast<uint64_t>(kv_token_stride)};
+  const CacheGeometry rows = {1, p.tokens, kv_token_stride, kv_token_stride, kv_head_stride};
   CUtensorMap map_k, map_v;
-  TK100_TRY(ctx_.bf16_map(key, dims, strides, {64u, 128u, 1u, 1u}, &map_k));
-  TK100_TRY(ctx_.bf16_map(value, dims, strides, {64u, static_cast<uint32_t>(attention_value_box(head_dim)), 1u, 1u}, &map_v));
+  TK100_TRY(kv_map(key, head_dim, p.kv_heads, rows, 128, true, &map_k));
+  TK100_TRY(kv_map(value, head_dim, p.kv_heads, rows, 128, false, &map_v));
   return launch(stream, what, head_dim, p, query, map_k, map_v);
 }
 

@@ -308,16 +308,20 @@ Status Context::scale_map(const void* base, uint64_t chunks, CUtensorMap* out) {
   return TK100_OK;
 }
 
-Status Context::bf16_map(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                         const uint32_t (&box)[4], CUtensorMap* out) {
+Status Context::bf16_map(const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+                         CUtensorMap* out) {
   auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode_fn_);
-  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
-  const cuuint64_t bytes[3] = {2 * strides[0], 2 * strides[1], 2 * strides[2]};
-  const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
-  const cuuint32_t elem[4] = {1u, 1u, 1u, 1u};
-  CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, bytes, b, elem,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t d[5], bytes[4];
+  cuuint32_t b[5];
+  const cuuint32_t elem[5] = {1u, 1u, 1u, 1u, 1u};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i > 0) bytes[i - 1] = 2 * strides[i - 1];
+  }
+  CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d,
+                      bytes, b, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(TK100_ERR_DRIVER, "[gpu.driver] cuTensorMapEncodeTiled (BF16 heads) failed with CUresult " +
                                       std::to_string(static_cast<int>(r)));

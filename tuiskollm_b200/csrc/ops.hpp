@@ -86,9 +86,9 @@ class Context {
   Status swiglu_map(const void* base, uint64_t outputs, uint64_t row_bytes, CUtensorMap* out);
   Status swiglu_scale_map(const void* base, uint64_t outputs, uint64_t chunks_per_tile, CUtensorMap* out);
 
-  // BF16 tensor of four dimensions (innermost first; strides of the outer three in elements), read in boxes of
-  // box[0] = 64 values with the 128-byte swizzle.  Encoded anew at each launch: activation planes move.
-  Status bf16_map(const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4],
+  // BF16 tensor of `rank` <= 5 dimensions (innermost first; strides of the outer ones in elements), read in boxes
+  // of 64 values and more with the 128-byte swizzle.  Encoded anew at each launch: activation planes move.
+  Status bf16_map(const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
                   CUtensorMap* out);
 
   const tk100_config& config() const { return config_; }
@@ -381,6 +381,8 @@ class AttentionOp {
  private:
   Status prepare(const char* what, int head_dim, AttentionParams* p, const uint16_t* query, const uint16_t* key,
                  const uint16_t* value, float scale, void* workspace);
+  Status kv_map(const uint16_t* plane, int head_dim, int kv_heads, const CacheGeometry& g, int most_rows, bool keys,
+                CUtensorMap* out);
   Status launch(cudaStream_t stream, const char* what, int head_dim, const AttentionParams& p, const uint16_t* query,
                 const CUtensorMap& map_k, const CUtensorMap& map_v);
   Context& ctx_;

@@ -455,7 +455,7 @@ __device__ __forceinline__ void join(const AttentionParams& p, int c0, int c1, i
 
 // ------------------------------------------------------------------------- the kernel
 
-template <int D>
+template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q1,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -523,52 +523,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 1;
       }
     };
-    const int per_step = p.block_table ? max(kKeys >> p.page_shift, 1) : 0;  // pages of a step
-    // lane l holds the page of keys [l * page tokens, ...) of the step
-    auto pages_of = [&](int row, int limit, int j) -> int {
+    // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (both where no page ends inside the 128
+    // keys), V boxes of `v_box` keys and all chunks.  What does not change from step to step:
+    const int shift = p.page_shift;
+    const int k_box = PAGED ? min(kKeys, 1 << shift) : kKeys, v_box = PAGED ? min(S::V_KEYS, 1 << shift) : S::V_KEYS;
+    const bool both = k_box == kKeys;
+    const int k_key = (both ? lane : lane >> 1) * k_box, k_chunk = both ? 0 : lane & 1, v_key = lane * v_box;
+    uint8_t* const k_to = ring + k_chunk * (kKeys * 128) + k_key * 128;
+    uint8_t* const v_to = ring + v_key * S::CHUNKS * 128;
+    const int within_page = PAGED ? (1 << shift) - 1 : -1;
+    // page of key `key` of the sequence in table row `row`; outside the planes -1, where TMA fills zeros
+    auto page_of = [&](int row, int key, bool needed) -> int {
+      if (!PAGED) return 0;
       int id = -1;
-      if (lane < per_step && j * kKeys + (lane << p.page_shift) < limit) {
-        const int index = p.page_shift >= 7 ? j >> (p.page_shift - 7) : j * per_step + lane;
+      if (needed) {
+        const int index = key >> shift;
         if (row >= 0 && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
         if (id < 0 || id >= p.pages) {
-          id = -1;  // outside the plane: TMA fills zeros
+          id = -1;
           atomicOr(p.status, STATUS_BAD_ARGUMENT);
         }
       }
       return id;
     };
-    // One unit: `rows` keys from key `key` of step j, of which those in front of `limit` are fetched, in boxes of
-    // `box` keys x `chunks_box` chunks, `chunks` from `chunk` on; each lane asks for a box.
-    auto load_unit = [&](const CUtensorMap* map, int ids, int start, int head, int limit, int j, int key, int rows, int box,
-                         int chunk, int chunks, int chunks_box, int chunk_bytes) {
-      ok = warp_wait(&empty[stage], phase, p.status);
-      if (!ok) return;
-      const int keys = min(rows, limit - j * kKeys - key);
-      const int boxes = max((keys + box - 1) / box, 1), across = chunks / chunks_box;
-      const int b = lane / across, c = lane % across;
-      const int at = key + b * box;  // within the step
-      int page = 0, within = start + j * kKeys + at;
-      if (p.block_table) {
-        page = __shfl_sync(0xffffffffu, ids, p.page_shift >= 7 ? 0 : (at >> p.page_shift) & 31);
-        within = (j * kKeys + at) & ((1 << p.page_shift) - 1);
+    struct Fetch {  // a step: its first key (as a coordinate for packed rows), how many of its keys exist, pages
+      int base, keys, head, k_page, v_page[S::V_UNITS];
+    };
+    auto fetch_of = [&](const Steps& at, int row) -> Fetch {
+      Fetch f;
+      const int first = at.j * kKeys;
+      f.keys = min(at.it.limit - first, kKeys);
+      f.head = at.it.head;
+      f.base = PAGED ? first : at.it.seq.start + first;
+      f.k_page = page_of(row, first + k_key, k_key < f.keys);
+#pragma unroll
+      for (int u = 0; u < S::V_UNITS; ++u) {
+        const int key = u * S::V_KEYS + v_key;
+        f.v_page[u] = page_of(row, first + key, v_key < S::V_KEYS && key < f.keys);
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * box * chunks * 128));
-      __syncwarp();
-      if (b < boxes) {
-        tma_load_5d(ring + stage * kUnit + c * chunks_box * chunk_bytes + b * box * (chunks_box > 1 ? chunks * 128 : 128), map,
-                    &full[stage], 0, within, chunk + c * chunks_box, head, page);
-      }
-      __syncwarp();
-      advance();
+      return f;
     };
     Steps now(p, stretch);
-    int ids = 0, row = 0, ids_before = 0, j_before = 0, limit_before = 0, head_before = 0, start_before = 0;
+    int row = 0;
+    Fetch fetch{}, earlier{};
     bool more = now.next(p), loaded = false;
+    auto open = [&]() {
+      if (PAGED) {
+        row = p.table_rows ? p.table_rows[now.it.sequence] : now.it.sequence;
+        if (row >= p.table_row_count) row = -1;
+      }
+    };
+    if (more) {
+      open();
+      fetch = fetch_of(now, row);
+    }
     // K of a step, then V of the step before it: the order in which the MMA warp asks for them
     while (ok && (more || loaded)) {
       if (more) {
-        const Item& it = now.it;
         if (now.opens()) {
+          const Item& it = now.it;
           if (now.item > 0) ok = warp_wait(&q_empty, (now.item - 1) & 1, p.status);
           if (!ok) break;
           if (lane < S::CHUNKS) {
@@ -580,33 +593,45 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
           ++items;
-          if (p.block_table) {
-            row = p.table_rows ? p.table_rows[it.sequence] : it.sequence;
-            if (row >= p.table_row_count) row = -1;
-            ids = pages_of(row, it.limit, now.j);
-          }
         }
-        const int k_box = p.block_table ? min(kKeys, 1 << p.page_shift) : kKeys;
-        for (int u = 0; ok && u < S::K_UNITS; ++u) {
-          load_unit(&map_k, ids, it.seq.start, it.head, it.limit, now.j, 0, kKeys, k_box, 2 * u, 2, k_box < kKeys ? 1 : 2, kKeys * 128);
+        const int boxes = max((fetch.keys + k_box - 1) / k_box, 1);
+        const uint32_t bytes = static_cast<uint32_t>(boxes * k_box * 256);
+        const bool mine = k_key < boxes * k_box;
+        const int at = (fetch.base + k_key) & within_page;
+#pragma unroll
+        for (int u = 0; u < S::K_UNITS; ++u) {
+          ok = ok && warp_wait(&empty[stage], phase, p.status);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+          __syncwarp();
+          if (mine) tma_load_5d(k_to + stage * kUnit, &map_k, &full[stage], 0, at, 2 * u + k_chunk, fetch.head, fetch.k_page);
+          advance();
         }
       }
       if (loaded) {
-        const int v_box = p.block_table ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
-        for (int u = 0; ok && u < S::V_UNITS && (u == 0 || j_before * kKeys + u * S::V_KEYS < limit_before); ++u) {
-          load_unit(&map_v, ids_before, start_before, head_before, limit_before, j_before, u * S::V_KEYS, S::V_KEYS, v_box, 0,
-                    S::CHUNKS, S::CHUNKS, 0);
+#pragma unroll
+        for (int u = 0; u < S::V_UNITS; ++u) {
+          const int keys = min(earlier.keys - u * S::V_KEYS, S::V_KEYS);
+          if (u > 0 && keys <= 0) break;
+          ok = ok && warp_wait(&empty[stage], phase, p.status);
+          if (!ok) break;
+          const int boxes = max((keys + v_box - 1) / v_box, 1);
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * v_box * S::CHUNKS * 128));
+          __syncwarp();
+          if (v_key < boxes * v_box)
+            tma_load_5d(v_to + stage * kUnit, &map_v, &full[stage], 0, (earlier.base + u * S::V_KEYS + v_key) & within_page, 0,
+                        earlier.head, earlier.v_page[u]);
+          advance();
         }
       }
       loaded = more;
       if (more) {
-        ids_before = ids;
-        j_before = now.j;
-        limit_before = now.it.limit;
-        head_before = now.it.head;
-        start_before = now.it.seq.start;
+        earlier = fetch;
         more = now.next(p);
-        if (more && !now.opens() && p.block_table) ids = pages_of(row, now.it.limit, now.j);
+        if (more) {
+          if (now.opens()) open();
+          fetch = fetch_of(now, row);
+        }
       }
     }
     if (!ok) {
@@ -633,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
-    const int v_box = p.block_table ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
+    const int v_box = PAGED ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
     Steps ahead(p, stretch);
     // S[buffer] = Q K^T of step `ahead`
     auto scores = [&](int buffer) {
@@ -904,20 +929,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
+template <int D, bool PAGED>
+static cudaError_t prepare_one() {
+  return cudaFuncSetAttribute(attention_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SHARED);
+}
+
 cudaError_t attention_prepare() {
-  cudaError_t e = cudaFuncSetAttribute(attention_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<256>::SHARED);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<128>::SHARED);
+  cudaError_t e = prepare_one<256, true>();
+  if (e == cudaSuccess) e = prepare_one<256, false>();
+  if (e == cudaSuccess) e = prepare_one<128, true>();
+  if (e == cudaSuccess) e = prepare_one<128, false>();
+  return e;
 }
 
 int attention_value_box(int dim) { return kUnit / (2 * dim); }
 
 cudaError_t launch_attention(cudaStream_t stream, int dim, int ctas, const CUtensorMap& map_q, const CUtensorMap& map_q1,
                              const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p) {
-  if (dim == 256) {
-    return launch_kernel(attention_kernel<256>, dim3(ctas), dim3(kThreads), Shape<256>::SHARED, stream, map_q, map_q1, map_k, map_v, p);
-  }
-  return launch_kernel(attention_kernel<128>, dim3(ctas), dim3(kThreads), Shape<128>::SHARED, stream, map_q, map_q1, map_k, map_v, p);
+  auto kernel = p.block_table ? (dim == 256 ? attention_kernel<256, true> : attention_kernel<128, true>)
+                              : (dim == 256 ? attention_kernel<256, false> : attention_kernel<128, false>);
+  return launch_kernel(kernel, dim3(ctas), dim3(kThreads), dim == 256 ? Shape<256>::SHARED : Shape<128>::SHARED, stream,
+                       map_q, map_q1, map_k, map_v, p);
 }
 
 }  // namespace tk100

@@ -34,19 +34,18 @@
 namespace tk100 {
 namespace {
 
-constexpr int kRows = 128;   // rows of a tile
+constexpr int kRows = 128;   // rows of a tile in each CTA of the pair
 constexpr int kKeys = 128;   // keys of a step
 constexpr int kThreads = 320;
-constexpr int kUnit = 32768;  // bytes of a ring stage
 
 template <int D>
 struct Shape {
-  static constexpr int CHUNKS = D / 64;           // 128-byte columns of a row
-  static constexpr int K_UNITS = CHUNKS / 2;      // a K unit is 128 keys x 2 chunks
-  static constexpr int V_KEYS = kUnit / (2 * D);  // a V unit is 64 or 128 keys x all chunks
-  static constexpr int V_UNITS = kKeys / V_KEYS;
-  static constexpr int STAGES = D == 256 ? 5 : 6;
-  static constexpr int SHARED = kRows * 2 * D + STAGES * kUnit + 1024;
+  static constexpr int CHUNKS = D / 64;      // 128-byte columns of a row
+  static constexpr int K_KEYS = kKeys / 2;   // a K unit: half of the keys, all chunks
+  static constexpr int V_CHUNKS = CHUNKS / 2;  // a V unit: all keys, half of the chunks
+  static constexpr int UNIT = K_KEYS * 2 * D;  // bytes of a ring stage
+  static constexpr int STAGES = D == 256 ? 5 : 12;
+  static constexpr int SHARED = kRows * 2 * D + STAGES * UNIT + 1024;
 };
 
 // ---------------------------------------------------------------- the line of steps
@@ -124,24 +123,26 @@ struct Place {
   long long line;
 };
 
-// This CTA's stretch [first, last) of the `total` steps that `ctas` CTAs share, and the places of its ends.
+// This pair's stretch [first, last) of the `total` steps that `pairs` share, and the places of its ends.
 struct Stretch {
   long long total, first, last;
-  int ctas;
+  int pairs;
   Place from, to;  // `to` is of use where it lies inside a tile (step > 0)
 };
 
 // Even cuts of the line.
-__device__ __forceinline__ long long cut(long long total, int ctas, int c) { return c * total / ctas; }
-// CTA whose even stretch holds step u.
-__device__ __forceinline__ int cta_of(long long total, int ctas, long long u) {
-  return static_cast<int>(((u + 1) * ctas - 1) / total);
+__device__ __forceinline__ long long cut(long long total, int pairs, int c) { return c * total / pairs; }
+// Pair whose even stretch holds step u.
+__device__ __forceinline__ int pair_of(long long total, int pairs, long long u) {
+  return static_cast<int>(((u + 1) * pairs - 1) / total);
 }
 // A cut closer than this to an end of the tile it falls into moves there: joining the parts of a tile of 128 rows
 // costs as much as some four steps (their fp32 rows through L2 and back), of a decoded token's as one.
-__device__ __forceinline__ int cut_margin(int rows) { return 1 + rows / 32; }
+__device__ __forceinline__ int cut_margin(const AttentionParams& p, int tokens) {
+  return 1 + min(tokens, p.half_tokens) * p.group / 32;
+}
 
-// One tile, or the part of it that this CTA works on.
+// One tile, or the part of it that this pair works on.
 struct Item {
   Sequence seq;
   int sequence, head, tile;
@@ -162,7 +163,7 @@ __device__ __forceinline__ void describe(const AttentionParams& p, const Sequenc
   it->tokens = min(p.tile_tokens, seq.q - tile * p.tile_tokens);
 }
 
-// The CTA's items.  A tile that it begins and another CTA goes on with comes first: with the tile that it goes on
+// The pair's items.  A tile that it begins and another pair goes on with comes first: with the tile that it goes on
 // with itself, parts are there early and are joined while the whole tiles run.
 struct Walk {
   int sequence, head, tile, step, tiles;
@@ -239,7 +240,7 @@ struct Scratch {
   Stretch stretch;
 };
 
-// Finds the CTA's stretch.  All threads sum up the sequences' steps; the thread that passes a cut names the
+// Finds the pair's stretch.  All threads sum up the sequences' steps; the thread that passes a cut names the
 // sequence, and one warp per cut finds head and tile in it.
 __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh) {
   const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
@@ -269,10 +270,10 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
   }
   before += sum - mine;
   if (total == 0) return;
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + p.min_steps - 1) / p.min_steps));
-  const int c = static_cast<int>(blockIdx.x);
-  if (c >= ctas) return;
-  const long long cuts[2] = {cut(total, ctas, c), cut(total, ctas, c + 1)};
+  const int pairs = static_cast<int>(min(static_cast<long long>(gridDim.x / 2), (total + p.min_steps - 1) / p.min_steps));
+  const int c = static_cast<int>(blockIdx.x / 2);
+  if (c >= pairs) return;
+  const long long cuts[2] = {cut(total, pairs, c), cut(total, pairs, c + 1)};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (before <= cuts[k] && cuts[k] < before + mine) {
@@ -313,7 +314,7 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
       at.step = static_cast<int>(rest);
       at.line = u - rest;
       const int steps = tile_steps(p, q, at.tile);
-      const int margin = cut_margin(min(p.tile_tokens, q.q - at.tile * p.tile_tokens) * p.group);
+      const int margin = cut_margin(p, min(p.tile_tokens, q.q - at.tile * p.tile_tokens));
       if (at.step < margin) {
         at.step = 0;
         u = at.line;
@@ -329,7 +330,7 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
         sh.stretch.from = at;
         sh.stretch.first = u;
         sh.stretch.total = total;
-        sh.stretch.ctas = ctas;
+        sh.stretch.pairs = pairs;
       } else {
         sh.stretch.to = at;
         sh.stretch.last = u;
@@ -364,6 +365,29 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int see
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
+// The same on a barrier that the other CTA's threads arrive on.  The bounded wait reads the clock on its way in, which
+// takes about 2000 cycles: not before the barrier has been looked at for a while.
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  bool done = false;
+#pragma unroll 1
+  for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait_cluster(bar, parity);
+  return __all_sync(0xffffffffu, done || mbar_wait_cluster(bar, parity, status));
+}
+
+// Keys of a step that count, of which the last 16 that are multiplied are not full: those behind them are zeroed.
+__device__ __forceinline__ bool ragged(int keys) { return keys < kKeys && (keys <= 0 || keys % 16 != 0); }
+template <int D>
+__device__ __forceinline__ void zero_behind(uint8_t* unit, int keys, int v_box, int lane) {
+  constexpr int PIECES = Shape<D>::V_CHUNKS * 8;  // of 16 bytes in a row
+  const int first = max(keys, 0), rows = keys <= 0 ? 16 : 16 - keys % 16;
+  for (int i = lane; i < rows * PIECES; i += 32) {
+    const int r = first + i / PIECES, c = (i / 8) % Shape<D>::V_CHUNKS, piece = i % 8;
+    *reinterpret_cast<uint4*>(unit + (r / v_box * Shape<D>::V_CHUNKS + c) * v_box * 128 + r % v_box * 128 + piece * 16) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
 
 // Rows of a tile whose first token row is `token`.
 __device__ __forceinline__ const uint16_t* gate_row(const AttentionParams& p, int token, int head, int row) {
@@ -378,13 +402,13 @@ __device__ __forceinline__ float gated(float v, float gate) {
   return __fdividef(v, 1.0f + exp2_approx(gate * -1.4426950408889634f));
 }
 
-// Joins the parts of a tile that CTAs c0 .. c1 left, in the order of their keys: a thread has four of a row's values
+// Joins the parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left, in the order of their keys: a thread has four of a row's values
 // at a time, and of four such places and four parts all loads are under way together.
 template <int D>
-__device__ __forceinline__ void join(const AttentionParams& p, int c0, int c1, int rows, int thread, int ahead, int token,
-                                     int head) {
+__device__ __forceinline__ void join(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread, int ahead,
+                                     int token, int head) {
   constexpr int PLACES = 4, PARTS = 4;
-  auto slot_of = [&](int k) { return 2 * static_cast<size_t>(k) + (k == c0 ? 1 : 0); };
+  auto slot_of = [&](int k) { return 2 * static_cast<size_t>(2 * k + rank) + (k == c0 ? 1 : 0); };
   const int places = rows * (D / 4);
   for (int base = thread; base < places; base += 128 * PLACES) {
     float top[PLACES], total[PLACES];
@@ -466,30 +490,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem_q + kRows * 2 * D;
 
-  __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done, o_full, o_free, stats_full, drained;
+  // Barriers that both CTAs' loads or threads arrive on are the even CTA's (full, q_full, p_full, o_free); those that
+  // the even CTA's MMA warp commits to are arrived on in both (empty, q_empty, s_full, pv_done, o_full).
+  __shared__ uint64_t full[STAGES], empty[STAGES], tail_full[STAGES];
+  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done, o_full, o_free, stats_full, stats_free, drained;
   __shared__ uint32_t tmem_base;
   __shared__ float row_max[kRows], row_sum[kRows];
   __shared__ int last_part;
   __shared__ Scratch scratch;
 
   const int warp = warp_index(), lane = static_cast<int>(threadIdx.x) & 31;
+  const int rank = static_cast<int>(cluster_cta_rank());
 
   if (warp == 0 && elect_one()) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);
       mbar_init(&empty[i], 1);
+      mbar_init(&tail_full[i], 1);
     }
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
     }
     mbar_init(&pv_done, 1);
     mbar_init(&o_full, 1);
-    mbar_init(&o_free, 4);
+    mbar_init(&o_free, 8);
     mbar_init(&stats_full, 4);
+    mbar_init(&stats_free, 4);
     mbar_init(&drained, 1);
     fence_mbar_init();
     prefetch_tensormap(&map_q);
@@ -497,19 +526,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&map_v);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(&tmem_base, 512);
+    tmem_relinquish_pair();
   }
   pdl_wait();
   pdl_trigger();
   tc_fence_before_sync();
   __syncthreads();
+  cluster_arrive();  // both CTAs' barriers exist before either touches the other's
+  find_stretch(p, scratch);
+  cluster_wait();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_base;
   const uint32_t tmem_o = tmem + 2 * kKeys;
-
-  find_stretch(p, scratch);
   const Stretch& stretch = scratch.stretch;
+  const int v_box = PAGED ? min(kKeys, 1 << p.page_shift) : kKeys;  // keys of a box of V
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
@@ -523,14 +554,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 1;
       }
     };
-    // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (both where no page ends inside the 128
-    // keys), V boxes of `v_box` keys and all chunks.  What does not change from step to step:
+    const uint32_t full_even = mapa_u32(smem_u32(&full[0]), 0), q_full_even = mapa_u32(smem_u32(&q_full), 0);
+    const uint32_t tail_mine = mapa_u32(smem_u32(&tail_full[0]), static_cast<uint32_t>(rank));
+    // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (all chunks where no page ends inside the
+    // 64 keys), V boxes of `v_box` keys and half of the chunks.  What does not change from step to step:
     const int shift = p.page_shift;
-    const int k_box = PAGED ? min(kKeys, 1 << shift) : kKeys, v_box = PAGED ? min(S::V_KEYS, 1 << shift) : S::V_KEYS;
-    const bool both = k_box == kKeys;
-    const int k_key = (both ? lane : lane >> 1) * k_box, k_chunk = both ? 0 : lane & 1, v_key = lane * v_box;
-    uint8_t* const k_to = ring + k_chunk * (kKeys * 128) + k_key * 128;
-    uint8_t* const v_to = ring + v_key * S::CHUNKS * 128;
+    const int k_box = PAGED ? min(S::K_KEYS, 1 << shift) : S::K_KEYS;
+    const bool all = k_box == S::K_KEYS;
+    const int k_key = (all ? lane : lane / S::CHUNKS) * k_box, k_chunk = all ? 0 : lane % S::CHUNKS, v_key = lane * v_box;
+    uint8_t* const k_to = ring + k_chunk * (S::K_KEYS * 128) + k_key * 128;
+    uint8_t* const v_to = ring + v_key * S::V_CHUNKS * 128;
     const int within_page = PAGED ? (1 << shift) - 1 : -1;
     // page of key `key` of the sequence in table row `row`; outside the planes -1, where TMA fills zeros
     auto page_of = [&](int row, int key, bool needed) -> int {
@@ -546,23 +579,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return id;
     };
-    struct Fetch {  // a step: its first key (as a coordinate for packed rows), how many of its keys exist, pages
-      int base, keys, head, k_page, v_page[S::V_UNITS];
+    struct Fetch {  // a step: its first key (as a coordinate for packed rows), how many of its keys count, pages
+      int base, keys, head, k_page, v_page;
     };
     auto fetch_of = [&](const Steps& at, int row) -> Fetch {
       Fetch f;
-      const int first = at.j * kKeys;
+      const int first = at.j * kKeys, k = rank * S::K_KEYS + k_key;
       f.keys = min(at.it.limit - first, kKeys);
       f.head = at.it.head;
       f.base = PAGED ? first : at.it.seq.start + first;
-      f.k_page = page_of(row, first + k_key, k_key < f.keys);
-#pragma unroll
-      for (int u = 0; u < S::V_UNITS; ++u) {
-        const int key = u * S::V_KEYS + v_key;
-        f.v_page[u] = page_of(row, first + key, v_key < S::V_KEYS && key < f.keys);
-      }
+      f.k_page = page_of(row, first + k, k_key < S::K_KEYS && k < f.keys);
+      f.v_page = page_of(row, first + v_key, v_key < f.keys);
       return f;
     };
+    // keys of CTA r's half of K that boxes fetch
+    auto k_fetched = [&](int keys, int r) { return (min(max(keys - r * S::K_KEYS, 0), S::K_KEYS) + k_box - 1) & ~(k_box - 1); };
     Steps now(p, stretch);
     int row = 0;
     Fetch fetch{}, earlier{};
@@ -584,45 +615,53 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Item& it = now.it;
           if (now.item > 0) ok = warp_wait(&q_empty, (now.item - 1) & 1, p.status);
           if (!ok) break;
-          if (lane < S::CHUNKS) {
-            const bool one = it.tokens == 1;
-            if (lane == 0) mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.group * (one ? 1 : p.tile_tokens) * 128 * S::CHUNKS));
-            __syncwarp((1u << S::CHUNKS) - 1u);
-            tma_load_4d(smem_q + lane * kRows * 128, one ? &map_q1 : &map_q, &q_full, 64 * lane, 0, it.head,
-                        it.seq.start + it.tile * p.tile_tokens);
+          const int mine = min(it.tokens - rank * p.half_tokens, p.half_tokens);  // tokens of this CTA's rows
+          if (rank == 0 && lane == 0) {
+            const int other = min(max(it.tokens - p.half_tokens, 0), p.half_tokens);
+            const int tokens = (mine == 1 ? 1 : p.half_tokens) + (other <= 1 ? other : p.half_tokens);
+            mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.group * tokens * 128 * S::CHUNKS));
+          }
+          if (lane < S::CHUNKS && mine > 0) {
+            tma_load_4d_pair(smem_q + lane * kRows * 128, mine == 1 ? &map_q1 : &map_q, q_full_even, 64 * lane, 0, it.head,
+                             it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens);
           }
           __syncwarp();
           ++items;
         }
-        const int boxes = max((fetch.keys + k_box - 1) / k_box, 1);
-        const uint32_t bytes = static_cast<uint32_t>(boxes * k_box * 256);
-        const bool mine = k_key < boxes * k_box;
-        const int at = (fetch.base + k_key) & within_page;
-#pragma unroll
-        for (int u = 0; u < S::K_UNITS; ++u) {
-          ok = ok && warp_wait(&empty[stage], phase, p.status);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-          __syncwarp();
-          if (mine) tma_load_5d(k_to + stage * kUnit, &map_k, &full[stage], 0, at, 2 * u + k_chunk, fetch.head, fetch.k_page);
-          advance();
+        ok = warp_wait(&empty[stage], phase, p.status);
+        if (!ok) break;
+        if (lane == 0) {
+          if (rank == 0) {
+            mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>((k_fetched(fetch.keys, 0) + k_fetched(fetch.keys, 1)) * 2 * D));
+          } else {
+            mbar_arrive_remote_light(full_even + stage * 8);
+          }
         }
+        if (k_key < k_fetched(fetch.keys, rank))
+          tma_load_5d_pair(k_to + stage * S::UNIT, &map_k, full_even + stage * 8, 0,
+                           (fetch.base + rank * S::K_KEYS + k_key) & within_page, k_chunk, fetch.head, fetch.k_page);
+        __syncwarp();
+        advance();
       }
       if (loaded) {
-#pragma unroll
-        for (int u = 0; u < S::V_UNITS; ++u) {
-          const int keys = min(earlier.keys - u * S::V_KEYS, S::V_KEYS);
-          if (u > 0 && keys <= 0) break;
-          ok = ok && warp_wait(&empty[stage], phase, p.status);
-          if (!ok) break;
-          const int boxes = max((keys + v_box - 1) / v_box, 1);
-          if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(boxes * v_box * S::CHUNKS * 128));
-          __syncwarp();
-          if (v_key < boxes * v_box)
-            tma_load_5d(v_to + stage * kUnit, &map_v, &full[stage], 0, (earlier.base + u * S::V_KEYS + v_key) & within_page, 0,
-                        earlier.head, earlier.v_page[u]);
-          advance();
+        ok = warp_wait(&empty[stage], phase, p.status);
+        if (!ok) break;
+        const int fetched = (max(earlier.keys, 0) + v_box - 1) & ~(v_box - 1);
+        const bool tail = ragged(earlier.keys);  // goes to this CTA's own barrier, `full` is arrived on behind the zeros
+        if (lane == 0) {
+          if (tail) {
+            mbar_arrive_expect_tx(&tail_full[stage], static_cast<uint32_t>(fetched * D));
+          } else if (rank == 0) {
+            mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(fetched * 2 * D));
+          } else {
+            mbar_arrive_remote_light(full_even + stage * 8);
+          }
         }
+        if (v_key < fetched)
+          tma_load_5d_pair(v_to + stage * S::UNIT, &map_v, (tail ? tail_mine : full_even) + stage * 8, 0,
+                           (earlier.base + v_key) & within_page, rank * S::V_CHUNKS, earlier.head, earlier.v_page);
+        __syncwarp();
+        advance();
       }
       loaded = more;
       if (more) {
@@ -635,21 +674,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) {
-      // what was asked for lands before the CTA's shared memory is somebody else's
-      for (int n = 0; items > 0 && n < 200000 && !mbar_try_wait(&q_full, (items - 1) & 1); ++n) {
+      // what was asked for lands before a CTA's shared memory is somebody else's; both leave together
+      for (int n = 0; rank == 0 && items > 0 && n < 200000 && !mbar_try_wait(&q_full, (items - 1) & 1); ++n) {
       }
       for (int i = 0; i < STAGES; ++i) {
-        for (int n = 0; n < 200000 && !mbar_try_wait(&full[stage], phase); ++n) {
+        for (int n = 0; rank == 0 && n < 200000 && !mbar_try_wait(&full[stage], phase); ++n) {
         }
         advance();
       }
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);  // what counts on other barriers
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------------- MMA
-    constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys, false);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, D, true);
+    constexpr uint32_t idesc_s = umma_idesc_bf16(2 * kRows, kKeys, false);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(2 * kRows, D, true);
     int stage = 0, n = 0;  // n: steps so far
-    uint32_t phase = 0;
+    uint32_t phase = 0, tail_phase = 0;
     bool ok = true;
     auto advance = [&]() {
       if (++stage == STAGES) {
@@ -658,99 +698,104 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
-    const int v_box = PAGED ? min(S::V_KEYS, 1 << p.page_shift) : S::V_KEYS;
-    Steps ahead(p, stretch);
-    // S[buffer] = Q K^T of step `ahead`
+    Steps next(p, stretch);
+    // S[buffer] = Q K^T of step `next`
     auto scores = [&](int buffer) {
-      if (ahead.opens()) ok = warp_wait(&q_full, ahead.item & 1, p.status);
-      for (int u = 0; ok && u < S::K_UNITS; ++u) {
-        ok = warp_wait(&full[stage], phase, p.status);
-        if (!ok) return;
-        if (elect_one()) {
-          const uint64_t a = umma_desc_sw128(q_addr + u * 2 * kRows * 128), b = umma_desc_sw128(ring_addr + stage * kUnit);
+      if (next.opens()) ok = warp_wait(&q_full, next.item & 1, p.status);
+      ok = ok && warp_wait_cluster(&full[stage], phase, p.status);
+      if (!ok) return;
+      if (elect_one()) {
+        const uint64_t a = umma_desc_sw128(q_addr), b = umma_desc_sw128(ring_addr + stage * S::UNIT);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t step = (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3);
-            umma_bf16(tmem + buffer * kKeys, a + step, b + step, idesc_s, u > 0 || k > 0);
-          }
-          umma_commit(&empty[stage]);
-          if (u == S::K_UNITS - 1) {
-            umma_commit(&s_full[buffer]);
-            if (ahead.closes()) umma_commit(&q_empty);
-          }
+        for (int k = 0; k < 4 * S::CHUNKS; ++k) {
+          umma_bf16_pair(tmem + buffer * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3),
+                         b + (k >> 2) * (S::K_KEYS * 128 >> 4) + 2 * (k & 3), idesc_s, k > 0);
         }
-        __syncwarp();
-        advance();
-      }
-    };
-    bool more = ahead.next(p);
-    if (more) scores(0);
-    while (ok && more) {
-      const int buffer = n & 1, keys = ahead.it.limit - ahead.j * kKeys, item = ahead.item;
-      const bool opens = ahead.opens(), closes = ahead.closes();
-      more = ahead.next(p);
-      if (more) scores(buffer ^ 1);
-      if (ok && opens && item > 0) ok = warp_wait(&o_free, (item - 1) & 1, p.status);
-      if (ok) ok = warp_wait(&p_full[buffer], (n >> 1) & 1, p.status);
-      if (!ok) break;
-      tc_fence_after_sync();
-      for (int u = 0; ok && u < S::V_UNITS && (u == 0 || u * S::V_KEYS < keys); ++u) {
-        ok = warp_wait(&full[stage], phase, p.status);
-        if (!ok) break;
-        uint8_t* unit = ring + stage * kUnit;
-        const int mine = min(max(keys - u * S::V_KEYS, 0), S::V_KEYS);  // keys of this unit that count
-        const int slices = max((mine + 15) / 16, 1);
-        // key r of the unit: box r / v_box of [chunk][v_box keys][128 bytes]
-        if (mine < slices * 16) {
-          // P is zero for the keys behind the last, but what lies there may be no number: zeros
-          for (int i = lane; i < (slices * 16 - mine) * S::CHUNKS * 8; i += 32) {
-            const int r = mine + i / (S::CHUNKS * 8), c = (i / 8) % S::CHUNKS, piece = i % 8;
-            *reinterpret_cast<uint4*>(unit + (r / v_box * S::CHUNKS + c) * v_box * 128 + r % v_box * 128 + piece * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        if (elect_one()) {
-          const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * kUnit, v_box * 128);
-          for (int k = 0; k < slices; ++k) {
-            const uint32_t r = 16 * k;
-            const uint32_t offset = (r & ~(v_box - 1u)) * S::CHUNKS * 128 + (r & (v_box - 1u)) * 128;
-            umma_bf16_ta(tmem_o, tmem + buffer * kKeys + u * (S::V_KEYS / 2) + 8 * k, b + (offset >> 4), idesc_o,
-                         !opens || u > 0 || k > 0);
-          }
-          umma_commit(&empty[stage]);
-        }
-        __syncwarp();
-        advance();
-      }
-      if (ok && elect_one()) {
-        umma_commit(&pv_done);
-        if (closes) umma_commit(&o_full);
+        umma_commit_pair(&empty[stage]);
+        umma_commit_pair(&s_full[buffer]);
+        if (next.closes()) umma_commit_pair(&q_empty);
       }
       __syncwarp();
+      advance();
+    };
+    bool more = next.next(p);
+    if (more) scores(0);
+    while (ok && more) {
+      const int buffer = n & 1, keys = next.it.limit - next.j * kKeys, item = next.item;
+      const bool opens = next.opens(), closes = next.closes();
+      more = next.next(p);
+      if (more) scores(buffer ^ 1);
+      if (!ok) break;
+      if (ragged(keys)) {
+        // P is zero for the keys behind the last, but what lies there may be no number
+        ok = warp_wait(&tail_full[stage], (tail_phase >> stage) & 1, p.status);
+        if (!ok) break;
+        tail_phase ^= 1u << stage;
+        zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
+        if (lane == 0) mbar_arrive(&full[stage]);
+      }
+      if (opens && item > 0) ok = warp_wait_cluster(&o_free, (item - 1) & 1, p.status);
+      ok = ok && warp_wait_cluster(&full[stage], phase, p.status) && warp_wait_cluster(&p_full[buffer], (n >> 1) & 1, p.status);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * S::UNIT, v_box * 128);
+        const int slices = keys <= 0 ? 1 : min((keys + 15) / 16, kKeys / 16);
+        for (int k = 0; k < slices; ++k) {
+          const uint32_t r = 16 * k;  // box r / v_box of [chunk][v_box keys][128 bytes]
+          const uint32_t offset = (r & ~(v_box - 1u)) * S::V_CHUNKS * 128 + (r & (v_box - 1u)) * 128;
+          umma_bf16_ta_pair(tmem_o, tmem + buffer * kKeys + 8 * k, b + (offset >> 4), idesc_o, !opens || k > 0);
+        }
+        umma_commit_pair(&empty[stage]);
+        umma_commit_pair(&pv_done);
+        if (closes) umma_commit_pair(&o_full);
+      }
+      __syncwarp();
+      advance();
       ++n;
     }
     if (!ok) {
-      if (elect_one()) umma_commit(&drained);
+      if (elect_one()) umma_commit_pair(&drained);
       __syncwarp();
       for (int i = 0; i < 200000 && !mbar_try_wait(&drained, 0); ++i) {
       }
     }
-  } else if (warp >= 2 && warp < 6) {
+  } else if (warp == 1) {
+    // ------------------------------------------- zeros behind the odd CTA's last keys
+    const uint32_t full_even = mapa_u32(smem_u32(&full[0]), 0);
+    uint32_t tail_phase = 0;
+    int stage = 0;
+    auto advance = [&]() { stage = stage + 1 == STAGES ? 0 : stage + 1; };
+    Steps next(p, stretch);
+    bool more = next.next(p);
+    if (more) advance();
+    while (more) {
+      const int keys = next.it.limit - next.j * kKeys;
+      more = next.next(p);
+      if (more) advance();
+      if (ragged(keys)) {
+        if (!warp_wait(&tail_full[stage], (tail_phase >> stage) & 1, p.status)) break;
+        tail_phase ^= 1u << stage;
+        zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
+        if (lane == 0) mbar_arrive_remote(full_even + stage * 8);
+      }
+      advance();
+    }
+  } else if (warp < 6) {
     // ----------------------------------------------------------------- softmax
     const int quadrant = warp & 3;  // the TMEM lanes this warp may touch
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     const float c = p.scale_log2;
+    const uint32_t p_full_even = mapa_u32(smem_u32(&p_full[0]), 0);
     int n = 0, item = 0;
     bool ok = true;
     Walk walk(p, stretch);
     Item it;
     while (ok && walk.next(p, &it)) {
-      const int rows = it.tokens * p.group;
+      const int rows = min(it.tokens - rank * p.half_tokens, p.half_tokens) * p.group;
       const bool active = quadrant * 32 < rows;
-      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens;
+      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
       const int limit = ahead + r / p.group + 1;  // keys this row sees
       float reference = -INFINITY, sum = 0.0f;
       for (int j = it.first; j < it.last; ++j, ++n) {
@@ -817,10 +862,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[buffer]);
+        if (lane == 0) mbar_arrive_remote_light(p_full_even + buffer * 8);
       }
       if (!ok) break;
-      if (item > 0) ok = warp_wait(&o_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
+      if (item > 0) ok = warp_wait(&stats_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
       if (!ok) break;
       row_max[r] = reference == -INFINITY ? -INFINITY : reference * c;
       row_sum[r] = sum;
@@ -833,6 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 192;
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+    const uint32_t o_free_even = mapa_u32(smem_u32(&o_free), 0);
     int item = 0;
     Walk walk(p, stretch);
     Item it;
@@ -841,9 +887,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && warp_wait(&stats_full, item & 1, p.status) && warp_wait(&o_full, item & 1, p.status);
       tc_fence_after_sync();
       const float m = row_max[r], sum = row_sum[r];
-      const int rows = it.tokens * p.group;
-      const int tile_token = it.seq.start + it.tile * p.tile_tokens;  // first token row
-      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens;
+      const int rows = min(it.tokens - rank * p.half_tokens, p.half_tokens) * p.group;  // of this CTA, below 1: none
+      const int tile_token = it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens;  // first token row
+      const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
       const bool whole = it.first == 0 && it.last == it.steps;
       if (whole) {
         const bool blind = ahead + r / p.group < 0;  // sees no key
@@ -879,13 +925,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free);
+        if (lane == 0) {
+          mbar_arrive_remote_light(o_free_even);
+          mbar_arrive(&stats_free);
+        }
       } else {
-        // the CTA that the tile begins in, and the last one that it reaches, with the cuts where they moved to
-        const int margin = cut_margin(rows);
+        // the pair that the tile begins in, and the last one that it reaches, with the cuts where they moved to
+        const int margin = cut_margin(p, it.tokens);
         const long long inner = it.line + min(margin, it.steps) - 1;
-        const int c0 = cta_of(stretch.total, stretch.ctas, inner);
-        const int c1 = cta_of(stretch.total, stretch.ctas, max(inner, it.line + it.steps - margin));
+        const int c0 = pair_of(stretch.total, stretch.pairs, inner);
+        const int c1 = pair_of(stretch.total, stretch.pairs, max(inner, it.line + it.steps - margin));
         // the part that begins a tile goes to the CTA's slot 1, one that goes on with a tile to slot 0
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (it.first == 0 ? 1 : 0);
         float* part = p.parts + slot * kRows * D;
@@ -906,15 +955,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free);
+        if (lane == 0) {
+          mbar_arrive_remote_light(o_free_even);
+          mbar_arrive(&stats_free);
+        }
         __threadfence();
         named_barrier(1, 128);
-        if (thread == 0) last_part = atomicAdd(&p.tickets[c0], 1u) == static_cast<unsigned>(c1 - c0);
+        unsigned int* ticket = p.tickets + 2 * c0 + rank;
+        if (thread == 0) last_part = rows > 0 && atomicAdd(ticket, 1u) == static_cast<unsigned>(c1 - c0);
         named_barrier(1, 128);
         if (last_part) {
           __threadfence();
-          join<D>(p, c0, c1, rows, thread, ahead, tile_token, it.head);
-          if (thread == 0) p.tickets[c0] = 0u;
+          join<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head);
+          if (thread == 0) *ticket = 0u;
         }
         named_barrier(1, 128);  // `last_part` is written again
       }
@@ -924,7 +977,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  cluster_arrive();  // nothing of the other CTA's works on this one's memory any more
+  cluster_wait();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 }  // namespace
@@ -942,14 +997,13 @@ cudaError_t attention_prepare() {
   return e;
 }
 
-int attention_value_box(int dim) { return kUnit / (2 * dim); }
 
-cudaError_t launch_attention(cudaStream_t stream, int dim, int ctas, const CUtensorMap& map_q, const CUtensorMap& map_q1,
+cudaError_t launch_attention(cudaStream_t stream, int dim, int pairs, const CUtensorMap& map_q, const CUtensorMap& map_q1,
                              const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p) {
   auto kernel = p.block_table ? (dim == 256 ? attention_kernel<256, true> : attention_kernel<128, true>)
                               : (dim == 256 ? attention_kernel<256, false> : attention_kernel<128, false>);
-  return launch_kernel(kernel, dim3(ctas), dim3(kThreads), dim == 256 ? Shape<256>::SHARED : Shape<128>::SHARED, stream,
-                       map_q, map_q1, map_k, map_v, p);
+  return launch_kernel_cluster(kernel, dim3(2 * pairs), dim3(kThreads), dim == 256 ? Shape<256>::SHARED : Shape<128>::SHARED,
+                               stream, dim3(2, 1, 1), map_q, map_q1, map_k, map_v, p);
 }
 
 }  // namespace tk100

@@ -245,7 +245,8 @@ Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, 
     if (out.meets(gate)) return refuse(ctx_, what, "the output overlaps the gate");
   }
   p->group = p->q_heads / p->kv_heads;
-  p->tile_tokens = kAttentionRows / p->group;
+  p->half_tokens = kAttentionRows / p->group;
+  p->tile_tokens = 2 * p->half_tokens;
   p->scale_log2 = scale * 1.4426950408889634f;
   p->min_steps = 1;
   uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -266,27 +267,27 @@ Status AttentionOp::launch(cudaStream_t stream, const char* what, int head_dim, 
                                static_cast<uint64_t>(p.query_head_stride) * p.group,
                                static_cast<uint64_t>(p.query_token_stride)};
   const uint32_t group = static_cast<uint32_t>(p.group);
-  const uint32_t box[4] = {64u, group, 1u, static_cast<uint32_t>(p.tile_tokens)}, box1[4] = {64u, group, 1u, 1u};
+  const uint32_t box[4] = {64u, group, 1u, static_cast<uint32_t>(p.half_tokens)}, box1[4] = {64u, group, 1u, 1u};
   TK100_TRY(ctx_.bf16_map(query, 4, dims, strides, box, &map_q));
   TK100_TRY(ctx_.bf16_map(query, 4, dims, strides, box1, &map_q1));
   DeviceScope device(ctx_);
   TK100_TRY(device.status());
   ctx_.count_launch();
-  return ctx_.check(launch_attention(stream, head_dim, ctx_.sm_count(), map_q, map_q1, map_k, map_v, p),
+  return ctx_.check(launch_attention(stream, head_dim, ctx_.sm_count() / 2, map_q, map_q1, map_k, map_v, p),
                     (std::string("launching the ") + what).c_str());
 }
 
-// Keys in boxes of up to 128 tokens x 2 chunks of 64 values, one chunk where a page ends inside the 128 (a chunk's
-// 128 keys lie next to each other in shared memory); values in boxes of up to one unit's tokens x the whole head.
+// Keys in boxes of up to 64 tokens x all chunks of 64 values, one chunk where a page ends inside the 64 (a chunk's
+// 64 keys lie next to each other in shared memory); values in boxes of up to 128 tokens x half of a head.
 Status AttentionOp::kv_map(const uint16_t* plane, int head_dim, int kv_heads, const CacheGeometry& g, int most_rows,
                            bool keys, CUtensorMap* out) {
-  const int rows = std::min(most_rows, keys ? 128 : attention_value_box(head_dim));
+  const int rows = std::min(most_rows, keys ? 64 : 128);
   const uint64_t dims[5] = {64u, static_cast<uint64_t>(g.page_tokens), static_cast<uint64_t>(head_dim / 64),
                             static_cast<uint64_t>(kv_heads), static_cast<uint64_t>(g.pages)};
   const uint64_t strides[4] = {static_cast<uint64_t>(g.token_stride), 64u, static_cast<uint64_t>(g.head_stride),
                                static_cast<uint64_t>(g.page_stride)};
   const uint32_t box[5] = {64u, static_cast<uint32_t>(rows),
-                           static_cast<uint32_t>(!keys ? head_dim / 64 : rows < 128 ? 1 : 2), 1u, 1u};
+                           static_cast<uint32_t>(!keys ? head_dim / 128 : rows < 64 ? 1 : head_dim / 64), 1u, 1u};
   return ctx_.bf16_map(plane, 5, dims, strides, box, out);
 }
 

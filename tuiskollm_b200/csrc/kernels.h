@@ -432,8 +432,9 @@ struct RotaryParams {
 cudaError_t launch_rotary(cudaStream_t stream, int dim, const RotaryParams& p);
 
 struct AttentionParams {
-  int sequences, tokens, q_heads, kv_heads, group, tile_tokens;
-  int min_steps;               // 128-key steps that a CTA takes at least
+  int sequences, tokens, q_heads, kv_heads, group;
+  int half_tokens, tile_tokens;  // tokens of the rows of one CTA, of both
+  int min_steps;               // 128-key steps that a pair takes at least
   const int32_t* starts;       // [sequences + 1]
   const int32_t* kv_lengths;   // null: as many keys as new tokens
   int key_capacity;            // keys that the block table has room for
@@ -450,8 +451,7 @@ struct AttentionParams {
   uint32_t* status;
 };
 cudaError_t attention_prepare();
-int attention_value_box(int dim);  // keys of a box of the value map
-cudaError_t launch_attention(cudaStream_t stream, int dim, int ctas, const CUtensorMap& map_q, const CUtensorMap& map_q1,
+cudaError_t launch_attention(cudaStream_t stream, int dim, int pairs, const CUtensorMap& map_q, const CUtensorMap& map_q1,
                              const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p);
 
 }  // namespace tk100

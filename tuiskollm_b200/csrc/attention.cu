@@ -48,30 +48,7 @@ struct Shape {
   static constexpr int SHARED = kRows * 2 * D + STAGES * UNIT + 1024;
 };
 
-// ---------------------------------------------------------------- the line of steps
-
-// Sum over k < n of floor((a k + b) / m): the lattice points under a line, by the Euclidean algorithm on (a, m).
-__device__ __forceinline__ long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  long long sum = 0;
-  while (n > 0) {
-    if (a >= m) {
-      sum += static_cast<long long>(n) * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += static_cast<long long>(n) * (b / m);
-      b %= m;
-    }
-    const unsigned top = a * n + b;  // below the number of keys
-    if (top < m) break;
-    n = top / m;
-    b = top % m;
-    const unsigned t = m;
-    m = a;
-    a = t;
-  }
-  return sum;
-}
+// ----------------------------------------------------------------- the line of keys
 
 struct Sequence {
   int start, q, kv;  // first token row, new tokens, keys
@@ -97,45 +74,44 @@ __device__ __forceinline__ int tile_count(const AttentionParams& p, const Sequen
   return (s.q + p.tile_tokens - 1) / p.tile_tokens;
 }
 
-// Steps of the first i tiles of one key/value head.
-__device__ __forceinline__ long long steps_before(const AttentionParams& p, const Sequence& s, int i) {
-  const int tiles = tile_count(p, s);
-  long long sum = 0;
-  int full = i;  // tiles that end at their own (i + 1) tile_tokens
+// What a tile costs besides its keys, in keys: the last step is half empty on average, and a tile's first scores and
+// last rows are not all hidden behind its neighbours' steps.
+constexpr int kTileKeys = 192;
+
+__device__ __forceinline__ int tile_cost(const AttentionParams& p, const Sequence& s, int i) {
+  return kTileKeys + tile_limit(p, s, i);
+}
+// Cost of the first i tiles of one key/value head, an arithmetic series but for tiles that see nothing and the last.
+__device__ __forceinline__ long long cost_before(const AttentionParams& p, const Sequence& s, int i, int tiles) {
+  long long sum = static_cast<long long>(i) * kTileKeys;
+  int full = i;  // tiles whose last token is their own
   if (i == tiles && i > 0) {
-    sum = tile_steps(p, s, i - 1);
+    sum += max(s.kv, 0);
     --full;
   }
   const int ahead = s.kv - s.q;  // keys in front of the first new token
-  // tiles of one step: ahead + (j + 1) tile_tokens <= 128
-  const int ones = min(max(ahead > kKeys ? 0 : (kKeys - ahead) / p.tile_tokens, 0), full);
-  sum += ones;
-  if (full > ones) {
-    const int b = ahead + (ones + 1) * p.tile_tokens + kKeys - 1;  // > 2 * 128 - 1
-    sum += floor_sum(static_cast<unsigned>(full - ones), kKeys, static_cast<unsigned>(p.tile_tokens), static_cast<unsigned>(b));
-  }
-  return sum;
+  const int blind = ahead < 0 ? min(-ahead / p.tile_tokens, full) : 0;
+  return sum + static_cast<long long>(full - blind) * ahead +
+         static_cast<long long>(p.tile_tokens) * (static_cast<long long>(full) * (full + 1) - static_cast<long long>(blind) * (blind + 1)) / 2;
 }
 
-// A place in the line: step `step` of a tile, whose step 0 is at `line`.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// Step `step` of a tile that begins at `line`.
 struct Place {
   int sequence, head, tile, step;
   long long line;
 };
 
-// This pair's stretch [first, last) of the `total` steps that `pairs` share, and the places of its ends.
+// This pair's stretch of the line, from one place up to another; `share` keys belong to each pair before cuts move.
 struct Stretch {
-  long long total, first, last;
-  int pairs;
-  Place from, to;  // `to` is of use where it lies inside a tile (step > 0)
+  long long share;
+  Place from, to;
 };
 
-// Even cuts of the line.
-__device__ __forceinline__ long long cut(long long total, int pairs, int c) { return c * total / pairs; }
-// Pair whose even stretch holds step u.
-__device__ __forceinline__ int pair_of(long long total, int pairs, long long u) {
-  return static_cast<int>(((u + 1) * pairs - 1) / total);
-}
 // A cut closer than this to an end of the tile it falls into moves there: joining the parts of a tile of 128 rows
 // costs as much as some four steps (their fp32 rows through L2 and back), of a decoded token's as one.
 __device__ __forceinline__ int cut_margin(const AttentionParams& p, int tokens) {
@@ -149,17 +125,18 @@ struct Item {
   int first, last, steps;  // its steps [first, last) of `steps`
   int limit;               // keys its last token sees
   int tokens;              // tokens of the tile
-  long long line;          // place of its step 0 in the line
+  long long line;          // where it begins
 };
 
 __device__ __forceinline__ void describe(const AttentionParams& p, const Sequence& seq, int sequence, int head, int tile,
-                                         Item* it) {
+                                         long long line, Item* it) {
   it->seq = seq;
   it->sequence = sequence;
   it->head = head;
   it->tile = tile;
-  it->steps = tile_steps(p, seq, tile);
+  it->line = line;
   it->limit = tile_limit(p, seq, tile);
+  it->steps = max((it->limit + kKeys - 1) / kKeys, 1);
   it->tokens = min(p.tile_tokens, seq.q - tile * p.tile_tokens);
 }
 
@@ -167,32 +144,28 @@ __device__ __forceinline__ void describe(const AttentionParams& p, const Sequenc
 // with itself, parts are there early and are joined while the whole tiles run.
 struct Walk {
   int sequence, head, tile, step, tiles;
-  long long at, end;
+  long long line;
   Sequence seq;
-  Place tail;
-  bool has_tail;
+  Place to;
 
   __device__ __forceinline__ Walk(const AttentionParams& p, const Stretch& s)
-      : sequence(s.from.sequence), head(s.from.head), tile(s.from.tile), step(s.from.step), tiles(0), at(s.first),
-        end(s.last), tail(s.to) {
+      : sequence(s.from.sequence), head(s.from.head), tile(s.from.tile), step(s.from.step), tiles(0), line(s.from.line),
+        to(s.to) {
     seq = {0, 0, 0};
-    has_tail = at < end && tail.step > 0 && tail.line >= at;
-    if (has_tail) end = tail.line;
-    if (at < end) {
+    if (line < to.line) {
       seq = read_sequence(p, sequence);
       tiles = tile_count(p, seq);
     }
   }
   __device__ __forceinline__ bool next(const AttentionParams& p, Item* it) {
-    if (has_tail) {
-      has_tail = false;
-      describe(p, read_sequence(p, tail.sequence), tail.sequence, tail.head, tail.tile, it);
-      it->first = 0;
-      it->last = tail.step;
-      it->line = tail.line;
+    if (to.step > 0) {
+      describe(p, read_sequence(p, to.sequence), to.sequence, to.head, to.tile, to.line, it);
+      it->first = to.line == line ? step : 0;  // both ends in one tile: its only item
+      it->last = to.step;
+      to.step = 0;
       return true;
     }
-    if (at >= end) return false;
+    if (line >= to.line) return false;
     while (tile >= tiles) {  // the next head, or the next sequence that has tokens
       tile = 0;
       if (tiles == 0 || ++head == p.kv_heads) {
@@ -202,11 +175,10 @@ struct Walk {
         tiles = tile_count(p, seq);
       }
     }
-    describe(p, seq, sequence, head, tile, it);
+    describe(p, seq, sequence, head, tile, line, it);
     it->first = step;
-    it->last = static_cast<int>(min(static_cast<long long>(it->steps), step + (end - at)));
-    it->line = at - step;
-    at += it->last - it->first;
+    it->last = it->steps;
+    line += kTileKeys + it->limit;
     step = 0;
     ++tile;
     return true;
@@ -235,21 +207,20 @@ struct Steps {
 
 struct Scratch {
   long long warp_sums[kThreads / 32];
-  int sequence[2];
+  Place cut[2];
   long long rest[2];
-  Stretch stretch;
 };
 
-// Finds the pair's stretch.  All threads sum up the sequences' steps; the thread that passes a cut names the
+// Finds the pair's stretch.  All threads sum up the sequences' costs; the thread that passes a cut names the
 // sequence, and one warp per cut finds head and tile in it.
-__device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh) {
+__device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratch& sh) {
   const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
   const int run = (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
   long long mine = 0;
   for (int s = s0; s < s1; ++s) {
     const Sequence q = read_sequence(p, s);
-    mine += steps_before(p, q, tile_count(p, q)) * p.kv_heads;
+    mine += cost_before(p, q, tile_count(p, q), tile_count(p, q)) * p.kv_heads;
     if (blockIdx.x == 0 && (q.start != p.starts[s] || q.start + q.q != p.starts[s + 1] || (p.kv_lengths && q.kv != p.kv_lengths[s])))
       atomicOr(p.status, STATUS_BAD_ARGUMENT);  // lengths outside the planes are cut to them
   }
@@ -260,7 +231,6 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
     if (lane >= o) sum += x;
   }
   if (lane == 31) sh.warp_sums[warp] = sum;
-  if (t == 0) sh.stretch = {};
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -269,85 +239,74 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
     total += sh.warp_sums[w];
   }
   before += sum - mine;
-  if (total == 0) return;
-  const int pairs = static_cast<int>(min(static_cast<long long>(gridDim.x / 2), (total + p.min_steps - 1) / p.min_steps));
-  const int c = static_cast<int>(blockIdx.x / 2);
-  if (c >= pairs) return;
-  const long long cuts[2] = {cut(total, pairs, c), cut(total, pairs, c + 1)};
+  Stretch r = {};
+  const long long least = static_cast<long long>(p.min_steps) * kKeys;
+  r.share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), least);
+  const long long first = min(static_cast<long long>(blockIdx.x / 2) * r.share, total), last = min(first + r.share, total);
+  if (first == last) return r;  // (all threads alike)
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (before <= cuts[k] && cuts[k] < before + mine) {
-      long long rest = cuts[k] - before;
+    const long long u = k == 0 ? first : last;
+    if (before <= u && u < before + mine) {
+      long long rest = u - before;
       int s = s0;
       for (;; ++s) {
         const Sequence q = read_sequence(p, s);
-        const long long steps = steps_before(p, q, tile_count(p, q)) * p.kv_heads;
-        if (rest < steps) break;
-        rest -= steps;
+        const long long cost = cost_before(p, q, tile_count(p, q), tile_count(p, q)) * p.kv_heads;
+        if (rest < cost) break;
+        rest -= cost;
       }
-      sh.sequence[k] = s;
+      sh.cut[k].sequence = s;
       sh.rest[k] = rest;
     }
   }
   __syncthreads();
   if (warp < 2) {
-    long long u = cuts[0];
+    const long long u = warp == 0 ? first : last;
     Place at = {};
-    if (warp == 1) u = cuts[1];
+    at.line = u;
     if (u < total) {
-      at.sequence = sh.sequence[warp];
+      at.sequence = sh.cut[warp].sequence;
       const Sequence q = read_sequence(p, at.sequence);
       const int tiles = tile_count(p, q);
+      const long long per_head = cost_before(p, q, tiles, tiles);
       long long rest = sh.rest[warp];
-      const long long per_head = steps_before(p, q, tiles);
-      at.head = static_cast<int>(rest / per_head);
+      at.head = static_cast<int>(divide(rest, per_head));
       rest -= at.head * per_head;
-      int low = 0, high = tiles;  // steps_before(low) <= rest < steps_before(high)
+      int low = 0, high = tiles;  // cost_before(low) <= rest < cost_before(high)
       while (high - low > 1) {
         const int width = (high - low + 31) / 32, probe = low + (lane + 1) * width;
-        const bool behind = probe < high && steps_before(p, q, probe) <= rest;
+        const bool behind = probe < high && cost_before(p, q, probe, tiles) <= rest;
         low += __popc(__ballot_sync(0xffffffffu, behind)) * width;
         high = min(high, low + width);
       }
       at.tile = low;
-      rest -= steps_before(p, q, low);
-      at.step = static_cast<int>(rest);
+      rest -= cost_before(p, q, low, tiles);
       at.line = u - rest;
-      const int steps = tile_steps(p, q, at.tile);
-      const int margin = cut_margin(p, min(p.tile_tokens, q.q - at.tile * p.tile_tokens));
+      at.step = static_cast<int>(rest / kKeys);
+      const int steps = tile_steps(p, q, low);
+      const int margin = cut_margin(p, min(p.tile_tokens, q.q - low * p.tile_tokens));
       if (at.step < margin) {
         at.step = 0;
-        u = at.line;
       } else if (steps - at.step < margin) {
         at.step = 0;
+        at.line += tile_cost(p, q, low);
         ++at.tile;
-        u = at.line + steps;
-        at.line = u;
       }
     }
-    if (lane == 0) {
-      if (warp == 0) {
-        sh.stretch.from = at;
-        sh.stretch.first = u;
-        sh.stretch.total = total;
-        sh.stretch.pairs = pairs;
-      } else {
-        sh.stretch.to = at;
-        sh.stretch.last = u;
-      }
-    }
+    __syncwarp();
+    if (lane == 0) sh.cut[warp] = at;
   }
   __syncthreads();
+  r.from = sh.cut[0];
+  r.to = sh.cut[1];
+  return r;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
-}
-
-__device__ __forceinline__ void named_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // One row of S; keys it does not see read as -infinity.
@@ -402,77 +361,124 @@ __device__ __forceinline__ float gated(float v, float gate) {
   return __fdividef(v, 1.0f + exp2_approx(gate * -1.4426950408889634f));
 }
 
-// Joins the parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left, in the order of their keys: a thread has four of a row's values
-// at a time, and of four such places and four parts all loads are under way together.
-template <int D>
-__device__ __forceinline__ void join(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread, int ahead,
-                                     int token, int head) {
-  constexpr int PLACES = 4, PARTS = 4;
-  auto slot_of = [&](int k) { return 2 * static_cast<size_t>(2 * k + rank) + (k == c0 ? 1 : 0); };
+// Joins the parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left, in the order of their keys.
+// Parts are [four values][128 rows][4], so that threads next to each other have rows next to each other.
+__device__ __forceinline__ size_t part_slot(int k, int c0, int rank) {
+  return 2 * static_cast<size_t>(2 * k + rank) + (k == c0 ? 1 : 0);
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The rows' common maximum, and 1 / the sum of their weights, with LANES lanes of the 128 threads to a row.
+template <int LANES>
+__device__ __forceinline__ void join_stats(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread,
+                                           float* row_top, float* row_scale) {
+  const int lane = thread % LANES;
+#pragma unroll 1
+  for (int base = 0; base < rows; base += 128 / LANES) {
+    const int row = base + thread / LANES, from = min(row, rows - 1);
+    float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+    for (int k = c0 + lane; k <= c1; k += 4 * LANES) {
+      float2 stats[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) stats[e] = __ldcg(p.part_stats + part_slot(min(k + e * LANES, c1), c0, rank) * kRows + from);
+      float most = top;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (k + e * LANES > c1) stats[e] = make_float2(-INFINITY, 0.0f);
+        most = fmaxf(most, stats[e].x);
+      }
+      const float shift = most == -INFINITY ? 0.0f : most;
+      total *= exp2_approx(top - shift);
+      top = most;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total = fmaf(stats[e].y, exp2_approx(stats[e].x - shift), total);
+    }
+    if (LANES > 1) {
+      float most = top;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      total *= exp2_approx(top - (most == -INFINITY ? 0.0f : most));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      top = most;
+    }
+    if (lane == 0 && row < rows) {
+      row_top[row] = top == -INFINITY ? 0.0f : top;
+      row_scale[row] = 1.0f / total;
+    }
+  }
+  named_barrier(1, 128);
+}
+
+// The rows: a thread has four of a row's values at PLACES places, and their loads of PARTS parts under way together.
+template <int D, int PLACES, int PARTS>
+__device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread, int ahead,
+                                          int token, int head, const float* row_top, const float* row_scale) {
   const int places = rows * (D / 4);
+#pragma unroll 1
   for (int base = thread; base < places; base += 128 * PLACES) {
-    float top[PLACES], total[PLACES];
     float4 acc[PLACES];
+    int row[PLACES], at[PLACES];
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
-      top[i] = -INFINITY;
-      total[i] = 0.0f;
+      const int place = min(base + 128 * i, places - 1), quad = place / rows;
+      row[i] = place - quad * rows;
+      at[i] = quad * kRows + row[i];
       acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+#pragma unroll 1
     for (int k = c0; k <= c1; k += PARTS) {
+      float2 stats[PLACES][PARTS];
+      float4 o[PLACES][PARTS];
+#pragma unroll
+      for (int e = 0; e < PARTS; ++e) {
+        const size_t slot = part_slot(min(k + e, c1), c0, rank);
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i) {
+          stats[i][e] = __ldcg(p.part_stats + slot * kRows + row[i]);
+          o[i][e] = __ldcg(reinterpret_cast<const float4*>(p.parts) + slot * kRows * (D / 4) + at[i]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < PLACES; ++i) {
-        const int at = min(base + 128 * i, places - 1), row = at / (D / 4), column = at % (D / 4) * 4;
-        float2 stats[PARTS];
-        float4 o[PARTS];
-#pragma unroll
-        for (int e = 0; e < PARTS; ++e) {
-          const size_t line = slot_of(min(k + e, c1)) * kRows + row;
-          stats[e] = __ldcg(&p.part_stats[line]);
-          o[e] = __ldcg(reinterpret_cast<const float4*>(p.parts + line * D + column));
-        }
-        float most = top[i];
+        const float top = row_top[row[i]];
 #pragma unroll
         for (int e = 0; e < PARTS; ++e) {
           // a part without a key of this row has nothing to add, whatever its O holds
-          if (k + e > c1 || (stats[e].x == -INFINITY && stats[e].y == 0.0f)) {
-            stats[e] = make_float2(-INFINITY, 0.0f);
-            o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (k + e <= c1 && !(stats[i][e].x == -INFINITY && stats[i][e].y == 0.0f)) {
+            const float w = exp2_approx(stats[i][e].x - top);
+            acc[i].x = fmaf(o[i][e].x, w, acc[i].x);
+            acc[i].y = fmaf(o[i][e].y, w, acc[i].y);
+            acc[i].z = fmaf(o[i][e].z, w, acc[i].z);
+            acc[i].w = fmaf(o[i][e].w, w, acc[i].w);
           }
-          most = fmaxf(most, stats[e].x);
-        }
-        const float shift = most == -INFINITY ? 0.0f : most;
-        const float before = exp2_approx(top[i] - shift);
-        top[i] = most;
-        total[i] *= before;
-        acc[i] = make_float4(acc[i].x * before, acc[i].y * before, acc[i].z * before, acc[i].w * before);
-#pragma unroll
-        for (int e = 0; e < PARTS; ++e) {
-          const float w = exp2_approx(stats[e].x - shift);
-          total[i] = fmaf(stats[e].y, w, total[i]);
-          acc[i].x = fmaf(o[e].x, w, acc[i].x);
-          acc[i].y = fmaf(o[e].y, w, acc[i].y);
-          acc[i].z = fmaf(o[e].z, w, acc[i].z);
-          acc[i].w = fmaf(o[e].w, w, acc[i].w);
         }
       }
     }
+    uint2 gate[PLACES];
+    if (p.gate) {
+#pragma unroll
+      for (int i = 0; i < PLACES; ++i)
+        gate[i] = __ldg(reinterpret_cast<const uint2*>(gate_row(p, token, head, row[i]) + 4 * (at[i] / kRows)));
+    }
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
-      const int at = base + 128 * i, row = at / (D / 4), column = at % (D / 4) * 4;
-      if (at >= places) break;
-      const float scale = 1.0f / total[i];
-      float v[4] = {acc[i].x * scale, acc[i].y * scale, acc[i].z * scale, acc[i].w * scale};
-      if (p.gate) {
-        const uint2 g = *reinterpret_cast<const uint2*>(gate_row(p, token, head, row) + column);
-        v[0] = gated(v[0], bf16x2_lo(g.x));
-        v[1] = gated(v[1], bf16x2_hi(g.x));
-        v[2] = gated(v[2], bf16x2_lo(g.y));
-        v[3] = gated(v[3], bf16x2_hi(g.y));
+      if (base + 128 * i < places) {
+        const float scale = row_scale[row[i]];
+        float v[4] = {acc[i].x * scale, acc[i].y * scale, acc[i].z * scale, acc[i].w * scale};
+        if (p.gate) {
+          v[0] = gated(v[0], bf16x2_lo(gate[i].x));
+          v[1] = gated(v[1], bf16x2_hi(gate[i].x));
+          v[2] = gated(v[2], bf16x2_lo(gate[i].y));
+          v[3] = gated(v[3], bf16x2_hi(gate[i].y));
+        }
+        if (ahead + row[i] / p.group < 0) v[0] = v[1] = v[2] = v[3] = 0.0f;  // sees no key
+        *reinterpret_cast<uint2*>(output_row<D>(p, token, head, row[i]) + 4 * (at[i] / kRows)) =
+            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
       }
-      if (ahead + row / p.group < 0) v[0] = v[1] = v[2] = v[3] = 0.0f;  // sees no key
-      *reinterpret_cast<uint2*>(output_row<D>(p, token, head, row) + column) =
-          make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     }
   }
 }
@@ -534,12 +540,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   cluster_arrive();  // both CTAs' barriers exist before either touches the other's
-  find_stretch(p, scratch);
+  const Stretch stretch = find_stretch(p, scratch);
   cluster_wait();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_base;
   const uint32_t tmem_o = tmem + 2 * kKeys;
-  const Stretch& stretch = scratch.stretch;
   const int v_box = PAGED ? min(kKeys, 1 << p.page_shift) : kKeys;  // keys of a box of V
 
   if (warp == 0) {
@@ -895,31 +900,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool blind = ahead + r / p.group < 0;  // sees no key
         const float scale = blind ? 0.0f : 1.0f / sum;
         if (ok && quadrant * 32 < rows) {
+          const int row = min(r, rows - 1);
+          uint16_t* out = output_row<D>(p, tile_token, it.head, row);
+          const uint4* gate = p.gate ? reinterpret_cast<const uint4*>(gate_row(p, tile_token, it.head, row)) : nullptr;
+          uint4 g[4];  // asked for a chunk ahead: nothing of the row waits for its gate
+          if (gate) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = __ldg(gate + e);
+          }
 #pragma unroll 1
           for (int k = 0; k < D; k += 32) {
             uint32_t o[32];
             tmem_ld32(tmem_o + lanes + k, o);
             tmem_ld_wait();
-            if (r < rows) {
-              uint16_t* out = output_row<D>(p, tile_token, it.head, r) + k;
-              const uint16_t* gate = p.gate ? gate_row(p, tile_token, it.head, r) + k : nullptr;
+            uint4 now[4];
+            if (gate) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = blind ? 0.0f : __uint_as_float(o[e + i]) * scale;
-                if (gate) {
-                  const uint4 g = *reinterpret_cast<const uint4*>(gate + e);
-                  const uint32_t w[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = gated(v[2 * i], bf16x2_lo(w[i]));
-                    v[2 * i + 1] = gated(v[2 * i + 1], bf16x2_hi(w[i]));
-                  }
-                }
-                *reinterpret_cast<uint4*>(out + e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                                pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+              for (int e = 0; e < 4; ++e) {
+                now[e] = g[e];
+                g[e] = __ldg(gate + (min(k + 32, D - 32) / 8 + e));
               }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = blind ? 0.0f : __uint_as_float(o[8 * e + i]) * scale;
+              if (gate) {
+                const uint32_t w[4] = {now[e].x, now[e].y, now[e].z, now[e].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  v[2 * i] = gated(v[2 * i], bf16x2_lo(w[i]));
+                  v[2 * i + 1] = gated(v[2 * i + 1], bf16x2_hi(w[i]));
+                }
+              }
+              if (r < rows)
+                *reinterpret_cast<uint4*>(out + k + 8 * e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                                        pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
             }
           }
         }
@@ -932,9 +949,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // the pair that the tile begins in, and the last one that it reaches, with the cuts where they moved to
         const int margin = cut_margin(p, it.tokens);
-        const long long inner = it.line + min(margin, it.steps) - 1;
-        const int c0 = pair_of(stretch.total, stretch.pairs, inner);
-        const int c1 = pair_of(stretch.total, stretch.pairs, max(inner, it.line + it.steps - margin));
+        const long long inner = static_cast<long long>(margin) * kKeys, cost = kTileKeys + it.limit;
+        const long long outer = max(inner, static_cast<long long>(it.steps - margin + 1) * kKeys);
+        const int c0 = static_cast<int>(divide(it.line + min(inner, cost) - 1, stretch.share));
+        const int c1 = static_cast<int>(divide(it.line + min(outer, cost) - 1, stretch.share));
         // the part that begins a tile goes to the CTA's slot 1, one that goes on with a tile to slot 0
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (it.first == 0 ? 1 : 0);
         float* part = p.parts + slot * kRows * D;
@@ -945,20 +963,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(tmem_o + lanes + k, o);
             tmem_ld_wait();
             if (r < rows) {
-              float* to = part + static_cast<size_t>(r) * D + k;
+              uint4* to = reinterpret_cast<uint4*>(part) + (k / 4) * kRows + r;
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<uint4*>(to + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int e = 0; e < 32; e += 4) to[e / 4 * kRows] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
           if (r < rows) p.part_stats[slot * kRows + r] = make_float2(m, sum);
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_remote_light(o_free_even);
-          mbar_arrive(&stats_free);
-        }
+        if (lane == 0) mbar_arrive_remote_light(o_free_even);
         __threadfence();
         named_barrier(1, 128);
         unsigned int* ticket = p.tickets + 2 * c0 + rank;
@@ -966,9 +980,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_barrier(1, 128);
         if (last_part) {
           __threadfence();
-          join<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head);
+          // row_max and row_sum have been read by their rows' threads: here they hold what the parts have in common
+          if (c1 - c0 < 8) {
+            join_stats<1>(p, c0, c1, rank, rows, thread, row_max, row_sum);
+          } else {
+            join_stats<8>(p, c0, c1, rank, rows, thread, row_max, row_sum);
+          }
+          if (c1 - c0 < 2) {
+            join_rows<D, 6, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, row_max, row_sum);
+          } else {
+            join_rows<D, 3, 4>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, row_max, row_sum);
+          }
           if (thread == 0) *ticket = 0u;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&stats_free);
         named_barrier(1, 128);  // `last_part` is written again
       }
       ++item;
@@ -977,8 +1003,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before_sync();
   __syncthreads();
-  cluster_arrive();  // nothing of the other CTA's works on this one's memory any more
-  cluster_wait();
+  cluster_arrive_relaxed();  // nothing of the other CTA's works on this one's memory any more
+  cluster_wait_relaxed();
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 

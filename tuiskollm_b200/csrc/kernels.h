@@ -445,7 +445,7 @@ struct AttentionParams {
   const uint16_t* gate;
   int query_token_stride, query_head_stride;
   uint16_t* output;
-  float* parts;        // [2 per CTA][128 rows][head_dim]
+  float* parts;        // [2 per CTA][head_dim / 4][128 rows][4]
   float2* part_stats;  // [2 per CTA][128 rows]
   unsigned int* tickets;
   uint32_t* status;

@@ -537,7 +537,7 @@ TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_
  * its block table row (request_rows[s], or s when that is NULL), the new tokens' own included; with q new
  * tokens over k keys token i sees keys 0 .. k - q + i.  A token that sees none gets zeros.
  *   output[token][head] = softmax(scale * q . K) V, times sigmoid(gate[token][head]) when gate is given
- * (the queries' strides).  output is [tokens, q_heads, head_dim]; rows outside the sequences are left as
+ * (the queries' strides).  output is [tokens, q_heads, head_dim] and starts on 32 bytes; rows outside the sequences are left as
  * they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
  * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used. */
 TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,

@@ -348,6 +348,13 @@ __device__ __forceinline__ void zero_behind(uint8_t* unit, int keys, int v_box, 
   __syncwarp();
 }
 
+// 32 bytes of an output row: each thread has a row of its own, so a narrower store would touch every sector twice.
+__device__ __forceinline__ void store_words8(uint16_t* to, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // Rows of a tile whose first token row is `token`.
 __device__ __forceinline__ const uint16_t* gate_row(const AttentionParams& p, int token, int head, int row) {
   return p.gate + static_cast<size_t>(token + row / p.group) * p.query_token_stride +
@@ -357,8 +364,14 @@ template <int D>
 __device__ __forceinline__ uint16_t* output_row(const AttentionParams& p, int token, int head, int row) {
   return p.output + (static_cast<size_t>(token + row / p.group) * p.q_heads + head * p.group + row % p.group) * D;
 }
-__device__ __forceinline__ float gated(float v, float gate) {
-  return __fdividef(v, 1.0f + exp2_approx(gate * -1.4426950408889634f));
+// Two values times the sigmoid of their packed gates.
+__device__ __forceinline__ F32x2 gated(F32x2 v, uint32_t gate) {
+  const float2 e = f32x2_parts(mul2(bf16x2_to_f32x2(gate), f32x2_splat(-1.4426950408889634f)));
+  const float2 d = f32x2_parts(add2(f32x2(exp2_approx(e.x), exp2_approx(e.y)), f32x2_splat(1.0f)));
+  float a, b;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(d.y));
+  return mul2(v, f32x2(a, b));
 }
 
 // Joins the parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left, in the order of their keys.
@@ -429,6 +442,12 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
       at[i] = quad * kRows + row[i];
       acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+    uint2 gate[PLACES];
+    if (p.gate) {
+#pragma unroll
+      for (int i = 0; i < PLACES; ++i)
+        gate[i] = __ldg(reinterpret_cast<const uint2*>(gate_row(p, token, head, row[i]) + 4 * (at[i] / kRows)));
+    }
 #pragma unroll 1
     for (int k = c0; k <= c1; k += PARTS) {
       float2 stats[PLACES][PARTS];
@@ -458,26 +477,18 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
         }
       }
     }
-    uint2 gate[PLACES];
-    if (p.gate) {
-#pragma unroll
-      for (int i = 0; i < PLACES; ++i)
-        gate[i] = __ldg(reinterpret_cast<const uint2*>(gate_row(p, token, head, row[i]) + 4 * (at[i] / kRows)));
-    }
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
       if (base + 128 * i < places) {
         const float scale = row_scale[row[i]];
-        float v[4] = {acc[i].x * scale, acc[i].y * scale, acc[i].z * scale, acc[i].w * scale};
+        F32x2 v[2] = {mul2(f32x2(acc[i].x, acc[i].y), f32x2_splat(scale)), mul2(f32x2(acc[i].z, acc[i].w), f32x2_splat(scale))};
         if (p.gate) {
-          v[0] = gated(v[0], bf16x2_lo(gate[i].x));
-          v[1] = gated(v[1], bf16x2_hi(gate[i].x));
-          v[2] = gated(v[2], bf16x2_lo(gate[i].y));
-          v[3] = gated(v[3], bf16x2_hi(gate[i].y));
+          v[0] = gated(v[0], gate[i].x);
+          v[1] = gated(v[1], gate[i].y);
         }
-        if (ahead + row[i] / p.group < 0) v[0] = v[1] = v[2] = v[3] = 0.0f;  // sees no key
-        *reinterpret_cast<uint2*>(output_row<D>(p, token, head, row[i]) + 4 * (at[i] / kRows)) =
-            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        uint2 w = make_uint2(f32x2_to_bf16x2(v[0]), f32x2_to_bf16x2(v[1]));
+        if (ahead + row[i] / p.group < 0) w = make_uint2(0u, 0u);  // sees no key
+        *reinterpret_cast<uint2*>(output_row<D>(p, token, head, row[i]) + 4 * (at[i] / kRows)) = w;
       }
     }
   }
@@ -889,54 +900,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     Item it;
     bool ok = true;  // a warp whose wait ran out still takes part in the barriers of the four
     while (walk.next(p, &it)) {
-      ok = ok && warp_wait(&stats_full, item & 1, p.status) && warp_wait(&o_full, item & 1, p.status);
-      tc_fence_after_sync();
-      const float m = row_max[r], sum = row_sum[r];
       const int rows = min(it.tokens - rank * p.half_tokens, p.half_tokens) * p.group;  // of this CTA, below 1: none
       const int tile_token = it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens;  // first token row
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
       const bool whole = it.first == 0 && it.last == it.steps;
+      // Half of the row's gate is there before the row is, the rest is asked for as it is used up: nothing of the next
+      // tile's O can be added before this one's has been read.
+      constexpr int WINDOW = 4;  // of 32 values
+      uint4 gates[WINDOW][4];
+      const uint4* gate = nullptr;
+      if (p.gate && whole && quadrant * 32 < rows) {
+        gate = reinterpret_cast<const uint4*>(gate_row(p, tile_token, it.head, min(r, rows - 1)));
+#pragma unroll
+        for (int k = 0; k < WINDOW; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) gates[k][e] = __ldg(gate + 4 * k + e);
+        }
+      }
+      ok = ok && warp_wait(&stats_full, item & 1, p.status) && warp_wait(&o_full, item & 1, p.status);
+      tc_fence_after_sync();
+      const float m = row_max[r], sum = row_sum[r];
       if (whole) {
         const bool blind = ahead + r / p.group < 0;  // sees no key
         const float scale = blind ? 0.0f : 1.0f / sum;
         if (ok && quadrant * 32 < rows) {
-          const int row = min(r, rows - 1);
-          uint16_t* out = output_row<D>(p, tile_token, it.head, row);
-          const uint4* gate = p.gate ? reinterpret_cast<const uint4*>(gate_row(p, tile_token, it.head, row)) : nullptr;
-          uint4 g[4];  // asked for a chunk ahead: nothing of the row waits for its gate
-          if (gate) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) g[e] = __ldg(gate + e);
-          }
+          uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
+          const F32x2 scale2 = f32x2_splat(scale);
 #pragma unroll 1
-          for (int k = 0; k < D; k += 32) {
-            uint32_t o[32];
-            tmem_ld32(tmem_o + lanes + k, o);
-            tmem_ld_wait();
-            uint4 now[4];
-            if (gate) {
+          for (int base = 0; base < D / 32; base += WINDOW) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                now[e] = g[e];
-                g[e] = __ldg(gate + (min(k + 32, D - 32) / 8 + e));
-              }
-            }
+            for (int k = 0; k < WINDOW; ++k) {
+              uint32_t o[32];
+              tmem_ld32(tmem_o + lanes + 32 * (base + k), o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v[8];
+              for (int h = 0; h < 2; ++h) {
+                uint32_t w[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = blind ? 0.0f : __uint_as_float(o[8 * e + i]) * scale;
-              if (gate) {
-                const uint32_t w[4] = {now[e].x, now[e].y, now[e].z, now[e].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  v[2 * i] = gated(v[2 * i], bf16x2_lo(w[i]));
-                  v[2 * i + 1] = gated(v[2 * i + 1], bf16x2_hi(w[i]));
+                for (int i = 0; i < 8; ++i) {
+                  F32x2 v = mul2(f32x2(__uint_as_float(o[16 * h + 2 * i]), __uint_as_float(o[16 * h + 2 * i + 1])), scale2);
+                  if (gate) {
+                    const uint4 g = gates[k][2 * h + i / 4];
+                    v = gated(v, i % 4 == 0 ? g.x : i % 4 == 1 ? g.y : i % 4 == 2 ? g.z : g.w);
+                  }
+                  w[i] = blind ? 0u : f32x2_to_bf16x2(v);
+                }
+                if (r < rows) store_words8(out + 32 * (base + k) + 16 * h, w);
+                if (gate) {  // (the last window's is asked for again)
+                  const uint4* next = gate + 4 * (min(base + WINDOW, D / 32 - WINDOW) + k) + 2 * h;
+                  gates[k][2 * h] = __ldg(next);
+                  gates[k][2 * h + 1] = __ldg(next + 1);
                 }
               }
-              if (r < rows)
-                *reinterpret_cast<uint4*>(out + k + 8 * e) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                                        pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
             }
           }
         }

@@ -231,7 +231,7 @@ Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, 
   TK100_TRY(plane(ctx_, what, "query", query, 16));
   TK100_TRY(plane(ctx_, what, "key", key, 16));
   TK100_TRY(plane(ctx_, what, "value", value, 16));
-  TK100_TRY(plane(ctx_, what, "output", p->output, 16));
+  TK100_TRY(plane(ctx_, what, "output", p->output, 32));
   TK100_TRY(plane(ctx_, what, "workspace", workspace, 16));
   if (p->gate) TK100_TRY(plane(ctx_, what, "gate", p->gate, 16));
   TK100_TRY(stride(ctx_, what, "query token", p->query_token_stride, head_dim));

@@ -24,9 +24,9 @@ def queries(tokens, heads, dim, seed, gated=False):
     return wide[..., :dim], wide[..., dim:] if gated else None
 
 
-def check(output, expected, size):
+def check(output, expected, size, gated=False):
     error = (ref.f64(output) - expected).abs()
-    bad = ~(error <= ref.attention_tolerance(expected, size))
+    bad = ~(error <= ref.attention_tolerance(expected, size, gated))
     assert not bool(bad.any()), (int(bad.sum()), bad.numel(), float(error[bad].max()), bad.nonzero()[:4].tolist())
 
 
@@ -43,7 +43,7 @@ def run_paged(ctx, new, cached, heads=(24, 4, 256), page=64, gated=False, order=
     assert ctx.device_status() == 0
     expected, size = ref.attention(query[:total], cache.keys, cache.values, starts, op.scale,
                                    None if gate is None else gate[:total])
-    check(output[:total], expected, size)
+    check(output[:total], expected, size, gated)
     assert bool((output[total:].view(torch.uint8) == SENTINEL).all()), "rows behind the last sequence were written"
     assert int(work[:4096].view(torch.int32).abs().sum()) == 0, "tickets were left behind"
     return output[:total]
@@ -135,7 +135,7 @@ def run_prompt(ctx, lengths, heads=(24, 4, 256), gated=False, plane=False, seed=
     split = [(starts[i], starts[i + 1]) for i in range(len(lengths))]
     expected, size = ref.attention(query[:total], [key[a:b] for a, b in split], [value[a:b] for a, b in split], starts,
                                    op.scale, None if gate is None else gate[:total])
-    check(output[:total], expected, size)
+    check(output[:total], expected, size, gated)
     assert bool((output[total:].view(torch.uint8) == SENTINEL).all())
 
 

@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kRows = 128;   // rows of a tile in each CTA of the pair
 constexpr int kKeys = 128;   // keys of a step
-constexpr int kThreads = 320;
+constexpr int kThreads = 512;
 
 template <int D>
 struct Shape {
@@ -45,7 +45,6 @@ struct Shape {
   static constexpr int V_CHUNKS = CHUNKS / 2;  // a V unit: all keys, half of the chunks
   static constexpr int UNIT = K_KEYS * 2 * D;  // bytes of a ring stage
   static constexpr int STAGES = D == 256 ? 5 : 12;
-  static constexpr int SHARED = kRows * 2 * D + STAGES * UNIT + 1024;
 };
 
 // ----------------------------------------------------------------- the line of keys
@@ -309,28 +308,68 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 
-// One row of S; keys it does not see read as -infinity.
-__device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int seen, uint32_t (&s)[kKeys]) {
-#pragma unroll
-  for (int k = 0; k < kKeys; k += 32) tmem_ld32(taddr + k, s + k);
+// Half a row of S; keys it does not see read as -infinity.
+__device__ __forceinline__ void load_scores(uint32_t taddr, bool masked, int seen, uint32_t (&s)[kKeys / 2]) {
+  tmem_ld32(taddr, s);
+  tmem_ld32(taddr + 32, s + 32);
   tmem_ld_wait();
   if (masked) {
 #pragma unroll
-    for (int k = 0; k < kKeys; ++k) s[k] = k < seen ? s[k] : 0xff800000u;
+    for (int k = 0; k < kKeys / 2; ++k) s[k] = k < seen ? s[k] : 0xff800000u;
   }
 }
-
-// A bounded wait of a whole warp, with one verdict.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+__device__ __forceinline__ float top_of(const uint32_t (&s)[kKeys / 2]) {
+  float tops[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
+#pragma unroll
+  for (int k = 8; k < kKeys / 2; k += 8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 4])));
+  }
+  return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
-// The same on a barrier that the other CTA's threads arrive on.  The bounded wait reads the clock on its way in, which
-// takes about 2000 cycles: not before the barrier has been looked at for a while.
-__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
+// The scores' weights, packed into the first half of the array; returns their sum.
+__device__ __forceinline__ float weights_of(uint32_t (&s)[kKeys / 2], float c, float shift) {
+  const F32x2 scale2 = f32x2_splat(c), shift2 = f32x2_splat(-shift);
+  F32x2 sums[2] = {f32x2_splat(0.0f), f32x2_splat(0.0f)};
+#pragma unroll
+  for (int k = 0; k < kKeys / 2; k += 2) {
+    const float2 e = f32x2_parts(fma2(f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale2, shift2));
+    const float a = exp2_approx(e.x), b = exp2_approx(e.y);
+    sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], f32x2(a, b));
+    s[k / 2] = pack_bf16x2(a, b);
+  }
+  const float2 sum = f32x2_parts(add2(sums[0], sums[1]));
+  return sum.x + sum.y;
+}
+
+// A bounded wait of a whole warp, with one verdict: mbar_wait written out, because a call, even one that is never
+// made, would hold all warps to one register count.  CLUSTER: threads of the other CTA arrive on the barrier.
+template <bool CLUSTER>
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
   bool done = false;
+  uint64_t start = 0;  // (reading the clock takes some 2000 cycles: not before the barrier has been looked at for a while)
 #pragma unroll 1
-  for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait_cluster(bar, parity);
-  return __all_sync(0xffffffffu, done || mbar_wait_cluster(bar, parity, status));
+  for (uint32_t i = 1; !done; ++i) {
+    done = CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+    if (!done && (i & 1023u) == 0) {
+      if (*reinterpret_cast<volatile uint32_t*>(status) & STATUS_WAIT_TIMEOUT) break;
+      const uint64_t now = global_timer_ns();
+      if (start == 0) start = now;
+      if (now - start > 2000000000ull) {
+        atomicOr(status, STATUS_WAIT_TIMEOUT);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, done);
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return bounded_wait<false>(bar, parity, status);
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return bounded_wait<true>(bar, parity, status);
 }
 
 // Keys of a step that count, of which the last 16 that are multiplied are not full: those behind them are zeroed.
@@ -348,8 +387,12 @@ __device__ __forceinline__ void zero_behind(uint8_t* unit, int keys, int v_box, 
   __syncwarp();
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // 32 bytes of an output row: each thread has a row of its own, so a narrower store would touch every sector twice.
-__device__ __forceinline__ void store_words8(uint16_t* to, const uint32_t (&w)[8]) {
+__device__ __forceinline__ void store_words8(uint16_t* to, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
                "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
@@ -496,6 +539,41 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
 
 // ------------------------------------------------------------------------- the kernel
 
+// Barriers that both CTAs' loads or threads arrive on are the even CTA's (full, q_full, p_full, o_free); those that
+// the even CTA's MMA warp commits to are arrived on in both (empty, q_empty, s_full, pv_done, o_full).
+template <int D>
+struct Control {
+  uint64_t full[Shape<D>::STAGES], empty[Shape<D>::STAGES], tail_full[Shape<D>::STAGES];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done, o_full, o_free, stats_full, stats_free, drained;
+  uint64_t reference_set[2][4];
+  uint32_t tmem_base;
+  int last_part;
+  float reference[kRows];  // the row's reference maximum, of the step before
+  float row_sum[2][kRows];  // what either softmax warpgroup has of a row at a tile's end
+  union {
+    float row_max[2][kRows];
+    Scratch scratch;  // in front of the roles
+  };
+};
+template <int D>
+constexpr int shared_bytes() {
+  return kRows * 2 * D + Shape<D>::STAGES * Shape<D>::UNIT + static_cast<int>(sizeof(Control<D>));
+}
+
+static_assert(shared_bytes<256>() <= 232448 && shared_bytes<128>() <= 232448, "more shared memory than a CTA may have");
+
+// Registers of the calling warpgroup from here on; the four shares make up the 4 x 128 that the block starts with.
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+constexpr int kControlRegisters = 64, kSoftmaxRegisters = 128 /* as at the start */, kEpilogueRegisters = 192;
+static_assert(kControlRegisters + 2 * kSoftmaxRegisters + kEpilogueRegisters <= 4 * 128, "the shares exceed the block's registers");
+
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q1,
@@ -503,47 +581,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ AttentionParams p) {
   using S = Shape<D>;
   constexpr int STAGES = S::STAGES;
-  extern __shared__ uint8_t dynamic[];
-  uint8_t* smem_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* ring = smem_q + kRows * 2 * D;
-
-  // Barriers that both CTAs' loads or threads arrive on are the even CTA's (full, q_full, p_full, o_free); those that
-  // the even CTA's MMA warp commits to are arrived on in both (empty, q_empty, s_full, pv_done, o_full).
-  __shared__ uint64_t full[STAGES], empty[STAGES], tail_full[STAGES];
-  __shared__ uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done, o_full, o_free, stats_full, stats_free, drained;
-  __shared__ uint32_t tmem_base;
-  __shared__ float row_max[kRows], row_sum[kRows];
-  __shared__ int last_part;
-  __shared__ Scratch scratch;
+  extern __shared__ __align__(1024) uint8_t dynamic[];
+  uint8_t* const smem_q = dynamic;
+  uint8_t* const ring = smem_q + kRows * 2 * D;
+  Control<D>& ctl = *reinterpret_cast<Control<D>*>(ring + STAGES * S::UNIT);
 
   const int warp = warp_index(), lane = static_cast<int>(threadIdx.x) & 31;
   const int rank = static_cast<int>(cluster_cta_rank());
 
   if (warp == 0 && elect_one()) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 2);
-      mbar_init(&empty[i], 1);
-      mbar_init(&tail_full[i], 1);
+      mbar_init(&ctl.full[i], 2);
+      mbar_init(&ctl.empty[i], 1);
+      mbar_init(&ctl.tail_full[i], 1);
     }
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
+    mbar_init(&ctl.q_full, 1);
+    mbar_init(&ctl.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.p_full[i], 8);
     }
-    mbar_init(&pv_done, 1);
-    mbar_init(&o_full, 1);
-    mbar_init(&o_free, 8);
-    mbar_init(&stats_full, 4);
-    mbar_init(&stats_free, 4);
-    mbar_init(&drained, 1);
+    mbar_init(&ctl.pv_done, 1);
+    mbar_init(&ctl.o_full, 1);
+    mbar_init(&ctl.o_free, 8);
+    mbar_init(&ctl.stats_full, 8);
+    mbar_init(&ctl.stats_free, 4);
+    mbar_init(&ctl.drained, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&ctl.reference_set[i / 4][i % 4], 1);
     fence_mbar_init();
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
   if (warp == 1) {
-    tmem_alloc_pair(&tmem_base, 512);
+    tmem_alloc_pair(&ctl.tmem_base, 512);
     tmem_relinquish_pair();
   }
   pdl_wait();
@@ -551,13 +622,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   cluster_arrive();  // both CTAs' barriers exist before either touches the other's
-  const Stretch stretch = find_stretch(p, scratch);
+  const Stretch stretch = find_stretch(p, ctl.scratch);
   cluster_wait();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = ctl.tmem_base;
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int v_box = PAGED ? min(kKeys, 1 << p.page_shift) : kKeys;  // keys of a box of V
 
+  if (warp < 4) {
+    fewer_registers<kControlRegisters>();
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
     int stage = 0;
@@ -570,8 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 1;
       }
     };
-    const uint32_t full_even = mapa_u32(smem_u32(&full[0]), 0), q_full_even = mapa_u32(smem_u32(&q_full), 0);
-    const uint32_t tail_mine = mapa_u32(smem_u32(&tail_full[0]), static_cast<uint32_t>(rank));
+    const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0), q_full_even = mapa_u32(smem_u32(&ctl.q_full), 0);
+    const uint32_t tail_mine = mapa_u32(smem_u32(&ctl.tail_full[0]), static_cast<uint32_t>(rank));
     // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (all chunks where no page ends inside the
     // 64 keys), V boxes of `v_box` keys and half of the chunks.  What does not change from step to step:
     const int shift = p.page_shift;
@@ -629,13 +702,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (more) {
         if (now.opens()) {
           const Item& it = now.it;
-          if (now.item > 0) ok = warp_wait(&q_empty, (now.item - 1) & 1, p.status);
+          if (now.item > 0) ok = warp_wait(&ctl.q_empty, (now.item - 1) & 1, p.status);
           if (!ok) break;
           const int mine = min(it.tokens - rank * p.half_tokens, p.half_tokens);  // tokens of this CTA's rows
           if (rank == 0 && lane == 0) {
             const int other = min(max(it.tokens - p.half_tokens, 0), p.half_tokens);
             const int tokens = (mine == 1 ? 1 : p.half_tokens) + (other <= 1 ? other : p.half_tokens);
-            mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.group * tokens * 128 * S::CHUNKS));
+            mbar_arrive_expect_tx(&ctl.q_full, static_cast<uint32_t>(p.group * tokens * 128 * S::CHUNKS));
           }
           if (lane < S::CHUNKS && mine > 0) {
             tma_load_4d_pair(smem_q + lane * kRows * 128, mine == 1 ? &map_q1 : &map_q, q_full_even, 64 * lane, 0, it.head,
@@ -644,11 +717,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           ++items;
         }
-        ok = warp_wait(&empty[stage], phase, p.status);
+        ok = warp_wait(&ctl.empty[stage], phase, p.status);
         if (!ok) break;
         if (lane == 0) {
           if (rank == 0) {
-            mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>((k_fetched(fetch.keys, 0) + k_fetched(fetch.keys, 1)) * 2 * D));
+            mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>((k_fetched(fetch.keys, 0) + k_fetched(fetch.keys, 1)) * 2 * D));
           } else {
             mbar_arrive_remote_light(full_even + stage * 8);
           }
@@ -660,15 +733,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance();
       }
       if (loaded) {
-        ok = warp_wait(&empty[stage], phase, p.status);
+        ok = warp_wait(&ctl.empty[stage], phase, p.status);
         if (!ok) break;
         const int fetched = (max(earlier.keys, 0) + v_box - 1) & ~(v_box - 1);
         const bool tail = ragged(earlier.keys);  // goes to this CTA's own barrier, `full` is arrived on behind the zeros
         if (lane == 0) {
           if (tail) {
-            mbar_arrive_expect_tx(&tail_full[stage], static_cast<uint32_t>(fetched * D));
+            mbar_arrive_expect_tx(&ctl.tail_full[stage], static_cast<uint32_t>(fetched * D));
           } else if (rank == 0) {
-            mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(fetched * 2 * D));
+            mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>(fetched * 2 * D));
           } else {
             mbar_arrive_remote_light(full_even + stage * 8);
           }
@@ -691,10 +764,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) {
       // what was asked for lands before a CTA's shared memory is somebody else's; both leave together
-      for (int n = 0; rank == 0 && items > 0 && n < 200000 && !mbar_try_wait(&q_full, (items - 1) & 1); ++n) {
+      for (int n = 0; rank == 0 && items > 0 && n < 200000 && !mbar_try_wait(&ctl.q_full, (items - 1) & 1); ++n) {
       }
       for (int i = 0; i < STAGES; ++i) {
-        for (int n = 0; rank == 0 && n < 200000 && !mbar_try_wait(&full[stage], phase); ++n) {
+        for (int n = 0; rank == 0 && n < 200000 && !mbar_try_wait(&ctl.full[stage], phase); ++n) {
         }
         advance();
       }
@@ -717,8 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     Steps next(p, stretch);
     // S[buffer] = Q K^T of step `next`
     auto scores = [&](int buffer) {
-      if (next.opens()) ok = warp_wait(&q_full, next.item & 1, p.status);
-      ok = ok && warp_wait_cluster(&full[stage], phase, p.status);
+      if (next.opens()) ok = warp_wait(&ctl.q_full, next.item & 1, p.status);
+      ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status);
       if (!ok) return;
       if (elect_one()) {
         const uint64_t a = umma_desc_sw128(q_addr), b = umma_desc_sw128(ring_addr + stage * S::UNIT);
@@ -727,9 +800,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_bf16_pair(tmem + buffer * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3),
                          b + (k >> 2) * (S::K_KEYS * 128 >> 4) + 2 * (k & 3), idesc_s, k > 0);
         }
-        umma_commit_pair(&empty[stage]);
-        umma_commit_pair(&s_full[buffer]);
-        if (next.closes()) umma_commit_pair(&q_empty);
+        umma_commit_pair(&ctl.empty[stage]);
+        umma_commit_pair(&ctl.s_full[buffer]);
+        if (next.closes()) umma_commit_pair(&ctl.q_empty);
       }
       __syncwarp();
       advance();
@@ -744,14 +817,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (ragged(keys)) {
         // P is zero for the keys behind the last, but what lies there may be no number
-        ok = warp_wait(&tail_full[stage], (tail_phase >> stage) & 1, p.status);
+        ok = warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status);
         if (!ok) break;
         tail_phase ^= 1u << stage;
         zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
-        if (lane == 0) mbar_arrive(&full[stage]);
+        if (lane == 0) mbar_arrive(&ctl.full[stage]);
       }
-      if (opens && item > 0) ok = warp_wait_cluster(&o_free, (item - 1) & 1, p.status);
-      ok = ok && warp_wait_cluster(&full[stage], phase, p.status) && warp_wait_cluster(&p_full[buffer], (n >> 1) & 1, p.status);
+      if (opens && item > 0) ok = warp_wait_cluster(&ctl.o_free, (item - 1) & 1, p.status);
+      ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status) && warp_wait_cluster(&ctl.p_full[buffer], (n >> 1) & 1, p.status);
       if (!ok) break;
       tc_fence_after_sync();
       if (elect_one()) {
@@ -762,23 +835,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t offset = (r & ~(v_box - 1u)) * S::V_CHUNKS * 128 + (r & (v_box - 1u)) * 128;
           umma_bf16_ta_pair(tmem_o, tmem + buffer * kKeys + 8 * k, b + (offset >> 4), idesc_o, !opens || k > 0);
         }
-        umma_commit_pair(&empty[stage]);
-        umma_commit_pair(&pv_done);
-        if (closes) umma_commit_pair(&o_full);
+        umma_commit_pair(&ctl.empty[stage]);
+        umma_commit_pair(&ctl.pv_done);
+        if (closes) umma_commit_pair(&ctl.o_full);
       }
       __syncwarp();
       advance();
       ++n;
     }
     if (!ok) {
-      if (elect_one()) umma_commit_pair(&drained);
+      if (elect_one()) umma_commit_pair(&ctl.drained);
       __syncwarp();
-      for (int i = 0; i < 200000 && !mbar_try_wait(&drained, 0); ++i) {
+      for (int i = 0; i < 200000 && !mbar_try_wait(&ctl.drained, 0); ++i) {
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------- zeros behind the odd CTA's last keys
-    const uint32_t full_even = mapa_u32(smem_u32(&full[0]), 0);
+    const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0);
     uint32_t tail_phase = 0;
     int stage = 0;
     auto advance = [&]() { stage = stage + 1 == STAGES ? 0 : stage + 1; };
@@ -790,20 +863,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       more = next.next(p);
       if (more) advance();
       if (ragged(keys)) {
-        if (!warp_wait(&tail_full[stage], (tail_phase >> stage) & 1, p.status)) break;
+        if (!warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status)) break;
         tail_phase ^= 1u << stage;
         zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
         if (lane == 0) mbar_arrive_remote(full_even + stage * 8);
       }
       advance();
     }
-  } else if (warp < 6) {
+  }
+  } else if (warp < 12) {
     // ----------------------------------------------------------------- softmax
-    const int quadrant = warp & 3;  // the TMEM lanes this warp may touch
+    const int group = (warp >> 2) - 1;  // has the steps of its parity, and S buffer `group`
+    const int quadrant = warp & 3;      // the TMEM lanes this warp may touch
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+    const uint32_t at = tmem + group * kKeys + lanes;
     const float c = p.scale_log2;
-    const uint32_t p_full_even = mapa_u32(smem_u32(&p_full[0]), 0);
+    const uint32_t p_full_even = mapa_u32(smem_u32(&ctl.p_full[group]), 0);
     int n = 0, item = 0;
     bool ok = true;
     Walk walk(p, stretch);
@@ -813,88 +889,81 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool active = quadrant * 32 < rows;
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
       const int limit = ahead + r / p.group + 1;  // keys this row sees
-      float reference = -INFINITY, sum = 0.0f;
-      for (int j = it.first; j < it.last; ++j, ++n) {
-        const int buffer = n & 1;
-        ok = warp_wait(&s_full[buffer], (n >> 1) & 1, p.status);
+      const int first = it.first, last = it.last;
+      float mine = -INFINITY, sum = 0.0f;  // the reference that `sum` is relative to
+      for (int j = first; j < last; ++j, ++n) {
+        if ((n & 1) != group) continue;
+        ok = warp_wait(&ctl.s_full[group], (n >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after_sync();
+        // the second half of the keys first: the first half stays in registers, and what P overwrites of S is of it
+        uint32_t s[kKeys / 2];
+        const int seen = limit - j * kKeys;
+        const bool masked = active && __any_sync(0xffffffffu, seen < kKeys);
+        float top = -INFINITY;
         if (active) {
-          uint32_t s[kKeys];
-          const uint32_t at = tmem + buffer * kKeys + lanes;
-          const int seen = limit - j * kKeys;
-          const bool masked = __any_sync(0xffffffffu, seen < kKeys);
+          load_scores(at + kKeys / 2, masked, seen - kKeys / 2, s);
+          top = top_of(s);
           load_scores(at, masked, seen, s);
-          float tops[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) tops[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
-#pragma unroll
-          for (int k = 8; k < kKeys; k += 8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              tops[e] = fmaxf(tops[e], fmaxf(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 4])));
-          }
-          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-          if (j == it.first) {
-            reference = top;
-          } else {
-            const bool grown = (top - reference) * c > 8.0f;
-            if (__any_sync(0xffffffffu, grown)) {
-              // O of the steps before this one is complete, and none is added until P of this one is
-              ok = warp_wait(&pv_done, (n - 1) & 1, p.status);
-              if (!ok) break;
-              tc_fence_after_sync();
-              const float alpha = grown ? exp2_approx((reference - top) * c) : 1.0f;
-              if (grown) reference = top;
-              sum *= alpha;
+          top = fmaxf(top, top_of(s));
+        }
+        if (n > 0) ok = warp_wait(&ctl.reference_set[group ^ 1][quadrant], ((n - 1) >> 1) & 1, p.status);
+        if (!ok) break;
+        const float before = j == first ? top : ctl.reference[r];
+        const bool grown = (top - before) * c > 8.0f;
+        const float now = grown ? top : before;
+        ctl.reference[r] = now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.reference_set[group][quadrant]);
+        if (active) {
+          if (__any_sync(0xffffffffu, grown)) {
+            // O of the steps before this one is complete, and none is added until P of this one is
+            ok = warp_wait(&ctl.pv_done, (n - 1) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const float alpha = grown ? exp2_approx((before - now) * c) : 1.0f;
 #pragma unroll 1
-              for (int k = 0; k < D; k += 32) {
-                uint32_t o[32];
-                tmem_ld32(tmem_o + lanes + k, o);
-                tmem_ld_wait();
+            for (int k = 0; k < D; k += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem_o + lanes + k, o);
+              tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st32(tmem_o + lanes + k, o);
-              }
-              tmem_st_wait();
-              load_scores(at, masked, seen, s);  // rather than 128 registers kept over the wait
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(tmem_o + lanes + k, o);
             }
+            tmem_st_wait();
+            load_scores(at, masked, seen, s);  // rather than 64 registers kept over the wait
           }
-          const float shift = reference == -INFINITY ? 0.0f : reference * c;
-          const F32x2 scale2 = f32x2_splat(c), shift2 = f32x2_splat(-shift);
-          F32x2 sums[2] = {f32x2_splat(0.0f), f32x2_splat(0.0f)};
-#pragma unroll
-          for (int k = 0; k < kKeys; k += 2) {
-            const float2 e = f32x2_parts(fma2(f32x2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale2, shift2));
-            const float a = exp2_approx(e.x), b = exp2_approx(e.y);
-            sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], f32x2(a, b));
-            s[k / 2] = pack_bf16x2(a, b);
-          }
-          const float2 part = f32x2_parts(add2(sums[0], sums[1]));
-          sum += part.x + part.y;
+          if (mine != now) sum *= exp2_approx((mine - now) * c);
+          mine = now;
+          const float shift = now == -INFINITY ? 0.0f : now * c;
+          sum += weights_of(s, c, shift);
           tmem_st32(at, s);
-          tmem_st32(at + 32, s + 32);
+          load_scores(at + kKeys / 2, masked, seen - kKeys / 2, s);
+          sum += weights_of(s, c, shift);
+          tmem_st32(at + kKeys / 4, s);
           tmem_st_wait();
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote_light(p_full_even + buffer * 8);
+        if (lane == 0) mbar_arrive_remote_light(p_full_even);
       }
       if (!ok) break;
-      if (item > 0) ok = warp_wait(&stats_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
+      if (item > 0) ok = warp_wait(&ctl.stats_free, (item - 1) & 1, p.status);  // the epilogue has read the last tile's
       if (!ok) break;
-      row_max[r] = reference == -INFINITY ? -INFINITY : reference * c;
-      row_sum[r] = sum;
+      ctl.row_max[group][r] = mine == -INFINITY ? -INFINITY : mine * c;
+      ctl.row_sum[group][r] = sum;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&stats_full);
+      if (lane == 0) mbar_arrive(&ctl.stats_full);
       ++item;
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 192;
+    more_registers<kEpilogueRegisters>();
+    const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 384;
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
-    const uint32_t o_free_even = mapa_u32(smem_u32(&o_free), 0);
+    const uint32_t o_free_even = mapa_u32(smem_u32(&ctl.o_free), 0);
     int item = 0;
     Walk walk(p, stretch);
     Item it;
@@ -904,54 +973,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tile_token = it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens;  // first token row
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
       const bool whole = it.first == 0 && it.last == it.steps;
-      // Half of the row's gate is there before the row is, the rest is asked for as it is used up: nothing of the next
-      // tile's O can be added before this one's has been read.
-      constexpr int WINDOW = 4;  // of 32 values
-      uint4 gates[WINDOW][4];
+      const bool mine = quadrant * 32 < rows;
       const uint4* gate = nullptr;
-      if (p.gate && whole && quadrant * 32 < rows) {
+      if (p.gate && whole && mine) {
         gate = reinterpret_cast<const uint4*>(gate_row(p, tile_token, it.head, min(r, rows - 1)));
 #pragma unroll
-        for (int k = 0; k < WINDOW; ++k) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) gates[k][e] = __ldg(gate + 4 * k + e);
-        }
+        for (int k = 0; k < D / 64; ++k) prefetch_l2(gate + 8 * k);
       }
-      ok = ok && warp_wait(&stats_full, item & 1, p.status) && warp_wait(&o_full, item & 1, p.status);
+      ok = ok && warp_wait(&ctl.stats_full, item & 1, p.status) && warp_wait(&ctl.o_full, item & 1, p.status);
       tc_fence_after_sync();
-      const float m = row_max[r], sum = row_sum[r];
+      const float m0 = ctl.row_max[0][r], m1 = ctl.row_max[1][r], m = fmaxf(m0, m1), base = m == -INFINITY ? 0.0f : m;
+      const float sum = ctl.row_sum[0][r] * exp2_approx(m0 - base) + ctl.row_sum[1][r] * exp2_approx(m1 - base);
       if (whole) {
         const bool blind = ahead + r / p.group < 0;  // sees no key
-        const float scale = blind ? 0.0f : 1.0f / sum;
-        if (ok && quadrant * 32 < rows) {
-          uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
-          const F32x2 scale2 = f32x2_splat(scale);
-#pragma unroll 1
-          for (int base = 0; base < D / 32; base += WINDOW) {
+        const F32x2 scale2 = f32x2_splat(blind ? 0.0f : 1.0f / sum);
+        // The row as BF16, so that O is free for the next tile before gate and stores.  A gated row is rounded a second
+        // time behind its gate (2^-8 each), as where the gate is an operation of its own.
+        uint32_t held[D / 2];
+        if (ok && mine) {
 #pragma unroll
-            for (int k = 0; k < WINDOW; ++k) {
-              uint32_t o[32];
-              tmem_ld32(tmem_o + lanes + 32 * (base + k), o);
-              tmem_ld_wait();
+          for (int k = 0; k < D / 32; ++k) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + lanes + 32 * k, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  F32x2 v = mul2(f32x2(__uint_as_float(o[16 * h + 2 * i]), __uint_as_float(o[16 * h + 2 * i + 1])), scale2);
-                  if (gate) {
-                    const uint4 g = gates[k][2 * h + i / 4];
-                    v = gated(v, i % 4 == 0 ? g.x : i % 4 == 1 ? g.y : i % 4 == 2 ? g.z : g.w);
-                  }
-                  w[i] = blind ? 0u : f32x2_to_bf16x2(v);
-                }
-                if (r < rows) store_words8(out + 32 * (base + k) + 16 * h, w);
-                if (gate) {  // (the last window's is asked for again)
-                  const uint4* next = gate + 4 * (min(base + WINDOW, D / 32 - WINDOW) + k) + 2 * h;
-                  gates[k][2 * h] = __ldg(next);
-                  gates[k][2 * h + 1] = __ldg(next + 1);
-                }
-              }
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t w = f32x2_to_bf16x2(mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), scale2));
+              held[16 * k + i] = blind ? 0u : w;
             }
           }
         }
@@ -959,7 +1007,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive_remote_light(o_free_even);
-          mbar_arrive(&stats_free);
+          mbar_arrive(&ctl.stats_free);
+        }
+        if (ok && mine) {
+          uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            if (gate) {
+              uint4 g[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) g[e] = __ldg(gate + 4 * k + e);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t* w = held + 16 * k + 4 * e;
+                w[0] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[0]), g[e].x));
+                w[1] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[1]), g[e].y));
+                w[2] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[2]), g[e].z));
+                w[3] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[3]), g[e].w));
+              }
+            }
+            if (r < rows) {
+              store_words8(out + 32 * k, held + 16 * k);
+              store_words8(out + 32 * k + 16, held + 16 * k + 8);
+            }
+          }
         }
       } else {
         // the pair that the tile begins in, and the last one that it reaches, with the cuts where they moved to
@@ -991,25 +1062,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         __threadfence();
         named_barrier(1, 128);
         unsigned int* ticket = p.tickets + 2 * c0 + rank;
-        if (thread == 0) last_part = rows > 0 && atomicAdd(ticket, 1u) == static_cast<unsigned>(c1 - c0);
+        if (thread == 0) ctl.last_part = rows > 0 && atomicAdd(ticket, 1u) == static_cast<unsigned>(c1 - c0);
         named_barrier(1, 128);
-        if (last_part) {
+        if (ctl.last_part) {
           __threadfence();
           // row_max and row_sum have been read by their rows' threads: here they hold what the parts have in common
           if (c1 - c0 < 8) {
-            join_stats<1>(p, c0, c1, rank, rows, thread, row_max, row_sum);
+            join_stats<1>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
           } else {
-            join_stats<8>(p, c0, c1, rank, rows, thread, row_max, row_sum);
+            join_stats<8>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
           }
           if (c1 - c0 < 2) {
-            join_rows<D, 6, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, row_max, row_sum);
+            join_rows<D, 6, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           } else {
-            join_rows<D, 3, 4>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, row_max, row_sum);
+            join_rows<D, 3, 4>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           }
           if (thread == 0) *ticket = 0u;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&stats_free);
+        if (lane == 0) mbar_arrive(&ctl.stats_free);
         named_barrier(1, 128);  // `last_part` is written again
       }
       ++item;
@@ -1027,7 +1098,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, bool PAGED>
 static cudaError_t prepare_one() {
-  return cudaFuncSetAttribute(attention_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SHARED);
+  return cudaFuncSetAttribute(attention_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes<D>());
 }
 
 cudaError_t attention_prepare() {
@@ -1043,7 +1114,7 @@ cudaError_t launch_attention(cudaStream_t stream, int dim, int pairs, const CUte
                              const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p) {
   auto kernel = p.block_table ? (dim == 256 ? attention_kernel<256, true> : attention_kernel<128, true>)
                               : (dim == 256 ? attention_kernel<256, false> : attention_kernel<128, false>);
-  return launch_kernel_cluster(kernel, dim3(2 * pairs), dim3(kThreads), dim == 256 ? Shape<256>::SHARED : Shape<128>::SHARED,
+  return launch_kernel_cluster(kernel, dim3(2 * pairs), dim3(kThreads), dim == 256 ? shared_bytes<256>() : shared_bytes<128>(),
                                stream, dim3(2, 1, 1), map_q, map_q1, map_k, map_v, p);
 }
 

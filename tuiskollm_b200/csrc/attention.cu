@@ -44,7 +44,7 @@ struct Shape {
   static constexpr int K_KEYS = kKeys / 2;   // a K unit: half of the keys, all chunks
   static constexpr int V_CHUNKS = CHUNKS / 2;  // a V unit: all keys, half of the chunks
   static constexpr int UNIT = K_KEYS * 2 * D;  // bytes of a ring stage
-  static constexpr int STAGES = D == 256 ? 5 : 12;
+  static constexpr int STAGES = D == 256 ? 4 : 7;
 };
 
 // ----------------------------------------------------------------- the line of keys
@@ -73,16 +73,12 @@ __device__ __forceinline__ int tile_count(const AttentionParams& p, const Sequen
   return (s.q + p.tile_tokens - 1) / p.tile_tokens;
 }
 
-// What a tile costs besides its keys, in keys: the last step is half empty on average, and a tile's first scores and
-// last rows are not all hidden behind its neighbours' steps.
-constexpr int kTileKeys = 192;
-
 __device__ __forceinline__ int tile_cost(const AttentionParams& p, const Sequence& s, int i) {
-  return kTileKeys + tile_limit(p, s, i);
+  return p.tile_keys + tile_limit(p, s, i);
 }
 // Cost of the first i tiles of one key/value head, an arithmetic series but for tiles that see nothing and the last.
 __device__ __forceinline__ long long cost_before(const AttentionParams& p, const Sequence& s, int i, int tiles) {
-  long long sum = static_cast<long long>(i) * kTileKeys;
+  long long sum = static_cast<long long>(i) * p.tile_keys;
   int full = i;  // tiles whose last token is their own
   if (i == tiles && i > 0) {
     sum += max(s.kv, 0);
@@ -142,29 +138,31 @@ __device__ __forceinline__ void describe(const AttentionParams& p, const Sequenc
 // The pair's items.  A tile that it begins and another pair goes on with comes first: with the tile that it goes on
 // with itself, parts are there early and are joined while the whole tiles run.
 struct Walk {
+  const Stretch& ends;  // in shared memory: every role walks, and few of its registers are free
   int sequence, head, tile, step, tiles;
   long long line;
   Sequence seq;
-  Place to;
+  bool tail;
 
   __device__ __forceinline__ Walk(const AttentionParams& p, const Stretch& s)
-      : sequence(s.from.sequence), head(s.from.head), tile(s.from.tile), step(s.from.step), tiles(0), line(s.from.line),
-        to(s.to) {
+      : ends(s), sequence(s.from.sequence), head(s.from.head), tile(s.from.tile), step(s.from.step), tiles(0),
+        line(s.from.line), tail(s.to.step > 0) {
     seq = {0, 0, 0};
-    if (line < to.line) {
+    if (line < s.to.line) {
       seq = read_sequence(p, sequence);
       tiles = tile_count(p, seq);
     }
   }
   __device__ __forceinline__ bool next(const AttentionParams& p, Item* it) {
-    if (to.step > 0) {
+    if (tail) {
+      tail = false;
+      const Place to = ends.to;
       describe(p, read_sequence(p, to.sequence), to.sequence, to.head, to.tile, to.line, it);
       it->first = to.line == line ? step : 0;  // both ends in one tile: its only item
       it->last = to.step;
-      to.step = 0;
       return true;
     }
-    if (line >= to.line) return false;
+    if (line >= ends.to.line) return false;
     while (tile >= tiles) {  // the next head, or the next sequence that has tokens
       tile = 0;
       if (tiles == 0 || ++head == p.kv_heads) {
@@ -177,7 +175,7 @@ struct Walk {
     describe(p, seq, sequence, head, tile, line, it);
     it->first = step;
     it->last = it->steps;
-    line += kTileKeys + it->limit;
+    line += p.tile_keys + it->limit;
     step = 0;
     ++tile;
     return true;
@@ -206,13 +204,13 @@ struct Steps {
 
 struct Scratch {
   long long warp_sums[kThreads / 32];
-  Place cut[2];
+  int sequence[2];
   long long rest[2];
 };
 
 // Finds the pair's stretch.  All threads sum up the sequences' costs; the thread that passes a cut names the
 // sequence, and one warp per cut finds head and tile in it.
-__device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratch& sh) {
+__device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh, Stretch& found) {
   const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
   const int run = (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
@@ -238,15 +236,13 @@ __device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratc
     total += sh.warp_sums[w];
   }
   before += sum - mine;
-  Stretch r = {};
   const long long least = static_cast<long long>(p.min_steps) * kKeys;
-  r.share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), least);
-  const long long first = min(static_cast<long long>(blockIdx.x / 2) * r.share, total), last = min(first + r.share, total);
-  if (first == last) return r;  // (all threads alike)
+  const long long share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), least);
+  const long long first = min(static_cast<long long>(blockIdx.x / 2) * share, total), last = min(first + share, total);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const long long u = k == 0 ? first : last;
-    if (before <= u && u < before + mine) {
+    if (first < last && before <= u && u < before + mine) {
       long long rest = u - before;
       int s = s0;
       for (;; ++s) {
@@ -255,7 +251,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratc
         if (rest < cost) break;
         rest -= cost;
       }
-      sh.cut[k].sequence = s;
+      sh.sequence[k] = s;
       sh.rest[k] = rest;
     }
   }
@@ -264,8 +260,8 @@ __device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratc
     const long long u = warp == 0 ? first : last;
     Place at = {};
     at.line = u;
-    if (u < total) {
-      at.sequence = sh.cut[warp].sequence;
+    if (first < last && u < total) {
+      at.sequence = sh.sequence[warp];
       const Sequence q = read_sequence(p, at.sequence);
       const int tiles = tile_count(p, q);
       const long long per_head = cost_before(p, q, tiles, tiles);
@@ -293,13 +289,10 @@ __device__ __forceinline__ Stretch find_stretch(const AttentionParams& p, Scratc
         ++at.tile;
       }
     }
-    __syncwarp();
-    if (lane == 0) sh.cut[warp] = at;
+    if (lane == 0) (warp == 0 ? found.from : found.to) = at;
+    if (t == 0) found.share = share;
   }
   __syncthreads();
-  r.from = sh.cut[0];
-  r.to = sh.cut[1];
-  return r;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -548,6 +541,7 @@ struct Control {
   uint64_t reference_set[2][4];
   uint32_t tmem_base;
   int last_part;
+  Stretch stretch;
   float reference[kRows];  // the row's reference maximum, of the step before
   float row_sum[2][kRows];  // what either softmax warpgroup has of a row at a tile's end
   union {
@@ -622,10 +616,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   cluster_arrive();  // both CTAs' barriers exist before either touches the other's
-  const Stretch stretch = find_stretch(p, ctl.scratch);
+  find_stretch(p, ctl.scratch, ctl.stretch);
   cluster_wait();
   tc_fence_after_sync();
   const uint32_t tmem = ctl.tmem_base;
+  const Stretch& stretch = ctl.stretch;
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int v_box = PAGED ? min(kKeys, 1 << p.page_shift) : kKeys;  // keys of a box of V
 
@@ -1035,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // the pair that the tile begins in, and the last one that it reaches, with the cuts where they moved to
         const int margin = cut_margin(p, it.tokens);
-        const long long inner = static_cast<long long>(margin) * kKeys, cost = kTileKeys + it.limit;
+        const long long inner = static_cast<long long>(margin) * kKeys, cost = p.tile_keys + it.limit;
         const long long outer = max(inner, static_cast<long long>(it.steps - margin + 1) * kKeys);
         const int c0 = static_cast<int>(divide(it.line + min(inner, cost) - 1, stretch.share));
         const int c1 = static_cast<int>(divide(it.line + min(outer, cost) - 1, stretch.share));

@@ -249,6 +249,7 @@ Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, 
   p->tile_tokens = 2 * p->half_tokens;
   p->scale_log2 = scale * 1.4426950408889634f;
   p->min_steps = 1;
+  p->tile_keys = head_dim == 256 ? 512 : 224;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   const size_t rows = 2 * static_cast<size_t>(ctx_.sm_count()) * kAttentionRows;
   p->tickets = reinterpret_cast<unsigned int*>(w);

@@ -10,6 +10,7 @@ model step through the compiled binding (csrc/binding.cpp), the rest through cty
 from __future__ import annotations
 
 import ctypes as C
+import types
 from typing import Optional
 
 import torch
@@ -55,6 +56,11 @@ def _launch(name, context, stream, *arguments):
                      *[_ptr(a) if t is C.c_void_p else a for a, t in zip(arguments, types, strict=True)]))
 
 
+def _not_read(*_):
+    """Stands in for the compiled binding's plane readers."""
+    return None
+
+
 class Context:
     """Owns one ``tk100_ctx`` (one per GPU / rank)."""
 
@@ -63,6 +69,9 @@ class Context:
                  workspace_bytes: int = 0):
         self._lib = _lib.load()
         self._native = _lib.native(_launch)
+        compiled = isinstance(self._native, types.ModuleType)
+        self._plane = self._native.plane if compiled else _not_read
+        self._heads = self._native.heads if compiled else _not_read
         cfg = _lib.Config(_lib.ABI_VERSION, device, hidden, intermediate, rms_norm_epsilon,
                           max_rows, workspace_bytes)
         handle = C.c_void_p()
@@ -362,35 +371,48 @@ class GdnRecurrenceOp:
 
 def _plane(context: Context, t, name, dtype, least):
     """Address of a contiguous plane of at least `least` values of one type on the context's device."""
-    if t.dtype != dtype or t.device.type != "cuda" or t.device.index != context.device:
-        raise GpuError(5, f"[gpu.launch] {name}: a {dtype} plane on the context's device is required, got {t.dtype} "
-                          f"on {t.device}")
+    address = context._plane(t, dtype, context.device, least)
+    if address is not None:
+        return address
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device.type != "cuda" or t.device.index != context.device:
+        got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise GpuError(5, f"[gpu.launch] {name}: a {dtype} plane on the context's device is required, got {got}")
     if t.numel() < least or not t.is_contiguous():
         raise GpuError(5, f"[gpu.launch] {name}: a contiguous plane of at least {least} values is required, got "
                           f"shape {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _heads(context: Context, t, name, shape):
-    """(address, strides) of a BF16 plane of the given shape (None: any extent) whose last dimension is dense."""
-    if t.dtype != torch.bfloat16 or t.device.type != "cuda" or t.device.index != context.device:
-        raise GpuError(5, f"[gpu.launch] {name}: a torch.bfloat16 plane on the context's device is required, got "
-                          f"{t.dtype} on {t.device}")
-    if t.dim() != len(shape) or any(b is not None and a != b for a, b in zip(t.shape, shape)):
+def _heads(context: Context, t, name, *shape):
+    """(address, strides, first extent) of a BF16 plane of the given shape (-1: any extent) whose last dimension is
+    dense.  An extent of one has the stride of a dense plane, whatever the tensor says of it."""
+    found = context._heads(t, context.device, *shape)
+    if found is not None:
+        return found
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device.type != "cuda" \
+            or t.device.index != context.device:
+        got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise GpuError(5, f"[gpu.launch] {name}: a torch.bfloat16 plane on the context's device is required, got {got}")
+    if t.dim() != len(shape) or any(b >= 0 and a != b for a, b in zip(t.shape, shape)):
         raise GpuError(5, f"[gpu.launch] {name}: shape {tuple(t.shape)} is not {shape}")
-    strides = t.stride()
-    if strides[-1] != 1 and t.shape[-1] > 1:
+    strides, dense = [], 1
+    for extent, stride in zip(reversed(t.shape), reversed(t.stride())):
+        strides.append(dense if extent == 1 else stride)
+        dense = strides[-1] * extent
+    strides = tuple(reversed(strides))
+    if strides[-1] != 1:
         raise GpuError(5, f"[gpu.launch] {name}: the values of a head are not next to each other")
-    return t.data_ptr(), strides
+    return t.data_ptr(), strides, t.shape[0]
 
 
 def _cache(context: Context, key_cache, value_cache, kv_heads, head_dim):
     """(addresses, pages, page tokens, strides) of a cache pair ``[pages, page tokens, heads, head_dim]``."""
-    key, strides = _heads(context, key_cache, "key cache", (None, None, kv_heads, head_dim))
-    value, others = _heads(context, value_cache, "value cache", key_cache.shape)
+    key, strides, pages = _heads(context, key_cache, "key cache", -1, -1, kv_heads, head_dim)
+    page_tokens = key_cache.shape[1]
+    value, others, _ = _heads(context, value_cache, "value cache", pages, page_tokens, kv_heads, head_dim)
     if strides != others:
         raise GpuError(5, f"[gpu.launch] key and value cache have different strides {strides} and {others}")
-    return key, value, key_cache.shape[0], key_cache.shape[1], strides
+    return key, value, pages, page_tokens, strides
 
 
 class PagePlanOp:
@@ -487,14 +509,15 @@ class RotaryCacheOp:
         ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output`` dense or None; caches
         ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
         c, dim = self.ctx, self.head_dim
-        q, qs = _heads(c, query, "query", (None, self.q_heads, dim))
-        k, ks = _heads(c, key, "key", (None, self.kv_heads, dim))
+        q, qs, q_rows = _heads(c, query, "query", -1, self.q_heads, dim)
+        k, ks, rows = _heads(c, key, "key", -1, self.kv_heads, dim)
         v = None
         if value is not None:
-            v, vs = _heads(c, value, "value", (None, self.kv_heads, dim))
+            v, vs, v_rows = _heads(c, value, "value", -1, self.kv_heads, dim)
+            rows = min(rows, v_rows)
             if vs != ks:
                 raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
-        if min(query.shape[0], key.shape[0], key.shape[0] if value is None else value.shape[0]) < tokens:
+        if q_rows < tokens or rows < tokens:
             raise GpuError(5, f"[gpu.launch] rotary: planes have fewer than {tokens} rows")
         axes = 1 if positions.dim() == 1 else positions.shape[0]
         if positions.shape[-1] != tokens:
@@ -522,25 +545,23 @@ class _AttentionOp:
     def __init__(self, context: Context, q_heads: int, kv_heads: int, head_dim: int, scale: Optional[float] = None):
         self.ctx, self.q_heads, self.kv_heads, self.head_dim = context, q_heads, kv_heads, head_dim
         self.scale = float(scale if scale is not None else head_dim ** -0.5)
+        self._workspace_bytes = int(context._lib.tk100_attention_workspace_bytes(context.handle, head_dim))
 
     def workspace(self):
         """A zeroed workspace.  Launches one behind the other share one; launches that may overlap (two streams,
         two captured graphs) need one each."""
-        nbytes = int(self.ctx._lib.tk100_attention_workspace_bytes(self.ctx.handle, self.head_dim))
-        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", self.ctx.device))
+        return torch.zeros(self._workspace_bytes, dtype=torch.uint8, device=torch.device("cuda", self.ctx.device))
 
     def _rows(self, sequences, starts, query, gate, workspace, output):
         c, dim = self.ctx, self.head_dim
-        q, qs = _heads(c, query, "query", (None, self.q_heads, dim))
+        q, qs, tokens = _heads(c, query, "query", -1, self.q_heads, dim)
         g = None
         if gate is not None:
-            g, gs = _heads(c, gate, "gate", query.shape)
+            g, gs, _ = _heads(c, gate, "gate", tokens, self.q_heads, dim)
             if gs != qs:
                 raise GpuError(5, f"[gpu.launch] query and gate have different strides {qs} and {gs}")
-        tokens = query.shape[0]
-        need = int(c._lib.tk100_attention_workspace_bytes(c.handle, dim))
         return (tokens, q, g, qs, _plane(c, starts, "starts", torch.int32, sequences + 1),
-                _plane(c, workspace, "workspace", torch.uint8, need),
+                _plane(c, workspace, "workspace", torch.uint8, self._workspace_bytes),
                 _plane(c, output, "output", torch.bfloat16, tokens * self.q_heads * dim))
 
 
@@ -576,9 +597,8 @@ class PromptAttentionOp(_AttentionOp):
     def launch(self, stream, sequences, starts, query, gate, key, value, workspace, output):
         c = self.ctx
         tokens, q, g, qs, at, work, out = self._rows(sequences, starts, query, gate, workspace, output)
-        shape = (tokens, self.kv_heads, self.head_dim)
-        k, ks = _heads(c, key, "key", shape)
-        v, vs = _heads(c, value, "value", shape)
+        k, ks, _ = _heads(c, key, "key", tokens, self.kv_heads, self.head_dim)
+        v, vs, _ = _heads(c, value, "value", tokens, self.kv_heads, self.head_dim)
         if vs != ks:
             raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
         c._native.tk100_prompt_attention(c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,

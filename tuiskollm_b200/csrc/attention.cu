@@ -208,25 +208,104 @@ struct Scratch {
   long long rest[2];
 };
 
-// Finds the pair's stretch.  All threads sum up the sequences' costs; the thread that passes a cut names the
-// sequence, and one warp per cut finds head and tile in it.
-__device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh, Stretch& found) {
-  const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
-  const int run = (p.sequences + kThreads - 1) / kThreads;
-  const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
-  long long mine = 0;
-  for (int s = s0; s < s1; ++s) {
-    const Sequence q = read_sequence(p, s);
-    mine += cost_before(p, q, tile_count(p, q), tile_count(p, q)) * p.kv_heads;
-    if (blockIdx.x == 0 && (q.start != p.starts[s] || q.start + q.q != p.starts[s + 1] || (p.kv_lengths && q.kv != p.kv_lengths[s])))
-      atomicOr(p.status, STATUS_BAD_ARGUMENT);  // lengths outside the planes are cut to them
+// Where cut u of the line falls, `rest` behind the first tile of sequence `sequence`, and where it moves to: by a warp,
+// which bisects the sequence's tiles 32 at a time.
+__device__ __forceinline__ Place locate(const AttentionParams& p, const Sequence& q, int sequence, long long rest, long long u,
+                                        int lane) {
+  Place at;
+  at.sequence = sequence;
+  const int tiles = tile_count(p, q);
+  const long long per_head = cost_before(p, q, tiles, tiles);
+  at.head = static_cast<int>(divide(rest, per_head));
+  rest -= at.head * per_head;
+  int low = 0, high = tiles;  // cost_before(low) <= rest < cost_before(high)
+  while (high - low > 1) {
+    const int width = (high - low + 31) / 32, probe = low + (lane + 1) * width;
+    const bool behind = probe < high && cost_before(p, q, probe, tiles) <= rest;
+    low += __popc(__ballot_sync(0xffffffffu, behind)) * width;
+    high = min(high, low + width);
   }
-  long long sum = mine;
+  at.tile = low;
+  rest -= cost_before(p, q, low, tiles);
+  at.line = u - rest;
+  at.step = static_cast<int>(static_cast<unsigned long long>(rest) / kKeys);
+  const int steps = tile_steps(p, q, low);
+  const int margin = cut_margin(p, min(p.tile_tokens, q.q - low * p.tile_tokens));
+  if (at.step < margin) {
+    at.step = 0;
+  } else if (steps - at.step < margin) {
+    at.step = 0;
+    at.line += tile_cost(p, q, low);
+    ++at.tile;
+  }
+  return at;
+}
+
+// The pair's even cuts; returns the keys of a pair.
+__device__ __forceinline__ long long even_cuts(const AttentionParams& p, long long total, long long (&cuts)[2]) {
+  const long long share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), static_cast<long long>(p.min_steps) * kKeys);
+  cuts[0] = min(static_cast<long long>(blockIdx.x / 2) * share, total);
+  cuts[1] = min(cuts[0] + share, total);
+  return share;
+}
+__device__ __forceinline__ long long sequence_cost(const AttentionParams& p, const Sequence& q) {
+  const int tiles = tile_count(p, q);
+  return cost_before(p, q, tiles, tiles) * p.kv_heads;
+}
+// Lengths outside the planes are cut to them, and reported.
+__device__ __forceinline__ void report_cut(const AttentionParams& p, const Sequence& q, int s) {
+  if (blockIdx.x == 0 && (q.start != p.starts[s] || q.start + q.q != p.starts[s + 1] || (p.kv_lengths && q.kv != p.kv_lengths[s])))
+    atomicOr(p.status, STATUS_BAD_ARGUMENT);
+}
+__device__ __forceinline__ long long warp_scan(long long sum, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += x;
   }
+  return sum;
+}
+
+// Finds the pair's stretch; warp 0 has its beginning, warp 1 its end.  Up to 32 sequences a lane each, so that a warp
+// needs no other; beyond, all threads sum up the sequences' costs and the thread that passes a cut names the sequence.
+__device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& sh, Stretch& found) {
+  const int t = static_cast<int>(threadIdx.x), lane = t & 31, warp = t >> 5;
+  long long cuts[2];
+  if (p.sequences <= 32) {
+    if (warp < 2) {
+      Sequence q = {0, 0, 0};
+      long long mine = 0;
+      if (lane < p.sequences) {
+        q = read_sequence(p, lane);
+        mine = sequence_cost(p, q);
+        if (warp == 0) report_cut(p, q, lane);
+      }
+      const long long sum = warp_scan(mine, lane), total = __shfl_sync(0xffffffffu, sum, 31);
+      const long long share = even_cuts(p, total, cuts), u = warp == 0 ? cuts[0] : cuts[1];
+      Place at = {};
+      at.line = u;
+      if (cuts[0] < cuts[1] && u < total) {
+        const int s = __ffs(__ballot_sync(0xffffffffu, u < sum)) - 1;
+        const long long rest = u - __shfl_sync(0xffffffffu, sum - mine, s);
+        const Sequence its = {__shfl_sync(0xffffffffu, q.start, s), __shfl_sync(0xffffffffu, q.q, s),
+                              __shfl_sync(0xffffffffu, q.kv, s)};
+        at = locate(p, its, s, rest, u, lane);
+      }
+      if (lane == 0) (warp == 0 ? found.from : found.to) = at;
+      if (t == 0) found.share = share;
+    }
+    __syncthreads();
+    return;
+  }
+  const int run = (p.sequences + kThreads - 1) / kThreads;
+  const int s0 = min(t * run, p.sequences), s1 = min(s0 + run, p.sequences);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Sequence q = read_sequence(p, s);
+    mine += sequence_cost(p, q);
+    report_cut(p, q, s);
+  }
+  const long long sum = warp_scan(mine, lane);
   if (lane == 31) sh.warp_sums[warp] = sum;
   __syncthreads();
   long long before = 0, total = 0;
@@ -236,18 +315,14 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
     total += sh.warp_sums[w];
   }
   before += sum - mine;
-  const long long least = static_cast<long long>(p.min_steps) * kKeys;
-  const long long share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), least);
-  const long long first = min(static_cast<long long>(blockIdx.x / 2) * share, total), last = min(first + share, total);
+  const long long share = even_cuts(p, total, cuts);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const long long u = k == 0 ? first : last;
-    if (first < last && before <= u && u < before + mine) {
-      long long rest = u - before;
+    if (cuts[0] < cuts[1] && before <= cuts[k] && cuts[k] < before + mine) {
+      long long rest = cuts[k] - before;
       int s = s0;
       for (;; ++s) {
-        const Sequence q = read_sequence(p, s);
-        const long long cost = cost_before(p, q, tile_count(p, q), tile_count(p, q)) * p.kv_heads;
+        const long long cost = sequence_cost(p, read_sequence(p, s));
         if (rest < cost) break;
         rest -= cost;
       }
@@ -257,38 +332,11 @@ __device__ __forceinline__ void find_stretch(const AttentionParams& p, Scratch& 
   }
   __syncthreads();
   if (warp < 2) {
-    const long long u = warp == 0 ? first : last;
+    const long long u = warp == 0 ? cuts[0] : cuts[1];
     Place at = {};
     at.line = u;
-    if (first < last && u < total) {
-      at.sequence = sh.sequence[warp];
-      const Sequence q = read_sequence(p, at.sequence);
-      const int tiles = tile_count(p, q);
-      const long long per_head = cost_before(p, q, tiles, tiles);
-      long long rest = sh.rest[warp];
-      at.head = static_cast<int>(divide(rest, per_head));
-      rest -= at.head * per_head;
-      int low = 0, high = tiles;  // cost_before(low) <= rest < cost_before(high)
-      while (high - low > 1) {
-        const int width = (high - low + 31) / 32, probe = low + (lane + 1) * width;
-        const bool behind = probe < high && cost_before(p, q, probe, tiles) <= rest;
-        low += __popc(__ballot_sync(0xffffffffu, behind)) * width;
-        high = min(high, low + width);
-      }
-      at.tile = low;
-      rest -= cost_before(p, q, low, tiles);
-      at.line = u - rest;
-      at.step = static_cast<int>(rest / kKeys);
-      const int steps = tile_steps(p, q, low);
-      const int margin = cut_margin(p, min(p.tile_tokens, q.q - low * p.tile_tokens));
-      if (at.step < margin) {
-        at.step = 0;
-      } else if (steps - at.step < margin) {
-        at.step = 0;
-        at.line += tile_cost(p, q, low);
-        ++at.tile;
-      }
-    }
+    if (cuts[0] < cuts[1] && u < total)
+      at = locate(p, read_sequence(p, sh.sequence[warp]), sh.sequence[warp], sh.rest[warp], u, lane);
     if (lane == 0) (warp == 0 ? found.from : found.to) = at;
     if (t == 0) found.share = share;
   }
@@ -419,6 +467,19 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Loads past L1 that stay where they are written: left to itself the compiler moves each of them into the branch
+// that uses it, and a join of 19 parts waits for L2 60 times instead of 4.
+__device__ __forceinline__ float4 load_part(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float2 load_part(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+
 // The rows' common maximum, and 1 / the sum of their weights, with LANES lanes of the 128 threads to a row.
 template <int LANES>
 __device__ __forceinline__ void join_stats(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread,
@@ -432,7 +493,7 @@ __device__ __forceinline__ void join_stats(const AttentionParams& p, int c0, int
     for (int k = c0 + lane; k <= c1; k += 4 * LANES) {
       float2 stats[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) stats[e] = __ldcg(p.part_stats + part_slot(min(k + e * LANES, c1), c0, rank) * kRows + from);
+      for (int e = 0; e < 4; ++e) stats[e] = load_part(p.part_stats + part_slot(min(k + e * LANES, c1), c0, rank) * kRows + from);
       float most = top;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -493,8 +554,8 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
         const size_t slot = part_slot(min(k + e, c1), c0, rank);
 #pragma unroll
         for (int i = 0; i < PLACES; ++i) {
-          stats[i][e] = __ldcg(p.part_stats + slot * kRows + row[i]);
-          o[i][e] = __ldcg(reinterpret_cast<const float4*>(p.parts) + slot * kRows * (D / 4) + at[i]);
+          stats[i][e] = load_part(p.part_stats + slot * kRows + row[i]);
+          o[i][e] = load_part(reinterpret_cast<const float4*>(p.parts) + slot * kRows * (D / 4) + at[i]);
         }
       }
 #pragma unroll
@@ -1068,9 +1129,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             join_stats<8>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
           }
           if (c1 - c0 < 2) {
-            join_rows<D, 6, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
+            join_rows<D, 4, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           } else {
-            join_rows<D, 3, 4>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
+            join_rows<D, 3, 5>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           }
           if (thread == 0) *ticket = 0u;
         }

@@ -10,9 +10,10 @@
 // remainder in [-1/2, 1/2] is rounded to fp32 (3e-8 of a turn) for sincospif.
 //
 // HBM-bound for many tokens (each query, key and value read once and written once), latency-bound for few.
-// One CTA per token: R/2 threads form the token's sines and cosines once for all heads while every warp
-// already holds its first head; a head is DIM / 8 lanes of 16 bytes, so the partner of a lane in a rotation is
-// R / 16 lanes away and comes by shuffle.
+// A CTA has TOKENS tokens: its threads form their sines and cosines once for all heads while every thread already
+// holds DEPTH heads' values; a head is DIM / 8 lanes of 16 bytes, so the partner of a lane in a rotation is R / 16
+// lanes away and comes by shuffle.  One token a CTA leaves most threads idle in the first half and has its chain of
+// loads, angles and stores to itself (8192 tokens of 32 + 8 heads of 128: 66 us); four share it.
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
@@ -21,150 +22,166 @@ namespace tk100 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRotaryManyTokens = 1024;
 
-template <int DIM>
+template <int DIM, int TOKENS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   constexpr int LANES = DIM / 8;             // lanes of a head
   constexpr int AT_ONCE = kThreads / LANES;  // heads of a CTA side by side
-  __shared__ float2 turn[DIM / 2];
+  constexpr int DEPTH = 4;                   // and one behind the other, all of them requested at once
+  __shared__ float2 turn[TOKENS][DIM / 2];
+  __shared__ long long places[TOKENS];  // of the tokens in the cache, -1: nowhere
   pdl_wait();
   pdl_trigger();
 
-  const int token = static_cast<int>(blockIdx.x);
+  const int first_token = static_cast<int>(blockIdx.x) * TOKENS, tokens = min(TOKENS, p.tokens - first_token);
   const int lane = static_cast<int>(threadIdx.x) % LANES, group = static_cast<int>(threadIdx.x) / LANES;
-  const int cached = p.key_cache ? p.kv_heads : 0;
-  const int heads = p.q_heads + p.kv_heads + cached;  // queries, keys, values that go to the cache
+  const int heads = p.q_heads + p.kv_heads + (p.key_cache ? p.kv_heads : 0);  // queries, keys, values for the cache
 
-  auto load = [&](int h) -> uint4 {
-    const uint16_t* src;
-    if (h < p.q_heads) {
-      src = p.query + static_cast<size_t>(token) * p.query_token_stride + static_cast<size_t>(h) * p.query_head_stride;
-    } else {
-      h -= p.q_heads;
-      src = p.key;
-      if (h >= p.kv_heads) {
-        h -= p.kv_heads;
-        src = p.value;
-      }
-      src += static_cast<size_t>(token) * p.kv_token_stride + static_cast<size_t>(h) * p.kv_head_stride;
+  // The thread's heads are the same ones for every token: where they are read, by how much a token moves that, and
+  // what becomes of them are found once.
+  const uint16_t* from[DEPTH];
+  int token_stride[DEPTH];
+  auto find = [&](int base) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      int h = min(base + d * AT_ONCE + group, heads - 1);
+      const bool query = h < p.q_heads;
+      if (!query) h -= p.q_heads;
+      const uint16_t* plane = query ? p.query : h < p.kv_heads ? p.key : p.value;
+      if (!query && h >= p.kv_heads) h -= p.kv_heads;
+      token_stride[d] = query ? p.query_token_stride : p.kv_token_stride;
+      from[d] = plane + static_cast<size_t>(first_token) * token_stride[d] +
+                static_cast<size_t>(h) * (query ? p.query_head_stride : p.kv_head_stride) + 8 * lane;
     }
-    return *reinterpret_cast<const uint4*>(src + 8 * lane);
   };
+  uint4 raw[DEPTH];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+      raw[d] = *reinterpret_cast<const uint4*>(from[d] + static_cast<size_t>(t) * token_stride[d]);
+  };
+  find(0);
+  request(0);
 
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  if (group < heads) raw = load(group);
-
-  for (int i = threadIdx.x; i < p.half; i += kThreads) {
-    int axis = p.pair_axes ? p.pair_axes[i] : 0;
+  for (int i = threadIdx.x; i < tokens * p.half; i += kThreads) {
+    const int t = TOKENS == 1 ? 0 : i / p.half, pair = i - t * p.half;
+    int axis = p.pair_axes ? p.pair_axes[pair] : 0;
     if (axis >= p.axes) {
       axis = 0;
-      if (token == 0) atomicOr(p.status, STATUS_BAD_ARGUMENT);
+      if (blockIdx.x == 0) atomicOr(p.status, STATUS_BAD_ARGUMENT);
     }
-    const double turns = static_cast<double>(p.positions[static_cast<size_t>(axis) * p.tokens + token]) *
-                         (p.frequencies[i] * 0.15915494309189533577);  // 1 / (2 pi)
+    const double turns = static_cast<double>(p.positions[static_cast<size_t>(axis) * p.tokens + first_token + t]) *
+                         (p.frequencies[pair] * 0.15915494309189533577);  // 1 / (2 pi)
     const float rest = static_cast<float>(turns - rint(turns));
     float s, c;
     sincospif(2.0f * rest, &s, &c);
-    turn[i] = make_float2(c, s);
+    turn[t][pair] = make_float2(c, s);
   }
-
-  // where the token's keys and values go; a negative slot (a padded row) goes nowhere
-  bool stored = false;
-  size_t place = 0;
-  if (p.key_cache) {
-    const long long slot = p.slots[token];
+  // where the tokens' keys and values go; a negative slot (a padded row) goes nowhere
+  if (p.key_cache && static_cast<int>(threadIdx.x) < tokens) {
+    const long long slot = p.slots[first_token + threadIdx.x];
     const long long page = slot >> p.page_shift;
-    stored = slot >= 0 && page < p.pages;
-    if (stored) {
-      place = static_cast<size_t>(page) * p.page_stride +
-              static_cast<size_t>(slot & ((1ll << p.page_shift) - 1)) * p.cache_token_stride;
-    } else if (slot >= 0 && threadIdx.x == 0) {
+    long long place = -1;
+    if (slot >= 0 && page < p.pages) {
+      place = page * p.page_stride + (slot & ((1ll << p.page_shift) - 1)) * p.cache_token_stride;
+    } else if (slot >= 0) {
       atomicOr(p.status, STATUS_BAD_ARGUMENT);
     }
+    places[threadIdx.x] = place;
   }
   __syncthreads();
 
   const int rotary_lanes = p.half / 8;  // lanes of the first half of the rotated values
   const bool first_half = lane < rotary_lanes, second_half = !first_half && lane < 2 * rotary_lanes;
   const int partner = first_half ? lane + rotary_lanes : second_half ? lane - rotary_lanes : lane;
-  float2 mine[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = (first_half ? lane : lane - rotary_lanes) * 8 + j;
-    mine[j] = first_half || second_half ? turn[i] : make_float2(1.0f, 0.0f);
-    if (first_half) mine[j].y = -mine[j].y;
-  }
+  const int pair0 = first_half ? 8 * lane : second_half ? 8 * (lane - rotary_lanes) : 0;
+  const bool normed = p.query_norm || p.key_norm;
 
-  for (int base = 0; base < heads; base += AT_ONCE) {
-    const int h = base + group;
-    const uint4 now = raw;
-    if (h + AT_ONCE < heads) raw = load(h + AT_ONCE);
-    uint16_t* out = nullptr;
-    uint16_t* second = nullptr;
-    const uint16_t* norm = nullptr;
-    bool turns = true;
-    if (h < p.q_heads) {
-      out = p.query_output + (static_cast<size_t>(token) * p.q_heads + h) * DIM;
-      norm = p.query_norm;
-    } else if (h < p.q_heads + p.kv_heads) {
-      const int k = h - p.q_heads;
-      if (stored) out = p.key_cache + place + static_cast<size_t>(k) * p.cache_head_stride;
-      if (p.key_output) second = p.key_output + (static_cast<size_t>(token) * p.kv_heads + k) * DIM;
-      norm = p.key_norm;
-    } else if (h < heads) {
-      if (stored) out = p.value_cache + place + static_cast<size_t>(h - p.q_heads - p.kv_heads) * p.cache_head_stride;
-      turns = false;
+  for (int base = 0; base < heads; base += DEPTH * AT_ONCE) {
+    if (base > 0) {
+      find(base);
+      request(0);
     }
-    uint4 result = now;
-    const uint32_t w[4] = {now.x, now.y, now.z, now.w};
-    float y[8];
+#pragma unroll 1
+    for (int t = 0; t < tokens; ++t) {
+      uint4 now[DEPTH];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      y[2 * j] = bf16x2_lo(w[j]);
-      y[2 * j + 1] = bf16x2_hi(w[j]);
-    }
-    float sum = 0.0f;
+      for (int d = 0; d < DEPTH; ++d) now[d] = raw[d];
+      if (t + 1 < tokens) request(t + 1);
+      const size_t token = static_cast<size_t>(first_token + t);
+      const long long place = p.key_cache ? places[t] : -1;
+      float2 cs[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(y[j], y[j], sum);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (norm) {
-      const float scale = __frsqrt_rn(sum * (1.0f / DIM) + p.epsilon);
-      const uint4 n = *reinterpret_cast<const uint4*>(norm + 8 * lane);
-      const uint32_t v[4] = {n.x, n.y, n.z, n.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[2 * j] = y[2 * j] * scale * (1.0f + bf16x2_lo(v[j]));
-        y[2 * j + 1] = y[2 * j + 1] * scale * (1.0f + bf16x2_hi(v[j]));
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = turn[t][pair0 + j];
+        if (first_half) cs[j].y = -cs[j].y;
       }
-    }
-    float other[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xffffffffu, y[j], partner, LANES);
-    if (turns) {
-      uint32_t r[4];
+      for (int d = 0; d < DEPTH; ++d) {
+        if (base + d * AT_ONCE >= heads) break;
+        const int h = base + d * AT_ONCE + group;
+        const bool query = h < p.q_heads, key = !query && h < p.q_heads + p.kv_heads;
+        const uint16_t* norm = query ? p.query_norm : key ? p.key_norm : nullptr;
+        const uint32_t w[4] = {now[d].x, now[d].y, now[d].z, now[d].w};
+        float y[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float z[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * j + e;
-          // a lane behind the rotated values passes its own on, whatever its sign or kind
-          z[e] = first_half || second_half ? fmaf(y[i], mine[i].x, other[i] * mine[i].y) : y[i];
+        for (int j = 0; j < 4; ++j) {
+          y[2 * j] = bf16x2_lo(w[j]);
+          y[2 * j + 1] = bf16x2_hi(w[j]);
         }
-        r[j] = pack_bf16x2(z[0], z[1]);
+        if (normed) {  // (all lanes: a warp may have heads of two kinds)
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum = fmaf(y[j], y[j], sum);
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (norm) {
+            const float scale = __frsqrt_rn(sum * (1.0f / DIM) + p.epsilon);
+            const uint4 n = __ldg(reinterpret_cast<const uint4*>(norm + 8 * lane));
+            const uint32_t v[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              y[2 * j] = y[2 * j] * scale * (1.0f + bf16x2_lo(v[j]));
+              y[2 * j + 1] = y[2 * j + 1] * scale * (1.0f + bf16x2_hi(v[j]));
+            }
+          }
+        }
+        uint32_t r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = __shfl_sync(0xffffffffu, y[2 * j], partner, LANES), b = __shfl_sync(0xffffffffu, y[2 * j + 1], partner, LANES);
+          // a lane behind the rotated values passes its own on, whatever their sign or kind
+          const bool turns = first_half || second_half;
+          r[j] = pack_bf16x2(turns ? fmaf(y[2 * j], cs[2 * j].x, a * cs[2 * j].y) : y[2 * j],
+                             turns ? fmaf(y[2 * j + 1], cs[2 * j + 1].x, b * cs[2 * j + 1].y) : y[2 * j + 1]);
+        }
+        if (h >= heads) continue;
+        const uint4 result = query || key ? make_uint4(r[0], r[1], r[2], r[3]) : now[d];
+        if (query) {
+          *reinterpret_cast<uint4*>(p.query_output + (token * p.q_heads + h) * DIM + 8 * lane) = result;
+        } else {
+          const int k = h - p.q_heads - (key ? 0 : p.kv_heads);
+          if (place >= 0)
+            *reinterpret_cast<uint4*>((key ? p.key_cache : p.value_cache) + place + static_cast<size_t>(k) * p.cache_head_stride + 8 * lane) = result;
+          if (key && p.key_output)
+            *reinterpret_cast<uint4*>(p.key_output + (token * p.kv_heads + k) * DIM + 8 * lane) = result;
+        }
       }
-      result = make_uint4(r[0], r[1], r[2], r[3]);
     }
-    if (out) *reinterpret_cast<uint4*>(out + 8 * lane) = result;
-    if (second) *reinterpret_cast<uint4*>(second + 8 * lane) = result;
   }
+}
+
+template <int TOKENS>
+cudaError_t launch(cudaStream_t stream, int dim, const RotaryParams& p) {
+  return launch_kernel(dim == 256 ? rotary_kernel<256, TOKENS> : rotary_kernel<128, TOKENS>,
+                       dim3((p.tokens + TOKENS - 1) / TOKENS), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
 
 cudaError_t launch_rotary(cudaStream_t stream, int dim, const RotaryParams& p) {
-  return launch_kernel(dim == 256 ? rotary_kernel<256> : rotary_kernel<128>, dim3(p.tokens), dim3(kThreads), 0, stream, p);
+  return p.tokens >= kRotaryManyTokens ? launch<4>(stream, dim, p) : launch<1>(stream, dim, p);
 }
 
 }  // namespace tk100

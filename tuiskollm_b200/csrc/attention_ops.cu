@@ -142,7 +142,6 @@ Status PagePlanOp::release(cudaStream_t stream, PageParams p) {
   const char* what = "page release";
   TK100_TRY(check(what, p));
   p.status = ctx_.status_word();
-  p.max_tokens = p.requests;  // sets the CTA count only
   DeviceScope device(ctx_);
   TK100_TRY(device.status());
   ctx_.count_launch();

@@ -38,8 +38,9 @@ def attention_tolerance(out, size, gated=False):
     """The weights are rounded to BF16 (2^-8 of each, so 2^-8 of `size`), the result is (2^-8 of it).  Scores and
     sums are fp32: the exponent's error, up to dim * 2^-24 * sum |q k| * scale, is below 2^-11 for the normal planes
     of these tests (256 * 2^-24 * 256 * 0.64 / 16 = 1.6e-4), and ex2 and the sums add less; 2^-10 covers them.  A gated row is rounded
-    in front of its gate too: 2^-8 more of the result."""
-    return (2.0 ** -8 + 2.0 ** -10) * size + (2.0 ** -7 if gated else 2.0 ** -8) * out.abs() + 1e-30
+    to FP16 in front of its gate: 2^-11 more of the result, and 2^-25 of the row's largest value, which lies far below
+    2^-10 of `size`; a row that holds a value that is not finite to BF16, 2^-8."""
+    return (2.0 ** -8 + 2.0 ** -10) * size + (2.0 ** -8 + 2.0 ** -11 if gated else 2.0 ** -8) * out.abs() + 1e-30
 
 
 def rotate(x, positions, frequencies, pair_axes, weight=None, epsilon=1e-6):

@@ -27,6 +27,8 @@
 // tile's ticket, and the CTA that draws the last one adds the parts in order of their keys (the same
 // bits whoever is last) and stores.  The lengths stay on the device: every CTA sums the tile counts up for
 // itself, so a captured launch follows them.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
@@ -447,6 +449,16 @@ __device__ __forceinline__ const uint16_t* gate_row(const AttentionParams& p, in
 template <int D>
 __device__ __forceinline__ uint16_t* output_row(const AttentionParams& p, int token, int head, int row) {
   return p.output + (static_cast<size_t>(token + row / p.group) * p.q_heads + head * p.group + row % p.group) * D;
+}
+__device__ __forceinline__ uint32_t f32x2_to_f16x2(F32x2 v) {
+  const float2 f = f32x2_parts(v);
+  uint32_t w;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(f.y), "f"(f.x));
+  return w;
+}
+__device__ __forceinline__ F32x2 f16x2_to_f32x2(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f32x2(f.x, f.y);
 }
 // Two values times the sigmoid of their packed gates.
 __device__ __forceinline__ F32x2 gated(F32x2 v, uint32_t gate) {
@@ -1043,8 +1055,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (whole) {
         const bool blind = ahead + r / p.group < 0;  // sees no key
         const F32x2 scale2 = f32x2_splat(blind ? 0.0f : 1.0f / sum);
-        // The row as BF16, so that O is free for the next tile before gate and stores.  A gated row is rounded a second
-        // time behind its gate (2^-8 each), as where the gate is an operation of its own.
+        // The row leaves tensor memory in 16 bits a value, so that O is free for the next tile before gate and stores: as
+        // the BF16 that is stored, or in front of a gate as FP16 times a power of two that puts the row's largest value
+        // near 2^14 (2^-11 of a value where BF16 has 2^-8; values below 2^-28 of the largest lose bits).  A row with
+        // a value that is not finite is held as BF16 there too.
+        float up = 1.0f, down = 1.0f;
+        bool fp16 = false;
+        if (ok && mine && gate) {
+          float most = 0.0f;
+#pragma unroll
+          for (int k = 0; k < D / 32; k += 2) {
+            uint32_t o[64];
+            tmem_ld32(tmem_o + lanes + 32 * k, o);
+            tmem_ld32(tmem_o + lanes + 32 * k + 32, o + 32);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 64; i += 2)
+              most = fmaxf(most, fmaxf(fabsf(__uint_as_float(o[i])), fabsf(__uint_as_float(o[i + 1]))));
+          }
+          most *= fabsf(f32x2_parts(scale2).x);
+          fp16 = most > 0.0f && most < INFINITY;
+          if (fp16) {
+            const int e = min(max(141 - static_cast<int>(__float_as_uint(most) >> 23), -100), 100);  // 14 - exponent
+            up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          }
+        }
+        const F32x2 factor = mul2(scale2, f32x2_splat(up));
         uint32_t held[D / 2];
         if (ok && mine) {
 #pragma unroll
@@ -1054,7 +1091,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const uint32_t w = f32x2_to_bf16x2(mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), scale2));
+              const F32x2 v = mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), factor);
+              const uint32_t w = fp16 ? f32x2_to_f16x2(v) : f32x2_to_bf16x2(v);
               held[16 * k + i] = blind ? 0u : w;
             }
           }
@@ -1066,6 +1104,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&ctl.stats_free);
         }
         if (ok && mine) {
+          const F32x2 down2 = f32x2_splat(down);
           uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
 #pragma unroll
           for (int k = 0; k < D / 32; ++k) {
@@ -1076,10 +1115,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 uint32_t* w = held + 16 * k + 4 * e;
-                w[0] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[0]), g[e].x));
-                w[1] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[1]), g[e].y));
-                w[2] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[2]), g[e].z));
-                w[3] = f32x2_to_bf16x2(gated(bf16x2_to_f32x2(w[3]), g[e].w));
+                w[0] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[0]), down2) : bf16x2_to_f32x2(w[0]), g[e].x));
+                w[1] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[1]), down2) : bf16x2_to_f32x2(w[1]), g[e].y));
+                w[2] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[2]), down2) : bf16x2_to_f32x2(w[2]), g[e].z));
+                w[3] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[3]), down2) : bf16x2_to_f32x2(w[3]), g[e].w));
               }
             }
             if (r < rows) {

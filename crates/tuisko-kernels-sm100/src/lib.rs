@@ -404,6 +404,171 @@ impl<A: Sm100Arch> GdnRecurrenceOp<A> {
     }
 }
 
+/// A pair of paged cache planes: element (page, token, head, d) at
+/// `page * page_stride + token * token_stride + head * head_stride + d`.
+#[derive(Clone, Copy, Debug)]
+pub struct CachePlanes {
+    pub key: *mut u16,
+    pub value: *mut u16,
+    pub pages: usize,
+    pub page_tokens: usize,
+    pub page_stride: usize,
+    pub token_stride: usize,
+    pub head_stride: usize,
+}
+
+/// Block tables, slot maps and lengths of a step, built on the device (no sm_120 counterpart).
+pub struct PagePlanOp {
+    ctx: Arc<Sm100Context>,
+    page_tokens: usize,
+}
+
+impl PagePlanOp {
+    pub fn new(ctx: &Arc<Sm100Context>, page_tokens: usize) -> GpuResult<Self> {
+        Ok(Self { ctx: Arc::clone(ctx), page_tokens })
+    }
+
+    /// `tk100_page_plan`; `free` = (stack, its capacity, count, count output).
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn launch(
+        &self, stream: &CudaStream, requests: usize, request_rows: *const i32,
+        new_tokens: *const i32, lengths: *const i32, lengths_output: *mut i32,
+        block_table: (*mut i32, usize, usize), free: (*const i32, usize, *const i32, *mut i32),
+        starts: *mut i32, kv_lengths: *mut i32, positions: *mut i32, slots: *mut i64,
+        max_tokens: usize,
+    ) -> GpuResult<()> {
+        let (table, rows, pages) = block_table;
+        let (stack, capacity, count, count_output) = free;
+        self.ctx.check(unsafe {
+            ffi::tk100_page_plan(
+                self.ctx.raw, stream.cu_stream().cast(), rows_i32(requests), rows_i32(rows),
+                rows_i32(pages), rows_i32(self.page_tokens), rows_i32(max_tokens),
+                rows_i32(capacity), request_rows, new_tokens, lengths, lengths_output, table, stack,
+                count, count_output, starts, kv_lengths, positions, slots,
+            )
+        })
+    }
+
+    /// `tk100_page_release`.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn release(
+        &self, stream: &CudaStream, requests: usize, request_rows: *const i32, lengths: *const i32,
+        lengths_output: *mut i32, block_table: (*const i32, usize, usize),
+        free: (*mut i32, usize, *const i32, *mut i32),
+    ) -> GpuResult<()> {
+        let (table, rows, pages) = block_table;
+        let (stack, capacity, count, count_output) = free;
+        self.ctx.check(unsafe {
+            ffi::tk100_page_release(
+                self.ctx.raw, stream.cu_stream().cast(), rows_i32(requests), rows_i32(rows),
+                rows_i32(pages), rows_i32(self.page_tokens), rows_i32(capacity), request_rows,
+                lengths, lengths_output, table, stack, count, count_output,
+            )
+        })
+    }
+}
+
+/// Head norms, rotary positions and the stores into the cache (no sm_120 counterpart).
+pub struct RotaryCacheOp {
+    ctx: Arc<Sm100Context>,
+    heads: (usize, usize, usize),
+    rotary_dim: usize,
+    axes: usize,
+}
+
+impl RotaryCacheOp {
+    /// `heads` = (query heads, key/value heads, values per head).
+    pub fn new(
+        ctx: &Arc<Sm100Context>, heads: (usize, usize, usize), rotary_dim: usize, axes: usize,
+    ) -> GpuResult<Self> {
+        Ok(Self { ctx: Arc::clone(ctx), heads, rotary_dim, axes })
+    }
+
+    /// `tk100_rotary_cache`; each plane with its (token stride, head stride).
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn launch(
+        &self, stream: &CudaStream, tokens: usize, frequencies: *const f64, pair_axes: *const u8,
+        positions: *const i32, query: (*const u16, usize, usize), key: *const u16,
+        value: *const u16, kv_strides: (usize, usize), norms: (*const u16, *const u16),
+        query_output: *mut u16, key_output: *mut u16, cache: &CachePlanes, slots: *const i64,
+    ) -> GpuResult<()> {
+        let (q_heads, kv_heads, head_dim) = self.heads;
+        self.ctx.check(unsafe {
+            ffi::tk100_rotary_cache(
+                self.ctx.raw, stream.cu_stream().cast(), rows_i32(tokens), rows_i32(q_heads),
+                rows_i32(kv_heads), rows_i32(head_dim), rows_i32(self.rotary_dim),
+                rows_i32(self.axes), frequencies, pair_axes, positions, query.0, rows_i32(query.1),
+                rows_i32(query.2), key, value, rows_i32(kv_strides.0), rows_i32(kv_strides.1),
+                norms.0, norms.1, query_output, key_output, cache.key, cache.value,
+                rows_i32(cache.pages), rows_i32(cache.page_tokens), rows_i32(cache.page_stride),
+                rows_i32(cache.token_stride), rows_i32(cache.head_stride), slots,
+            )
+        })
+    }
+}
+
+/// Causal attention over a paged cache or over packed prompt rows (no sm_120 counterpart).
+pub struct AttentionOp {
+    ctx: Arc<Sm100Context>,
+    heads: (usize, usize, usize),
+    scale: f32,
+}
+
+impl AttentionOp {
+    /// `heads` = (query heads, key/value heads, values per head).
+    pub fn new(
+        ctx: &Arc<Sm100Context>, heads: (usize, usize, usize), scale: f32,
+    ) -> GpuResult<Self> {
+        Ok(Self { ctx: Arc::clone(ctx), heads, scale })
+    }
+
+    /// Bytes of a zeroed workspace; launches that may overlap need one each.
+    pub fn workspace_bytes(&self) -> usize {
+        unsafe { ffi::tk100_attention_workspace_bytes(self.ctx.raw, rows_i32(self.heads.2)) }
+    }
+
+    /// `tk100_paged_attention`; `query` and `gate` share the (token stride, head stride).
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn launch_paged(
+        &self, stream: &CudaStream, sequences: usize, tokens: usize, starts: *const i32,
+        kv_lengths: *const i32, query: *const u16, gate: *const u16, q_strides: (usize, usize),
+        cache: &CachePlanes, block_table: (*const i32, usize, usize), request_rows: *const i32,
+        workspace: *mut core::ffi::c_void, output: *mut u16,
+    ) -> GpuResult<()> {
+        let (q_heads, kv_heads, head_dim) = self.heads;
+        self.ctx.check(unsafe {
+            ffi::tk100_paged_attention(
+                self.ctx.raw, stream.cu_stream().cast(), rows_i32(sequences), rows_i32(tokens),
+                rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, kv_lengths,
+                query, gate, rows_i32(q_strides.0), rows_i32(q_strides.1), cache.key, cache.value,
+                rows_i32(cache.pages), rows_i32(cache.page_tokens), rows_i32(cache.page_stride),
+                rows_i32(cache.token_stride), rows_i32(cache.head_stride), block_table.0,
+                rows_i32(block_table.1), rows_i32(block_table.2), request_rows, self.scale,
+                workspace, output,
+            )
+        })
+    }
+
+    /// `tk100_prompt_attention`.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn launch_prompt(
+        &self, stream: &CudaStream, sequences: usize, tokens: usize, starts: *const i32,
+        query: *const u16, gate: *const u16, q_strides: (usize, usize), key: *const u16,
+        value: *const u16, kv_strides: (usize, usize), workspace: *mut core::ffi::c_void,
+        output: *mut u16,
+    ) -> GpuResult<()> {
+        let (q_heads, kv_heads, head_dim) = self.heads;
+        self.ctx.check(unsafe {
+            ffi::tk100_prompt_attention(
+                self.ctx.raw, stream.cu_stream().cast(), rows_i32(sequences), rows_i32(tokens),
+                rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, query, gate,
+                rows_i32(q_strides.0), rows_i32(q_strides.1), key, value, rows_i32(kv_strides.0),
+                rows_i32(kv_strides.1), self.scale, workspace, output,
+            )
+        })
+    }
+}
+
 macro_rules! fp8_mlp_op {
     ($(#[$doc:meta])* $name:ident, $entry:ident) => {
         $(#[$doc])*

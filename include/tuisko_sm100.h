@@ -539,7 +539,9 @@ TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_
  *   output[token][head] = softmax(scale * q . K) V, times sigmoid(gate[token][head]) when gate is given
  * (the queries' strides).  output is [tokens, q_heads, head_dim] and starts on 32 bytes; rows outside the sequences are left as
  * they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
- * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used. */
+ * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used,
+ * whatever it is.  A key or value of the sequence itself that is not finite reaches the tokens that see it,
+ * and through 0 * NaN may reach those up to 127 positions in front of it. */
 TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
                                              int q_heads, int kv_heads, int head_dim, const int32_t* starts,
                                              const int32_t* kv_lengths, const uint16_t* query,

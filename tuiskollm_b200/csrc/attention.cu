@@ -605,6 +605,71 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
 
 // ------------------------------------------------------------------------- the kernel
 
+// The same where there are many rows: a thread has one, 16 of its values at a time, and the loads of two parts of them
+// under way together.
+template <int D>
+__device__ __forceinline__ void join_tall(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread, int ahead,
+                                          int token, int head, const float* row_top, const float* row_scale) {
+  constexpr int QUADS = 4;
+  const int row = min(thread, rows - 1);
+  const float top = row_top[row];
+  const F32x2 scale = f32x2_splat(row_scale[row]);
+  const bool blind = ahead + row / p.group < 0;  // sees no key
+  uint16_t* out = output_row<D>(p, token, head, row);
+  const uint4* gate = p.gate ? reinterpret_cast<const uint4*>(gate_row(p, token, head, row)) : nullptr;
+#pragma unroll 1
+  for (int quad = 0; quad < D / 4; quad += QUADS) {
+    float4 acc[QUADS];
+    uint4 g[QUADS / 2];
+    if (gate) {
+#pragma unroll
+      for (int i = 0; i < QUADS / 2; ++i) g[i] = __ldg(gate + quad / 2 + i);
+    }
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int k = c0; k <= c1; k += 2) {
+      float2 stats[2];
+      float4 o[2][QUADS];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const size_t slot = part_slot(min(k + e, c1), c0, rank);
+        stats[e] = load_part(p.part_stats + slot * kRows + row);
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i)
+          o[e][i] = load_part(reinterpret_cast<const float4*>(p.parts) + slot * kRows * (D / 4) + (quad + i) * kRows + row);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // a part without a key of this row has nothing to add, whatever its O holds
+        if (k + e <= c1 && !(stats[e].x == -INFINITY && stats[e].y == 0.0f)) {
+          const float w = exp2_approx(stats[e].x - top);
+#pragma unroll
+          for (int i = 0; i < QUADS; ++i) {
+            acc[i].x = fmaf(o[e][i].x, w, acc[i].x);
+            acc[i].y = fmaf(o[e][i].y, w, acc[i].y);
+            acc[i].z = fmaf(o[e][i].z, w, acc[i].z);
+            acc[i].w = fmaf(o[e][i].w, w, acc[i].w);
+          }
+        }
+      }
+    }
+    uint32_t w[2 * QUADS];
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      F32x2 a = mul2(f32x2(acc[i].x, acc[i].y), scale), b = mul2(f32x2(acc[i].z, acc[i].w), scale);
+      if (gate) {
+        const uint4 v = g[i / 2];
+        a = gated(a, i % 2 == 0 ? v.x : v.z);
+        b = gated(b, i % 2 == 0 ? v.y : v.w);
+      }
+      w[2 * i] = blind ? 0u : f32x2_to_bf16x2(a);
+      w[2 * i + 1] = blind ? 0u : f32x2_to_bf16x2(b);
+    }
+    if (thread < rows) store_words8(out + 4 * quad, w);
+  }
+}
+
 // Barriers that both CTAs' loads or threads arrive on are the even CTA's (full, q_full, p_full, o_free); those that
 // the even CTA's MMA warp commits to are arrived on in both (empty, q_empty, s_full, pv_done, o_full).
 template <int D>
@@ -638,8 +703,13 @@ template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-constexpr int kControlRegisters = 64, kSoftmaxRegisters = 128 /* as at the start */, kEpilogueRegisters = 192;
-static_assert(kControlRegisters + 2 * kSoftmaxRegisters + kEpilogueRegisters <= 4 * 128, "the shares exceed the block's registers");
+// Heads of 256 hold 128 words of a row in the epilogue; heads of 128 half of it, and their softmax is what counts (112
+// registers there cost packed prompts 7 %, 128 cost a prompt of heads of 256 5 %).
+template <int D>
+struct Shares {
+  static constexpr int CONTROL = D == 256 ? 80 : 64, SOFTMAX = D == 256 ? 112 : 128, EPILOGUE = D == 256 ? 208 : 192;
+  static_assert(CONTROL + 2 * SOFTMAX + EPILOGUE <= 4 * 128, "the shares exceed the block's registers");
+};
 
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -696,9 +766,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Stretch& stretch = ctl.stretch;
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int v_box = PAGED ? min(kKeys, 1 << p.page_shift) : kKeys;  // keys of a box of V
+  // A box of K that has all chunks of fewer than 64 keys leaves those keys' chunks behind one another: right for an
+  // MMA when it has 8 keys, a swizzle's rows, whose distance the descriptor names.  Pages of 16 keys then take 8
+  // boxes a unit, not one per page and chunk, 16, at which the loads of a step take twice its products (512 tokens over
+  // 16000 keys).
+  const bool eights = PAGED && attention_eights(D, p.page_shift);
 
   if (warp < 4) {
-    fewer_registers<kControlRegisters>();
+    fewer_registers<Shares<D>::CONTROL>();
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
     int stage = 0;
@@ -716,10 +791,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (all chunks where no page ends inside the
     // 64 keys), V boxes of `v_box` keys and half of the chunks.  What does not change from step to step:
     const int shift = p.page_shift;
-    const int k_box = PAGED ? min(S::K_KEYS, 1 << shift) : S::K_KEYS;
-    const bool all = k_box == S::K_KEYS;
+    const int k_box = eights ? 8 : PAGED ? min(S::K_KEYS, 1 << shift) : S::K_KEYS;
+    const bool all = eights || k_box == S::K_KEYS;
     const int k_key = (all ? lane : lane / S::CHUNKS) * k_box, k_chunk = all ? 0 : lane % S::CHUNKS, v_key = lane * v_box;
-    uint8_t* const k_to = ring + k_chunk * (S::K_KEYS * 128) + k_key * 128;
+    uint8_t* const k_to = ring + k_chunk * (S::K_KEYS * 128) + k_key * (eights ? 2 * D : 128);
     uint8_t* const v_to = ring + v_key * S::V_CHUNKS * 128;
     const int within_page = PAGED ? (1 << shift) - 1 : -1;
     // page of key `key` of the sequence in table row `row`; outside the planes -1, where TMA fills zeros
@@ -862,11 +937,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status);
       if (!ok) return;
       if (elect_one()) {
-        const uint64_t a = umma_desc_sw128(q_addr), b = umma_desc_sw128(ring_addr + stage * S::UNIT);
+        const uint64_t a = umma_desc_sw128(q_addr);
+        const uint64_t b = umma_desc_sw128(ring_addr + stage * S::UNIT, eights ? 16 * D : 1024);
+        const uint32_t chunk = (eights ? 1024 : S::K_KEYS * 128) >> 4;
 #pragma unroll
         for (int k = 0; k < 4 * S::CHUNKS; ++k) {
           umma_bf16_pair(tmem + buffer * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3),
-                         b + (k >> 2) * (S::K_KEYS * 128 >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                         b + (k >> 2) * chunk + 2 * (k & 3), idesc_s, k > 0);
         }
         umma_commit_pair(&ctl.empty[stage]);
         umma_commit_pair(&ctl.s_full[buffer]);
@@ -941,6 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else if (warp < 12) {
     // ----------------------------------------------------------------- softmax
+    if constexpr (Shares<D>::SOFTMAX < 128) fewer_registers<Shares<D>::SOFTMAX>();
     const int group = (warp >> 2) - 1;  // has the steps of its parity, and S buffer `group`
     const int quadrant = warp & 3;      // the TMEM lanes this warp may touch
     const int r = quadrant * 32 + lane;
@@ -1027,7 +1105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    more_registers<kEpilogueRegisters>();
+    more_registers<Shares<D>::EPILOGUE>();
     const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 384;
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
@@ -1167,7 +1245,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             join_stats<8>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
           }
-          if (c1 - c0 < 2) {
+          if (rows > 48) {
+            join_tall<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
+          } else if (c1 - c0 < 2) {
             join_rows<D, 4, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           } else {
             join_rows<D, 3, 5>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);

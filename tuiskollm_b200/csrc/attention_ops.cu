@@ -281,13 +281,14 @@ Status AttentionOp::launch(cudaStream_t stream, const char* what, int head_dim, 
 // 64 keys lie next to each other in shared memory); values in boxes of up to 128 tokens x half of a head.
 Status AttentionOp::kv_map(const uint16_t* plane, int head_dim, int kv_heads, const CacheGeometry& g, int most_rows,
                            bool keys, CUtensorMap* out) {
-  const int rows = std::min(most_rows, keys ? 64 : 128);
+  const bool eights = keys && most_rows == g.page_tokens && attention_eights(head_dim, log2_of(g.page_tokens));
+  const int rows = eights ? 8 : std::min(most_rows, keys ? 64 : 128);
   const uint64_t dims[5] = {64u, static_cast<uint64_t>(g.page_tokens), static_cast<uint64_t>(head_dim / 64),
                             static_cast<uint64_t>(kv_heads), static_cast<uint64_t>(g.pages)};
   const uint64_t strides[4] = {static_cast<uint64_t>(g.token_stride), 64u, static_cast<uint64_t>(g.head_stride),
                                static_cast<uint64_t>(g.page_stride)};
   const uint32_t box[5] = {64u, static_cast<uint32_t>(rows),
-                           static_cast<uint32_t>(!keys ? head_dim / 128 : rows < 64 ? 1 : head_dim / 64), 1u, 1u};
+                           static_cast<uint32_t>(!keys ? head_dim / 128 : rows < 64 && !eights ? 1 : head_dim / 64), 1u, 1u};
   return ctx_.bf16_map(plane, 5, dims, strides, box, out);
 }
 

@@ -451,6 +451,8 @@ struct AttentionParams {
   unsigned int* tickets;
   uint32_t* status;
 };
+// Whether boxes of the key map have 8 keys and all chunks.
+__host__ __device__ constexpr bool attention_eights(int dim, int page_shift) { return dim == 256 && page_shift == 4; }
 cudaError_t attention_prepare();
 cudaError_t launch_attention(cudaStream_t stream, int dim, int pairs, const CUtensorMap& map_q, const CUtensorMap& map_q1,
                              const CUtensorMap& map_k, const CUtensorMap& map_v, const AttentionParams& p);

@@ -576,13 +576,13 @@ __device__ __forceinline__ void tmem_cp_32x128b_warpx4_pair(uint32_t tmem_dst, u
 
 // Shared-memory matrix descriptor for a K-major operand stored as rows of 128 bytes
 // with the 128-byte swizzle (what a TMA box of 128 bytes x R rows writes): groups of
-// 8 rows are 1024 bytes apart; the tile base must be 1024-byte aligned.  Stepping
+// 8 rows are 1024 bytes apart (or `group_bytes`); the tile base must be 1024-byte aligned.  Stepping
 // along K inside the 128-byte row is done by adding the byte offset to `addr`.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t group_bytes = 1024) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);  // start address [0,14)
   d |= static_cast<uint64_t>(1) << 16;                      // leading byte offset (unused) [16,30)
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;              // stride byte offset [32,46)
+  d |= static_cast<uint64_t>(group_bytes >> 4) << 32;       // stride byte offset [32,46)
   d |= static_cast<uint64_t>(1) << 46;                      // descriptor version (sm_100)
   d |= static_cast<uint64_t>(2) << 61;                      // layout: 128-byte swizzle
   return d;

@@ -134,3 +134,23 @@ def test_tensors_and_streams(recorder):
         ops._launch("tk100_rms_norm", types.SimpleNamespace(_lib=_lib.load(), handle=None, check=None), side, 1,
                     x[:, ::2], x, x)
     assert info.value.code == "gpu.launch"
+
+
+@pytest.mark.gpu
+def test_plane_readers():
+    """`plane` and `heads` take what fits and leave the rest, which the operators refuse in words, to them."""
+    native = _lib.native(ops._launch)
+    t = torch.zeros(6, 4, 128, dtype=torch.bfloat16, device="cuda")
+    assert native.plane(t, torch.bfloat16, 0, 6 * 4 * 128) == t.data_ptr()
+    for other in [(t, torch.float16, 0, 1), (t, torch.bfloat16, 1, 1), (t, torch.bfloat16, 0, 6 * 4 * 128 + 1),
+                  (t[:, ::2], torch.bfloat16, 0, 1), (t.cpu(), torch.bfloat16, 0, 1), (7, torch.bfloat16, 0, 1)]:
+        assert native.plane(*other) is None
+    assert native.heads(t, 0, -1, 4, 128) == (t.data_ptr(), (512, 128, 1), 6)
+    assert native.heads(t[2:, 1:3], 0, 4, 2, 128) == (t[2:, 1:3].data_ptr(), (512, 128, 1), 4)
+    # one row, one head: the strides of a dense plane, whatever the tensor says
+    assert native.heads(t[:1, ::3][:, :1], 0, -1, 1, 128) == (t.data_ptr(), (128, 128, 1), 1)
+    for other in [(t, 1, -1, 4, 128), (t, 0, -1, 4), (t, 0, 5, 4, 128), (t.float(), 0, -1, 4, 128), (t[..., ::2], 0, -1, 4, 64),
+                  (t.cpu(), 0, -1, 4, 128), (None, 0, -1, 4, 128)]:
+        assert native.heads(*other) is None
+    # a broadcast plane has no dense heads
+    assert native.heads(torch.zeros(1, dtype=torch.bfloat16, device="cuda").expand(2, 4, 128), 0, -1, 4, 128) is None

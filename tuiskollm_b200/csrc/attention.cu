@@ -4,29 +4,41 @@
 //     o_i = sum_j softmax_j(scale * q_i . k_j) v_j,   optionally times sigmoid(gate_i);
 // a token that sees nothing (k - q + i < 0) gets zeros.
 //
-// Tiles.  The G query heads that share a key/value head are rows of one tile: row r = token r / G, head
-// r % G, floor(128 / G) whole tokens, so a decoded token's heads read the cache once and a prompt's diagonal
-// tile wastes 128 / G keys instead of 128.  A tile walks over its keys 128 at a time:
+// Tiles.  Two CTAs of a cluster are one MMA unit of 256 rows (cta_group::2).  The G query heads that share a key/value
+// head are rows of one tile: a CTA has floor(128 / G) whole tokens, row r = token r / G, head r % G, so a decoded
+// token's heads read the cache once, and the keys that a prompt's diagonal tile computes in vain are 256 / G, not 256.
+// A tile walks over its keys 128 at a time:
 //     S = Q K^T (tcgen05, both from shared memory) -> TMEM, two buffers
 //     P = exp2(scale log2e (S - m)) -> BF16 into the first half of S's columns
 //     O += P V (tcgen05, P from TMEM, V from shared memory) -> TMEM
 // m is the row's reference maximum: it follows the running maximum only when that has grown by more than 2^8,
 // so O is rescaled in TMEM a few times per row, not per tile, and P stays below 2^8, where BF16 and the
-// fp32 sum of P lose nothing.  P is rounded to BF16 (half a step 2^-9 each, the tensor core's operand type);
-// sums, maxima, O and the join of split rows are fp32.
+// fp32 sum of P lose nothing.  P is rounded to BF16 (2^-8 of each, the tensor core's operand type); sums,
+// maxima, O and the join of split rows are fp32.
+// Each CTA brings half of the keys of K and half of the values of V, so a step costs its shared memory 64 KB written
+// and 128 KB read by the MMAs at heads of 256; one CTA by itself moves 320 KB a step and took 3800 cycles where the
+// MMAs take 2048 (prompt of 8192 tokens 1649 -> 1232 us with the pair).
 //
-// Roles, ten warps: TMA producer; MMA issuer; four softmax warps (thread = row); four epilogue warps, which
-// read O, normalise, gate and store while the softmax warps are on the next tile.  S of tile j + 1 is issued
-// before P V of tile j, so that the tensor pipe works during the softmax of j.  K arrives in units of 128 keys x
-// 64 values and V in units of 8192 values (32 or 64 keys), 16 KB each, one ring for both; a unit is read where
-// the page of the block table says, page by page.
+// Roles, sixteen warps: TMA producer (each lane asks for a box: one elected lane needed 500 cycles a unit); MMA issuer
+// in the even CTA, one step of scores ahead of the values so that the tensor pipe works during the softmax;
+// two softmax warpgroups (thread = row) that take the steps in turn and hand on the rows' references, so that one
+// step's exponentials run beside the other's loads and maxima; four epilogue warps, which normalise, gate and store
+// while the others are on the next tile.  K and V share a ring of four (heads of 128: seven) units; a unit is
+// read where the block table says, page by page.
 //
-// Work split.  All tiles of a launch in order (sequence, key/value head, tile) form one line of 128-key
-// steps, and each CTA (one per SM) takes an equal stretch of the line, wherever tiles begin and end.  A tile
-// whose steps lie in several CTAs is joined: each leaves its fp32 O, m and sum in the workspace, takes the
-// tile's ticket, and the CTA that draws the last one adds the parts in order of their keys (the same
-// bits whoever is last) and stores.  The lengths stay on the device: every CTA sums the tile counts up for
-// itself, so a captured launch follows them.
+// Work split.  All tiles of a launch in order (sequence, key/value head, tile) form one line of keys, and each pair
+// takes an equal stretch of it, wherever tiles begin and end, but for cuts near a tile's end, which move there.  A
+// tile that several pairs have is joined: each leaves its fp32 O, m and sum in the workspace, takes the tile's
+// ticket, and the CTA that draws the last one adds the parts in order of their keys (the same bits whoever is last)
+// and stores.  Pairs begin with such tiles, so that joins run beside whole ones.  The lengths stay on the device:
+// every CTA sums the costs up for itself, in closed form, so a captured launch follows them.
+//
+// Measured (B200 at 1.65 to 1.9 GHz), us: prompt of 8192 tokens, 24 heads over 4 of 256, gated, 701 (1.18 PFLOP/s,
+// 0.70 of cuBLAS' BF16 burst rate); seven packed prompts of up to 1777, 32 over 8 of 128, 114; decode batch of 32
+// over up to 16384 keys 203 (855 MB: 0.64 of the copy rate); 512 tokens over 16000 keys 219; one token over
+// 4096 keys 24.8.  A step takes 2400 cycles at heads of 256, where the MMAs take 2048, and 1600 at 128 (1024, of
+// which the exponentials take 1024 too): the chain scores -> softmax -> values of a step, with one buffer of S per
+// warpgroup, bounds both.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -774,248 +786,248 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     fewer_registers<Shares<D>::CONTROL>();
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    int stage = 0;
-    uint32_t phase = 1;  // parity to wait for on `empty`: a fresh barrier's earlier phase
-    bool ok = true;
-    int items = 0;
-    auto advance = [&]() {
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1;
-      }
-    };
-    const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0), q_full_even = mapa_u32(smem_u32(&ctl.q_full), 0);
-    const uint32_t tail_mine = mapa_u32(smem_u32(&ctl.tail_full[0]), static_cast<uint32_t>(rank));
-    // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (all chunks where no page ends inside the
-    // 64 keys), V boxes of `v_box` keys and half of the chunks.  What does not change from step to step:
-    const int shift = p.page_shift;
-    const int k_box = eights ? 8 : PAGED ? min(S::K_KEYS, 1 << shift) : S::K_KEYS;
-    const bool all = eights || k_box == S::K_KEYS;
-    const int k_key = (all ? lane : lane / S::CHUNKS) * k_box, k_chunk = all ? 0 : lane % S::CHUNKS, v_key = lane * v_box;
-    uint8_t* const k_to = ring + k_chunk * (S::K_KEYS * 128) + k_key * (eights ? 2 * D : 128);
-    uint8_t* const v_to = ring + v_key * S::V_CHUNKS * 128;
-    const int within_page = PAGED ? (1 << shift) - 1 : -1;
-    // page of key `key` of the sequence in table row `row`; outside the planes -1, where TMA fills zeros
-    auto page_of = [&](int row, int key, bool needed) -> int {
-      if (!PAGED) return 0;
-      int id = -1;
-      if (needed) {
-        const int index = key >> shift;
-        if (row >= 0 && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
-        if (id < 0 || id >= p.pages) {
-          id = -1;
-          atomicOr(p.status, STATUS_BAD_ARGUMENT);
+    if (warp == 0) {
+      // ---------------------------------------------------------------- producer
+      int stage = 0;
+      uint32_t phase = 1;  // parity to wait for on `empty`: a fresh barrier's earlier phase
+      bool ok = true;
+      int items = 0;
+      auto advance = [&]() {
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
         }
-      }
-      return id;
-    };
-    struct Fetch {  // a step: its first key (as a coordinate for packed rows), how many of its keys count, pages
-      int base, keys, head, k_page, v_page;
-    };
-    auto fetch_of = [&](const Steps& at, int row) -> Fetch {
-      Fetch f;
-      const int first = at.j * kKeys, k = rank * S::K_KEYS + k_key;
-      f.keys = min(at.it.limit - first, kKeys);
-      f.head = at.it.head;
-      f.base = PAGED ? first : at.it.seq.start + first;
-      f.k_page = page_of(row, first + k, k_key < S::K_KEYS && k < f.keys);
-      f.v_page = page_of(row, first + v_key, v_key < f.keys);
-      return f;
-    };
-    // keys of CTA r's half of K that boxes fetch
-    auto k_fetched = [&](int keys, int r) { return (min(max(keys - r * S::K_KEYS, 0), S::K_KEYS) + k_box - 1) & ~(k_box - 1); };
-    Steps now(p, stretch);
-    int row = 0;
-    Fetch fetch{}, earlier{};
-    bool more = now.next(p), loaded = false;
-    auto open = [&]() {
-      if (PAGED) {
-        row = p.table_rows ? p.table_rows[now.it.sequence] : now.it.sequence;
-        if (row >= p.table_row_count) row = -1;
-      }
-    };
-    if (more) {
-      open();
-      fetch = fetch_of(now, row);
-    }
-    // K of a step, then V of the step before it: the order in which the MMA warp asks for them
-    while (ok && (more || loaded)) {
+      };
+      const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0), q_full_even = mapa_u32(smem_u32(&ctl.q_full), 0);
+      const uint32_t tail_mine = mapa_u32(smem_u32(&ctl.tail_full[0]), static_cast<uint32_t>(rank));
+      // Boxes of a unit, one per lane: K boxes of `k_box` keys and one chunk (all chunks where no page ends inside the
+      // 64 keys), V boxes of `v_box` keys and half of the chunks.  What does not change from step to step:
+      const int shift = p.page_shift;
+      const int k_box = eights ? 8 : PAGED ? min(S::K_KEYS, 1 << shift) : S::K_KEYS;
+      const bool all = eights || k_box == S::K_KEYS;
+      const int k_key = (all ? lane : lane / S::CHUNKS) * k_box, k_chunk = all ? 0 : lane % S::CHUNKS, v_key = lane * v_box;
+      uint8_t* const k_to = ring + k_chunk * (S::K_KEYS * 128) + k_key * (eights ? 2 * D : 128);
+      uint8_t* const v_to = ring + v_key * S::V_CHUNKS * 128;
+      const int within_page = PAGED ? (1 << shift) - 1 : -1;
+      // page of key `key` of the sequence in table row `row`; outside the planes -1, where TMA fills zeros
+      auto page_of = [&](int row, int key, bool needed) -> int {
+        if (!PAGED) return 0;
+        int id = -1;
+        if (needed) {
+          const int index = key >> shift;
+          if (row >= 0 && index < p.max_pages) id = p.block_table[static_cast<size_t>(row) * p.max_pages + index];
+          if (id < 0 || id >= p.pages) {
+            id = -1;
+            atomicOr(p.status, STATUS_BAD_ARGUMENT);
+          }
+        }
+        return id;
+      };
+      struct Fetch {  // a step: its first key (as a coordinate for packed rows), how many of its keys count, pages
+        int base, keys, head, k_page, v_page;
+      };
+      auto fetch_of = [&](const Steps& at, int row) -> Fetch {
+        Fetch f;
+        const int first = at.j * kKeys, k = rank * S::K_KEYS + k_key;
+        f.keys = min(at.it.limit - first, kKeys);
+        f.head = at.it.head;
+        f.base = PAGED ? first : at.it.seq.start + first;
+        f.k_page = page_of(row, first + k, k_key < S::K_KEYS && k < f.keys);
+        f.v_page = page_of(row, first + v_key, v_key < f.keys);
+        return f;
+      };
+      // keys of CTA r's half of K that boxes fetch
+      auto k_fetched = [&](int keys, int r) { return (min(max(keys - r * S::K_KEYS, 0), S::K_KEYS) + k_box - 1) & ~(k_box - 1); };
+      Steps now(p, stretch);
+      int row = 0;
+      Fetch fetch{}, earlier{};
+      bool more = now.next(p), loaded = false;
+      auto open = [&]() {
+        if (PAGED) {
+          row = p.table_rows ? p.table_rows[now.it.sequence] : now.it.sequence;
+          if (row >= p.table_row_count) row = -1;
+        }
+      };
       if (more) {
-        if (now.opens()) {
-          const Item& it = now.it;
-          if (now.item > 0) ok = warp_wait(&ctl.q_empty, (now.item - 1) & 1, p.status);
-          if (!ok) break;
-          const int mine = min(it.tokens - rank * p.half_tokens, p.half_tokens);  // tokens of this CTA's rows
-          if (rank == 0 && lane == 0) {
-            const int other = min(max(it.tokens - p.half_tokens, 0), p.half_tokens);
-            const int tokens = (mine == 1 ? 1 : p.half_tokens) + (other <= 1 ? other : p.half_tokens);
-            mbar_arrive_expect_tx(&ctl.q_full, static_cast<uint32_t>(p.group * tokens * 128 * S::CHUNKS));
-          }
-          if (lane < S::CHUNKS && mine > 0) {
-            tma_load_4d_pair(smem_q + lane * kRows * 128, mine == 1 ? &map_q1 : &map_q, q_full_even, 64 * lane, 0, it.head,
-                             it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens);
-          }
-          __syncwarp();
-          ++items;
-        }
-        ok = warp_wait(&ctl.empty[stage], phase, p.status);
-        if (!ok) break;
-        if (lane == 0) {
-          if (rank == 0) {
-            mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>((k_fetched(fetch.keys, 0) + k_fetched(fetch.keys, 1)) * 2 * D));
-          } else {
-            mbar_arrive_remote_light(full_even + stage * 8);
-          }
-        }
-        if (k_key < k_fetched(fetch.keys, rank))
-          tma_load_5d_pair(k_to + stage * S::UNIT, &map_k, full_even + stage * 8, 0,
-                           (fetch.base + rank * S::K_KEYS + k_key) & within_page, k_chunk, fetch.head, fetch.k_page);
-        __syncwarp();
-        advance();
+        open();
+        fetch = fetch_of(now, row);
       }
-      if (loaded) {
-        ok = warp_wait(&ctl.empty[stage], phase, p.status);
-        if (!ok) break;
-        const int fetched = (max(earlier.keys, 0) + v_box - 1) & ~(v_box - 1);
-        const bool tail = ragged(earlier.keys);  // goes to this CTA's own barrier, `full` is arrived on behind the zeros
-        if (lane == 0) {
-          if (tail) {
-            mbar_arrive_expect_tx(&ctl.tail_full[stage], static_cast<uint32_t>(fetched * D));
-          } else if (rank == 0) {
-            mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>(fetched * 2 * D));
-          } else {
-            mbar_arrive_remote_light(full_even + stage * 8);
-          }
-        }
-        if (v_key < fetched)
-          tma_load_5d_pair(v_to + stage * S::UNIT, &map_v, (tail ? tail_mine : full_even) + stage * 8, 0,
-                           (earlier.base + v_key) & within_page, rank * S::V_CHUNKS, earlier.head, earlier.v_page);
-        __syncwarp();
-        advance();
-      }
-      loaded = more;
-      if (more) {
-        earlier = fetch;
-        more = now.next(p);
+      // K of a step, then V of the step before it: the order in which the MMA warp asks for them
+      while (ok && (more || loaded)) {
         if (more) {
-          if (now.opens()) open();
-          fetch = fetch_of(now, row);
+          if (now.opens()) {
+            const Item& it = now.it;
+            if (now.item > 0) ok = warp_wait(&ctl.q_empty, (now.item - 1) & 1, p.status);
+            if (!ok) break;
+            const int mine = min(it.tokens - rank * p.half_tokens, p.half_tokens);  // tokens of this CTA's rows
+            if (rank == 0 && lane == 0) {
+              const int other = min(max(it.tokens - p.half_tokens, 0), p.half_tokens);
+              const int tokens = (mine == 1 ? 1 : p.half_tokens) + (other <= 1 ? other : p.half_tokens);
+              mbar_arrive_expect_tx(&ctl.q_full, static_cast<uint32_t>(p.group * tokens * 128 * S::CHUNKS));
+            }
+            if (lane < S::CHUNKS && mine > 0) {
+              tma_load_4d_pair(smem_q + lane * kRows * 128, mine == 1 ? &map_q1 : &map_q, q_full_even, 64 * lane, 0, it.head,
+                               it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens);
+            }
+            __syncwarp();
+            ++items;
+          }
+          ok = warp_wait(&ctl.empty[stage], phase, p.status);
+          if (!ok) break;
+          if (lane == 0) {
+            if (rank == 0) {
+              mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>((k_fetched(fetch.keys, 0) + k_fetched(fetch.keys, 1)) * 2 * D));
+            } else {
+              mbar_arrive_remote_light(full_even + stage * 8);
+            }
+          }
+          if (k_key < k_fetched(fetch.keys, rank))
+            tma_load_5d_pair(k_to + stage * S::UNIT, &map_k, full_even + stage * 8, 0,
+                             (fetch.base + rank * S::K_KEYS + k_key) & within_page, k_chunk, fetch.head, fetch.k_page);
+          __syncwarp();
+          advance();
+        }
+        if (loaded) {
+          ok = warp_wait(&ctl.empty[stage], phase, p.status);
+          if (!ok) break;
+          const int fetched = (max(earlier.keys, 0) + v_box - 1) & ~(v_box - 1);
+          const bool tail = ragged(earlier.keys);  // goes to this CTA's own barrier, `full` is arrived on behind the zeros
+          if (lane == 0) {
+            if (tail) {
+              mbar_arrive_expect_tx(&ctl.tail_full[stage], static_cast<uint32_t>(fetched * D));
+            } else if (rank == 0) {
+              mbar_arrive_expect_tx(&ctl.full[stage], static_cast<uint32_t>(fetched * 2 * D));
+            } else {
+              mbar_arrive_remote_light(full_even + stage * 8);
+            }
+          }
+          if (v_key < fetched)
+            tma_load_5d_pair(v_to + stage * S::UNIT, &map_v, (tail ? tail_mine : full_even) + stage * 8, 0,
+                             (earlier.base + v_key) & within_page, rank * S::V_CHUNKS, earlier.head, earlier.v_page);
+          __syncwarp();
+          advance();
+        }
+        loaded = more;
+        if (more) {
+          earlier = fetch;
+          more = now.next(p);
+          if (more) {
+            if (now.opens()) open();
+            fetch = fetch_of(now, row);
+          }
         }
       }
-    }
-    if (!ok) {
-      // what was asked for lands before a CTA's shared memory is somebody else's; both leave together
-      for (int n = 0; rank == 0 && items > 0 && n < 200000 && !mbar_try_wait(&ctl.q_full, (items - 1) & 1); ++n) {
+      if (!ok) {
+        // what was asked for lands before a CTA's shared memory is somebody else's; both leave together
+        for (int n = 0; rank == 0 && items > 0 && n < 200000 && !mbar_try_wait(&ctl.q_full, (items - 1) & 1); ++n) {
+        }
+        for (int i = 0; i < STAGES; ++i) {
+          for (int n = 0; rank == 0 && n < 200000 && !mbar_try_wait(&ctl.full[stage], phase); ++n) {
+          }
+          advance();
+        }
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // what counts on other barriers
       }
-      for (int i = 0; i < STAGES; ++i) {
-        for (int n = 0; rank == 0 && n < 200000 && !mbar_try_wait(&ctl.full[stage], phase); ++n) {
+    } else if (warp == 1 && rank == 0) {
+      // ------------------------------------------------------------------- MMA
+      constexpr uint32_t idesc_s = umma_idesc_bf16(2 * kRows, kKeys, false);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(2 * kRows, D, true);
+      int stage = 0, n = 0;  // n: steps so far
+      uint32_t phase = 0, tail_phase = 0;
+      bool ok = true;
+      auto advance = [&]() {
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      };
+      const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
+      Steps next(p, stretch);
+      // S[buffer] = Q K^T of step `next`
+      auto scores = [&](int buffer) {
+        if (next.opens()) ok = warp_wait(&ctl.q_full, next.item & 1, p.status);
+        ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status);
+        if (!ok) return;
+        if (elect_one()) {
+          const uint64_t a = umma_desc_sw128(q_addr);
+          const uint64_t b = umma_desc_sw128(ring_addr + stage * S::UNIT, eights ? 16 * D : 1024);
+          const uint32_t chunk = (eights ? 1024 : S::K_KEYS * 128) >> 4;
+#pragma unroll
+          for (int k = 0; k < 4 * S::CHUNKS; ++k) {
+            umma_bf16_pair(tmem + buffer * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3),
+                           b + (k >> 2) * chunk + 2 * (k & 3), idesc_s, k > 0);
+          }
+          umma_commit_pair(&ctl.empty[stage]);
+          umma_commit_pair(&ctl.s_full[buffer]);
+          if (next.closes()) umma_commit_pair(&ctl.q_empty);
+        }
+        __syncwarp();
+        advance();
+      };
+      bool more = next.next(p);
+      if (more) scores(0);
+      while (ok && more) {
+        const int buffer = n & 1, keys = next.it.limit - next.j * kKeys, item = next.item;
+        const bool opens = next.opens(), closes = next.closes();
+        more = next.next(p);
+        if (more) scores(buffer ^ 1);
+        if (!ok) break;
+        if (ragged(keys)) {
+          // P is zero for the keys behind the last, but what lies there may be no number
+          ok = warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status);
+          if (!ok) break;
+          tail_phase ^= 1u << stage;
+          zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
+          if (lane == 0) mbar_arrive(&ctl.full[stage]);
+        }
+        if (opens && item > 0) ok = warp_wait_cluster(&ctl.o_free, (item - 1) & 1, p.status);
+        ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status) && warp_wait_cluster(&ctl.p_full[buffer], (n >> 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * S::UNIT, v_box * 128);
+          const int slices = keys <= 0 ? 1 : min((keys + 15) / 16, kKeys / 16);
+          for (int k = 0; k < slices; ++k) {
+            const uint32_t r = 16 * k;  // box r / v_box of [chunk][v_box keys][128 bytes]
+            const uint32_t offset = (r & ~(v_box - 1u)) * S::V_CHUNKS * 128 + (r & (v_box - 1u)) * 128;
+            umma_bf16_ta_pair(tmem_o, tmem + buffer * kKeys + 8 * k, b + (offset >> 4), idesc_o, !opens || k > 0);
+          }
+          umma_commit_pair(&ctl.empty[stage]);
+          umma_commit_pair(&ctl.pv_done);
+          if (closes) umma_commit_pair(&ctl.o_full);
+        }
+        __syncwarp();
+        advance();
+        ++n;
+      }
+      if (!ok) {
+        if (elect_one()) umma_commit_pair(&ctl.drained);
+        __syncwarp();
+        for (int i = 0; i < 200000 && !mbar_try_wait(&ctl.drained, 0); ++i) {
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------- zeros behind the odd CTA's last keys
+      const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0);
+      uint32_t tail_phase = 0;
+      int stage = 0;
+      auto advance = [&]() { stage = stage + 1 == STAGES ? 0 : stage + 1; };
+      Steps next(p, stretch);
+      bool more = next.next(p);
+      if (more) advance();
+      while (more) {
+        const int keys = next.it.limit - next.j * kKeys;
+        more = next.next(p);
+        if (more) advance();
+        if (ragged(keys)) {
+          if (!warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status)) break;
+          tail_phase ^= 1u << stage;
+          zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
+          if (lane == 0) mbar_arrive_remote(full_even + stage * 8);
         }
         advance();
       }
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);  // what counts on other barriers
     }
-  } else if (warp == 1 && rank == 0) {
-    // ------------------------------------------------------------------- MMA
-    constexpr uint32_t idesc_s = umma_idesc_bf16(2 * kRows, kKeys, false);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(2 * kRows, D, true);
-    int stage = 0, n = 0;  // n: steps so far
-    uint32_t phase = 0, tail_phase = 0;
-    bool ok = true;
-    auto advance = [&]() {
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1;
-      }
-    };
-    const uint32_t q_addr = smem_u32(smem_q), ring_addr = smem_u32(ring);
-    Steps next(p, stretch);
-    // S[buffer] = Q K^T of step `next`
-    auto scores = [&](int buffer) {
-      if (next.opens()) ok = warp_wait(&ctl.q_full, next.item & 1, p.status);
-      ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status);
-      if (!ok) return;
-      if (elect_one()) {
-        const uint64_t a = umma_desc_sw128(q_addr);
-        const uint64_t b = umma_desc_sw128(ring_addr + stage * S::UNIT, eights ? 16 * D : 1024);
-        const uint32_t chunk = (eights ? 1024 : S::K_KEYS * 128) >> 4;
-#pragma unroll
-        for (int k = 0; k < 4 * S::CHUNKS; ++k) {
-          umma_bf16_pair(tmem + buffer * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3),
-                         b + (k >> 2) * chunk + 2 * (k & 3), idesc_s, k > 0);
-        }
-        umma_commit_pair(&ctl.empty[stage]);
-        umma_commit_pair(&ctl.s_full[buffer]);
-        if (next.closes()) umma_commit_pair(&ctl.q_empty);
-      }
-      __syncwarp();
-      advance();
-    };
-    bool more = next.next(p);
-    if (more) scores(0);
-    while (ok && more) {
-      const int buffer = n & 1, keys = next.it.limit - next.j * kKeys, item = next.item;
-      const bool opens = next.opens(), closes = next.closes();
-      more = next.next(p);
-      if (more) scores(buffer ^ 1);
-      if (!ok) break;
-      if (ragged(keys)) {
-        // P is zero for the keys behind the last, but what lies there may be no number
-        ok = warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status);
-        if (!ok) break;
-        tail_phase ^= 1u << stage;
-        zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
-        if (lane == 0) mbar_arrive(&ctl.full[stage]);
-      }
-      if (opens && item > 0) ok = warp_wait_cluster(&ctl.o_free, (item - 1) & 1, p.status);
-      ok = ok && warp_wait_cluster(&ctl.full[stage], phase, p.status) && warp_wait_cluster(&ctl.p_full[buffer], (n >> 1) & 1, p.status);
-      if (!ok) break;
-      tc_fence_after_sync();
-      if (elect_one()) {
-        const uint64_t b = umma_desc_sw128_mn(ring_addr + stage * S::UNIT, v_box * 128);
-        const int slices = keys <= 0 ? 1 : min((keys + 15) / 16, kKeys / 16);
-        for (int k = 0; k < slices; ++k) {
-          const uint32_t r = 16 * k;  // box r / v_box of [chunk][v_box keys][128 bytes]
-          const uint32_t offset = (r & ~(v_box - 1u)) * S::V_CHUNKS * 128 + (r & (v_box - 1u)) * 128;
-          umma_bf16_ta_pair(tmem_o, tmem + buffer * kKeys + 8 * k, b + (offset >> 4), idesc_o, !opens || k > 0);
-        }
-        umma_commit_pair(&ctl.empty[stage]);
-        umma_commit_pair(&ctl.pv_done);
-        if (closes) umma_commit_pair(&ctl.o_full);
-      }
-      __syncwarp();
-      advance();
-      ++n;
-    }
-    if (!ok) {
-      if (elect_one()) umma_commit_pair(&ctl.drained);
-      __syncwarp();
-      for (int i = 0; i < 200000 && !mbar_try_wait(&ctl.drained, 0); ++i) {
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------- zeros behind the odd CTA's last keys
-    const uint32_t full_even = mapa_u32(smem_u32(&ctl.full[0]), 0);
-    uint32_t tail_phase = 0;
-    int stage = 0;
-    auto advance = [&]() { stage = stage + 1 == STAGES ? 0 : stage + 1; };
-    Steps next(p, stretch);
-    bool more = next.next(p);
-    if (more) advance();
-    while (more) {
-      const int keys = next.it.limit - next.j * kKeys;
-      more = next.next(p);
-      if (more) advance();
-      if (ragged(keys)) {
-        if (!warp_wait(&ctl.tail_full[stage], (tail_phase >> stage) & 1, p.status)) break;
-        tail_phase ^= 1u << stage;
-        zero_behind<D>(ring + stage * S::UNIT, keys, v_box, lane);
-        if (lane == 0) mbar_arrive_remote(full_even + stage * 8);
-      }
-      advance();
-    }
-  }
   } else if (warp < 12) {
     // ----------------------------------------------------------------- softmax
     if constexpr (Shares<D>::SOFTMAX < 128) fewer_registers<Shares<D>::SOFTMAX>();

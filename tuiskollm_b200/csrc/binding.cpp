@@ -238,6 +238,10 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
         long long dense = 1;
         for (Py_ssize_t i = dims - 1; i >= 0; --i) {
           const long long stride = t.size(i) == 1 ? dense : static_cast<long long>(t.stride(i));
+          if (stride > 0x7fffffffll) {  // the C side takes ints
+            Py_DECREF(strides);
+            Py_RETURN_NONE;
+          }
           dense = stride * static_cast<long long>(t.size(i));
           PyObject* value = PyLong_FromLongLong(stride);
           if (!value) {

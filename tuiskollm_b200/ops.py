@@ -402,6 +402,8 @@ def _heads(context: Context, t, name, *shape):
     strides = tuple(reversed(strides))
     if strides[-1] != 1:
         raise GpuError(5, f"[gpu.launch] {name}: the values of a head are not next to each other")
+    if max(strides) > 0x7fffffff:
+        raise GpuError(5, f"[gpu.launch] {name}: strides {strides} reach beyond 2^31 values")
     return t.data_ptr(), strides, t.shape[0]
 
 

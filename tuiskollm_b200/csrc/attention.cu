@@ -23,7 +23,7 @@
 // in the even CTA, one step of scores ahead of the values so that the tensor pipe works during the softmax;
 // two softmax warpgroups (thread = row) that take the steps in turn and hand on the rows' references, so that one
 // step's exponentials run beside the other's loads and maxima; four epilogue warps, which normalise, gate and store
-// while the others are on the next tile.  K and V share a ring of four (heads of 128: seven) units; a unit is
+// while the others are on the next tile.  K and V share a ring of three (heads of 128: seven) units; a unit is
 // read where the block table says, page by page.
 //
 // Work split.  All tiles of a launch in order (sequence, key/value head, tile) form one line of keys, and each pair
@@ -40,6 +40,8 @@
 // which the exponentials take 1024 too): the chain scores -> softmax -> values of a step, with one buffer of S per
 // warpgroup, bounds both.
 #include <cuda_fp16.h>
+
+#include <new>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -58,7 +60,7 @@ struct Shape {
   static constexpr int K_KEYS = kKeys / 2;   // a K unit: half of the keys, all chunks
   static constexpr int V_CHUNKS = CHUNKS / 2;  // a V unit: all keys, half of the chunks
   static constexpr int UNIT = K_KEYS * 2 * D;  // bytes of a ring stage
-  static constexpr int STAGES = D == 256 ? 4 : 7;
+  static constexpr int STAGES = D == 256 ? 3 : 7;
 };
 
 // ----------------------------------------------------------------- the line of keys
@@ -193,6 +195,24 @@ struct Walk {
     step = 0;
     ++tile;
     return true;
+  }
+};
+
+// A warp's walk in shared memory, one lane's work: the softmax and epilogue warps have no registers to spare for it.
+struct Stroll {
+  alignas(16) unsigned char walk[sizeof(Walk)];
+  Item it;
+  int more;
+
+  __device__ __forceinline__ void begin(const AttentionParams& p, const Stretch& s, int lane) {
+    if (lane == 0) new (walk) Walk(p, s);
+    __syncwarp();
+  }
+  __device__ __forceinline__ bool next(const AttentionParams& p, int lane) {
+    __syncwarp();
+    if (lane == 0) more = reinterpret_cast<Walk*>(walk)->next(p, &it);
+    __syncwarp();
+    return more != 0;
   }
 };
 
@@ -692,6 +712,8 @@ struct Control {
   uint32_t tmem_base;
   int last_part;
   Stretch stretch;
+  uint4 rows[D == 256 ? 16 : 1][kRows];  // the second halves of rows of 256 between tensor memory and their gate
+  Stroll strolls[12];      // of the softmax and epilogue warps
   float reference[kRows];  // the row's reference maximum, of the step before
   float row_sum[2][kRows];  // what either softmax warpgroup has of a row at a tile's end
   union {
@@ -715,13 +737,9 @@ template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-// Heads of 256 hold 128 words of a row in the epilogue; heads of 128 half of it, and their softmax is what counts (112
-// registers there cost packed prompts 7 %, 128 cost a prompt of heads of 256 5 %).
-template <int D>
-struct Shares {
-  static constexpr int CONTROL = D == 256 ? 80 : 64, SOFTMAX = D == 256 ? 112 : 128, EPILOGUE = D == 256 ? 208 : 192;
-  static_assert(CONTROL + 2 * SOFTMAX + EPILOGUE <= 4 * 128, "the shares exceed the block's registers");
-};
+// (Nothing spills at these; 8 fewer for the epilogue, or for the softmax, do.)
+constexpr int kControlRegisters = 80, kSoftmaxRegisters = 120, kEpilogueRegisters = 192;
+static_assert(kControlRegisters + 2 * kSoftmaxRegisters + kEpilogueRegisters <= 4 * 128, "the shares exceed the block's registers");
 
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -785,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool eights = PAGED && attention_eights(D, p.page_shift);
 
   if (warp < 4) {
-    fewer_registers<Shares<D>::CONTROL>();
+    fewer_registers<kControlRegisters>();
     if (warp == 0) {
       // ---------------------------------------------------------------- producer
       int stage = 0;
@@ -1030,7 +1048,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 12) {
     // ----------------------------------------------------------------- softmax
-    if constexpr (Shares<D>::SOFTMAX < 128) fewer_registers<Shares<D>::SOFTMAX>();
+    fewer_registers<kSoftmaxRegisters>();
     const int group = (warp >> 2) - 1;  // has the steps of its parity, and S buffer `group`
     const int quadrant = warp & 3;      // the TMEM lanes this warp may touch
     const int r = quadrant * 32 + lane;
@@ -1040,9 +1058,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t p_full_even = mapa_u32(smem_u32(&ctl.p_full[group]), 0);
     int n = 0, item = 0;
     bool ok = true;
-    Walk walk(p, stretch);
-    Item it;
-    while (ok && walk.next(p, &it)) {
+    Stroll& stroll = ctl.strolls[warp - 4];
+    stroll.begin(p, stretch, lane);
+    const Item& it = stroll.it;
+    while (ok && stroll.next(p, lane)) {
       const int rows = min(it.tokens - rank * p.half_tokens, p.half_tokens) * p.group;
       const bool active = quadrant * 32 < rows;
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
@@ -1117,16 +1136,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    more_registers<Shares<D>::EPILOGUE>();
+    more_registers<kEpilogueRegisters>();
     const int quadrant = warp & 3, thread = static_cast<int>(threadIdx.x) - 384;
     const int r = quadrant * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
     const uint32_t o_free_even = mapa_u32(smem_u32(&ctl.o_free), 0);
     int item = 0;
-    Walk walk(p, stretch);
-    Item it;
+    Stroll& stroll = ctl.strolls[warp - 4];
+    stroll.begin(p, stretch, lane);
+    const Item& it = stroll.it;
     bool ok = true;  // a warp whose wait ran out still takes part in the barriers of the four
-    while (walk.next(p, &it)) {
+    while (stroll.next(p, lane)) {
       const int rows = min(it.tokens - rank * p.half_tokens, p.half_tokens) * p.group;  // of this CTA, below 1: none
       const int tile_token = it.seq.start + it.tile * p.tile_tokens + rank * p.half_tokens;  // first token row
       const int ahead = it.seq.kv - it.seq.q + it.tile * p.tile_tokens + rank * p.half_tokens;
@@ -1154,10 +1174,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && mine && gate) {
           float most = 0.0f;
 #pragma unroll
-          for (int k = 0; k < D / 32; k += 2) {
+          for (int k = 0; k < D / 64; ++k) {
             uint32_t o[64];
-            tmem_ld32(tmem_o + lanes + 32 * k, o);
-            tmem_ld32(tmem_o + lanes + 32 * k + 32, o + 32);
+            tmem_ld32(tmem_o + lanes + 64 * k, o);
+            tmem_ld32(tmem_o + lanes + 64 * k + 32, o + 32);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 64; i += 2)
@@ -1172,18 +1192,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const F32x2 factor = mul2(scale2, f32x2_splat(up));
-        uint32_t held[D / 2];
+        constexpr int HELD = D == 256 ? 64 : D / 2;  // words of a row in registers, the rest in shared memory
+        uint32_t held[HELD];
         if (ok && mine) {
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            uint32_t o[32];
-            tmem_ld32(tmem_o + lanes + 32 * k, o);
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t o[16];
+            tmem_ld16(tmem_o + lanes + 16 * k, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8; ++i) {
               const F32x2 v = mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), factor);
               const uint32_t w = fp16 ? f32x2_to_f16x2(v) : f32x2_to_bf16x2(v);
-              held[16 * k + i] = blind ? 0u : w;
+              if (8 * k < HELD) {
+                held[(8 * k + i) % HELD] = blind ? 0u : w;
+              } else {
+                o[i] = blind ? 0u : w;  // (values 0 .. 2 i + 1 have been used)
+              }
+            }
+            if (8 * k >= HELD) {
+              ctl.rows[(8 * k - HELD) / 4][r] = make_uint4(o[0], o[1], o[2], o[3]);
+              ctl.rows[(8 * k - HELD) / 4 + 1][r] = make_uint4(o[4], o[5], o[6], o[7]);
             }
           }
         }
@@ -1198,22 +1227,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
 #pragma unroll
           for (int k = 0; k < D / 32; ++k) {
+            uint32_t w[16];
+            if (16 * k < HELD) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = held[(16 * k + i) % HELD];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint4 v = ctl.rows[(16 * k - HELD) / 4 + e][r];
+                w[4 * e] = v.x;
+                w[4 * e + 1] = v.y;
+                w[4 * e + 2] = v.z;
+                w[4 * e + 3] = v.w;
+              }
+            }
             if (gate) {
               uint4 g[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) g[e] = __ldg(gate + 4 * k + e);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t* w = held + 16 * k + 4 * e;
-                w[0] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[0]), down2) : bf16x2_to_f32x2(w[0]), g[e].x));
-                w[1] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[1]), down2) : bf16x2_to_f32x2(w[1]), g[e].y));
-                w[2] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[2]), down2) : bf16x2_to_f32x2(w[2]), g[e].z));
-                w[3] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[3]), down2) : bf16x2_to_f32x2(w[3]), g[e].w));
+              for (int i = 0; i < 16; ++i) {
+                const uint32_t pair = i % 4 == 0 ? g[i / 4].x : i % 4 == 1 ? g[i / 4].y : i % 4 == 2 ? g[i / 4].z : g[i / 4].w;
+                w[i] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[i]), down2) : bf16x2_to_f32x2(w[i]), pair));
               }
             }
             if (r < rows) {
-              store_words8(out + 32 * k, held + 16 * k);
-              store_words8(out + 32 * k + 16, held + 16 * k + 8);
+              store_words8(out + 32 * k, w);
+              store_words8(out + 32 * k + 16, w + 8);
             }
           }
         }

@@ -11,7 +11,7 @@
 // fit its shared memory), then the cluster meets once -- from there nobody reads the lengths, the counter
 // or the pages' old owners again, so outputs may be the planes they were read from -- and the CTAs share the
 // writing: a token or a new page finds its request by bisection of the sums.  Latency-bound: 8 requests of
-// one token 3 us, of which the launch is most.
+// one token 3.8 us, 301 requests with 24000 tokens 12.
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"

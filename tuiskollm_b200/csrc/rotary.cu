@@ -13,7 +13,8 @@
 // A CTA has TOKENS tokens: its threads form their sines and cosines once for all heads while every thread already
 // holds DEPTH heads' values; a head is DIM / 8 lanes of 16 bytes, so the partner of a lane in a rotation is R / 16
 // lanes away and comes by shuffle.  One token a CTA leaves most threads idle in the first half and has its chain of
-// loads, angles and stores to itself (8192 tokens of 32 + 8 heads of 128: 66 us); four share it.
+// loads, angles and stores to itself; four share it: 8192 tokens of 32 + 8 heads of 128 57 us with one, 48.5 with four
+// (4.1 TB/s), 777 tokens of 24 + 4 heads of 256 8.9 with one, 11 with four, so four from 1024 tokens on.
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"

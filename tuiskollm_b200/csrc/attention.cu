@@ -1167,12 +1167,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const F32x2 scale2 = f32x2_splat(blind ? 0.0f : 1.0f / sum);
         // The row leaves tensor memory in 16 bits a value, so that O is free for the next tile before gate and stores: as
         // the BF16 that is stored, or in front of a gate as FP16 times a power of two that puts the row's largest value
-        // near 2^14 (2^-11 of a value where BF16 has 2^-8; values below 2^-28 of the largest lose bits).  A row with
-        // a value that is not finite is held as BF16 there too.
+        // in [2^14, 2^15).  All values that are not zero then have to be normal there, 2^-28 of the largest or more, so that
+        // each is rounded by 2^-11 of itself, where BF16 would take 2^-8.  A warp that has another row (with smaller
+        // values, one that is infinite, or a largest one whose factor fp32 does not hold) gates its rows in fp32 as they leave.
         float up = 1.0f, down = 1.0f;
-        bool fp16 = false;
+        bool direct = false;
         if (ok && mine && gate) {
           float most = 0.0f;
+          uint32_t lowest = 0xffffffffu;  // of 2 |bits| - 1, which puts zeros behind all others
 #pragma unroll
           for (int k = 0; k < D / 64; ++k) {
             uint32_t o[64];
@@ -1180,21 +1182,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(tmem_o + lanes + 64 * k + 32, o + 32);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 64; i += 2)
+            for (int i = 0; i < 64; i += 2) {
               most = fmaxf(most, fmaxf(fabsf(__uint_as_float(o[i])), fabsf(__uint_as_float(o[i + 1]))));
+              lowest = min(lowest, min(2 * o[i] - 1, 2 * o[i + 1] - 1));
+            }
           }
-          most *= fabsf(f32x2_parts(scale2).x);
-          fp16 = most > 0.0f && most < INFINITY;
-          if (fp16) {
-            const int e = min(max(141 - static_cast<int>(__float_as_uint(most) >> 23), -100), 100);  // 14 - exponent
+          const float scale = fabsf(f32x2_parts(scale2).x);
+          const float least = __uint_as_float((lowest + 1) >> 1) * scale;  // (with zeros alone, of no use)
+          most *= scale;
+          if (most >= 0x1p-90f && most <= 0x1p100f) {
+            const int e = 141 - static_cast<int>(__float_as_uint(most) >> 23);  // 14 - exponent
             up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            direct = least < most * 0x1p-28f;
+          } else {
+            direct = most != 0.0f;  // a row of zeros, or of zeros and NaN, waits as it is
           }
+          direct = __any_sync(0xffffffffu, direct && !blind && r < rows);
         }
         const F32x2 factor = mul2(scale2, f32x2_splat(up));
         constexpr int HELD = D == 256 ? 64 : D / 2;  // words of a row in registers, the rest in shared memory
         uint32_t held[HELD];
-        if (ok && mine) {
+        uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, max(rows, 1) - 1));
+        if (direct) {
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t o[16];
+            tmem_ld16(tmem_o + lanes + 16 * k, o);
+            const uint4 g[2] = {__ldg(gate + 2 * k), __ldg(gate + 2 * k + 1)};
+            const uint32_t pairs[8] = {g[0].x, g[0].y, g[0].z, g[0].w, g[1].x, g[1].y, g[1].z, g[1].w};
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const F32x2 v = mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), scale2);
+              o[i] = blind ? 0u : f32x2_to_bf16x2(gated(v, pairs[i]));  // (values 0 .. 2 i + 1 have been used)
+            }
+            if (r < rows) store_words8(out + 16 * k, o);
+          }
+        } else if (ok && mine) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             uint32_t o[16];
@@ -1203,7 +1228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const F32x2 v = mul2(f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), factor);
-              const uint32_t w = fp16 ? f32x2_to_f16x2(v) : f32x2_to_bf16x2(v);
+              const uint32_t w = gate ? f32x2_to_f16x2(v) : f32x2_to_bf16x2(v);
               if (8 * k < HELD) {
                 held[(8 * k + i) % HELD] = blind ? 0u : w;
               } else {
@@ -1222,9 +1247,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_remote_light(o_free_even);
           mbar_arrive(&ctl.stats_free);
         }
-        if (ok && mine) {
+        if (ok && mine && !direct) {
           const F32x2 down2 = f32x2_splat(down);
-          uint16_t* out = output_row<D>(p, tile_token, it.head, min(r, rows - 1));
 #pragma unroll
           for (int k = 0; k < D / 32; ++k) {
             uint32_t w[16];
@@ -1248,7 +1272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const uint32_t pair = i % 4 == 0 ? g[i / 4].x : i % 4 == 1 ? g[i / 4].y : i % 4 == 2 ? g[i / 4].z : g[i / 4].w;
-                w[i] = f32x2_to_bf16x2(gated(fp16 ? mul2(f16x2_to_f32x2(w[i]), down2) : bf16x2_to_f32x2(w[i]), pair));
+                w[i] = f32x2_to_bf16x2(gated(mul2(f16x2_to_f32x2(w[i]), down2), pair));
               }
             }
             if (r < rows) {

@@ -515,7 +515,8 @@ TK100_API tk100_status tk100_page_release(tk100_ctx* ctx, tk100_stream stream, i
  * (may be NULL when there is a cache) and, with the untouched values, to slots[token] of the cache (both
  * planes NULL = no cache; a negative slot is skipped, one behind the last page is skipped and reported).
  * No two tokens have the same slot.  An output may be the plane it is computed from where that has its
- * layout; other overlaps are refused. */
+ * layout; other overlaps of queries, keys, values, outputs and caches are refused.  (A cache counts from its first
+ * page to its last; key and value planes that lie in turn in one another's gaps do not overlap.) */
 TK100_API tk100_status tk100_rotary_cache(tk100_ctx* ctx, tk100_stream stream, int tokens, int q_heads,
                                           int kv_heads, int head_dim, int rotary_dim, int axes,
                                           const double* frequencies, const uint8_t* pair_axes,
@@ -540,9 +541,10 @@ TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_
  * (the queries' strides).  output is [tokens, q_heads, head_dim] and starts on 32 bytes; rows outside the sequences are left as
  * they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
  * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used,
- * whatever it is.  Weights times values are summed in FP32, with weights of up to 2^8, in front of the division by
- * the weights' sum; a sigmoid below 2^-126 (a gate below -87.3) counts as zero.  A key or value of the sequence itself that is not finite reaches the tokens that see it,
- * and through 0 * NaN may reach those up to 127 positions in front of it. */
+ * whatever it is.  The output overlaps nothing that is read.  Weights times values are summed in FP32, with weights
+ * of up to 2^8, in front of the division by the weights' sum; a sigmoid below 2^-126 (a gate below -87.3) counts as
+ * zero.  A key or value of the sequence itself that is not finite reaches the tokens that see it, and through
+ * 0 * NaN may reach those up to 127 positions in front of it. */
 TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
                                              int q_heads, int kv_heads, int head_dim, const int32_t* starts,
                                              const int32_t* kv_lengths, const uint16_t* query,

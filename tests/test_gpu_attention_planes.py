@@ -1,0 +1,103 @@
+"""Planes that the full-attention operators take, and those that they refuse: shapes, overlaps, positions."""
+import pytest
+import torch
+
+import attention_ref as ref
+import tuiskollm_b200 as tk
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return tk.Context()
+
+
+def ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device="cuda")
+
+
+def zeros(*shape):
+    return torch.zeros(*shape, dtype=BF16, device="cuda")
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+
+
+class Calls:
+    """One call of each operator that writes rows of heads, whose planes can be replaced."""
+
+    def __init__(self, ctx, tokens=5, q_heads=6, kv_heads=2, dim=128):
+        self.cache = ref.Paged([40], kv_heads, dim, 16, 3)
+        self.query = normal(1, tokens, q_heads, dim)
+        self.key, self.value = normal(2, tokens, kv_heads, dim), normal(3, tokens, kv_heads, dim)
+        self.q_out, self.k_out = zeros(tokens, q_heads, dim), zeros(tokens, kv_heads, dim)
+        self.paged_op = tk.PagedAttentionOp(ctx, q_heads, kv_heads, dim)
+        self.prompt_op = tk.PromptAttentionOp(ctx, q_heads, kv_heads, dim)
+        self.rotary_op = tk.RotaryCacheOp(ctx, q_heads, kv_heads, dim, tk.rotary_frequencies(64, 1e4))
+        self.work, self.starts = self.paged_op.workspace(), ints([0, tokens])
+        self.paged_base = dict(sequences=1, starts=self.starts, kv_lengths=ints([40]), query=self.query, gate=None,
+                               key_cache=self.cache.key, value_cache=self.cache.value, block_table=self.cache.table,
+                               request_rows=None, workspace=self.work, output=self.q_out)
+        self.prompt_base = dict(sequences=1, starts=self.starts, query=self.query, gate=None, key=self.key, value=self.value,
+                                workspace=self.work, output=self.q_out)
+        self.rotary_base = dict(tokens=tokens, positions=torch.arange(tokens, dtype=torch.int32, device="cuda"),
+                                query=self.query, key=self.key, value=self.value, query_norm=None, key_norm=None,
+                                query_output=self.q_out, key_output=self.k_out, key_cache=zeros(2, 16, kv_heads, dim),
+                                value_cache=zeros(2, 16, kv_heads, dim), slots=torch.arange(tokens, device="cuda"))
+
+    def paged(self, **change):
+        self.paged_op.launch(None, **{**self.paged_base, **change})
+
+    def prompt(self, **change):
+        self.prompt_op.launch(None, **{**self.prompt_base, **change})
+
+    def rotary(self, **change):
+        self.rotary_op.launch(None, **{**self.rotary_base, **change})
+
+
+@pytest.fixture(scope="module")
+def calls(ctx):
+    return Calls(ctx)
+
+
+def test_overlaps_are_refused(ctx, calls):
+    def refused(call, text, **change):
+        with pytest.raises(tk.GpuError, match=text):
+            call(**change)
+
+    # caches over rows that other CTAs still read, or over the outputs
+    pool = zeros(2 * 16 * 2 * 128 + 5 * 768)
+    cache, rows = pool[:2 * 16 * 2 * 128].view(2, 16, 2, 128), pool[2 * 16 * 2 * 128 - 512:][:5 * 768].view(5, 6, 128)
+    kv_rows = pool[512:][:5 * 256].view(5, 2, 128)
+    for name in ("key_cache", "value_cache"):
+        refused(calls.rotary, "cache overlaps the queries", query=rows, **{name: cache})
+        refused(calls.rotary, "cache overlaps the query output", query_output=rows, **{name: cache})
+        refused(calls.rotary, "cache overlaps the keys", key=kv_rows, **{name: cache})
+        refused(calls.rotary, "cache overlaps the values", value=kv_rows, **{name: cache})
+        refused(calls.rotary, "cache overlaps the key output", key_output=kv_rows, **{name: cache})
+        apart = dict(key_cache=zeros(2, 16, 2, 128), value_cache=zeros(2, 16, 2, 128))
+        refused(calls.paged, "output overlaps the key or value cache", output=rows, **{**apart, name: cache})
+    # one plane for both caches, and planes that share some of their values
+    refused(calls.rotary, "key cache overlaps the value cache", key_cache=cache, value_cache=cache)
+    both = zeros(2, 16, 2, 192)
+    refused(calls.rotary, "key cache overlaps the value cache", key_cache=both[..., :128], value_cache=both[..., 64:])
+    shifted = zeros(3, 16, 2, 128)
+    refused(calls.rotary, "key cache overlaps the value cache", key_cache=shifted[:2], value_cache=shifted[1:])
+    assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("order", ["heads", "tokens", "pages", "page heads"])
+def test_caches_in_one_plane_are_taken(ctx, calls, order):
+    """Keys and values in turn: next to each other in a head, a token or a page, and in a page of [heads, tokens]."""
+    both = {"heads": zeros(2, 16, 2, 2, 128), "tokens": zeros(2, 16, 2, 2, 128), "pages": zeros(2, 2, 16, 2, 128),
+            "page heads": zeros(2, 2, 2, 16, 128)}[order]
+    pick = {"heads": lambda i: both[:, :, :, i], "tokens": lambda i: both[:, :, i], "pages": lambda i: both[:, i],
+            "page heads": lambda i: both[:, i].transpose(1, 2)}[order]
+    calls.rotary(key_cache=pick(0), value_cache=pick(1))
+    assert ctx.device_status() == 0
+    assert torch.equal(pick(0)[0, :5], calls.k_out) and torch.equal(pick(1)[0, :5], calls.value)
+    assert int(both.count_nonzero()) == int(calls.k_out.count_nonzero()) + int(calls.value.count_nonzero())

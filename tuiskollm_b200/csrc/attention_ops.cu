@@ -97,8 +97,38 @@ struct Span {
   Span(const uint16_t* p, long long tokens, long long token_stride, long long heads, long long head_stride, int dim)
       : first(reinterpret_cast<uintptr_t>(p)),
         last(first + 2 * static_cast<uintptr_t>((tokens - 1) * token_stride + (heads - 1) * head_stride + dim)) {}
+  // the same for a cache plane, from its first page to its last
+  Span(const uint16_t* p, const CacheGeometry& g, int heads, int dim) : Span(p, g.page_tokens, g.token_stride, heads, g.head_stride, dim) {
+    last += 2 * static_cast<uintptr_t>(static_cast<long long>(g.pages - 1) * g.page_stride);
+  }
   bool meets(const Span& o) const { return first < o.last && o.first < last; }
 };
+
+// Whether two planes of the same extents and strides, the second `apart` values behind the first, have one in common:
+// whether multiples of the strides, each below its extent either way, add up to less than `least` from `apart`.
+// Strides fall; where they nest, as a plane's do whose own values lie apart, two multiples of each come near enough at
+// most.  Where many do, the answer is yes.
+struct Dimension {
+  long long extent, stride;
+};
+bool planes_share(long long apart, const Dimension* dims, int count, long long least) {
+  if (count == 0) return apart > -least && apart < least;
+  const long long extent = dims[0].extent, stride = dims[0].stride;
+  long long reach = least - 1;  // of what is left, either way
+  for (int i = 1; i < count; ++i) reach += (dims[i].extent - 1) * dims[i].stride;
+  auto below = [](long long a, long long b) { return a / b - (a % b < 0); };  // a / b rounded down, b > 0
+  const long long from = std::max(-below(reach - apart, stride), 1 - extent), to = std::min(below(apart + reach, stride), extent - 1);
+  if (to - from > 2) return true;
+  for (long long m = from; m <= to; ++m)
+    if (planes_share(apart - m * stride, dims + 1, count - 1, least)) return true;
+  return false;
+}
+
+bool caches_share(const uint16_t* key, const uint16_t* value, const CacheGeometry& g, int heads, int dim) {
+  Dimension dims[3] = {{g.pages, g.page_stride}, {g.page_tokens, g.token_stride}, {heads, g.head_stride}};
+  std::sort(dims, dims + 3, [](const Dimension& a, const Dimension& b) { return a.stride > b.stride; });
+  return planes_share((reinterpret_cast<intptr_t>(value) - reinterpret_cast<intptr_t>(key)) / 2, dims, 3, dim);
+}
 
 }  // namespace
 
@@ -183,8 +213,8 @@ Status RotaryCacheOp::launch(cudaStream_t stream, int head_dim, RotaryParams p, 
   } else if (!p.key_output) {
     return refuse(ctx_, what, "rotated keys go nowhere: neither a key output nor a cache");
   }
-  // An output may be the plane it is computed from, element for element; any other overlap would have one
-  // CTA write what another still reads.
+  // An output may be the plane it is computed from, element for element; any other overlap would have one CTA write
+  // what another still reads, or two CTAs write one place.
   const Span query(p.query, p.tokens, p.query_token_stride, p.q_heads, p.query_head_stride, head_dim);
   const Span key(p.key, p.tokens, p.kv_token_stride, p.kv_heads, p.kv_head_stride, head_dim);
   const Span q_out(p.query_output, p.tokens, static_cast<long long>(p.q_heads) * head_dim, p.q_heads, head_dim, head_dim);
@@ -201,10 +231,18 @@ Status RotaryCacheOp::launch(cudaStream_t stream, int head_dim, RotaryParams p, 
   if (p.key_cache) {
     const Span value(p.value, p.tokens, p.kv_token_stride, p.kv_heads, p.kv_head_stride, head_dim);
     if (q_out.meets(value)) return refuse(ctx_, what, "the query output overlaps the values");
-    if (p.key_output) {
-      const Span k_out(p.key_output, p.tokens, static_cast<long long>(p.kv_heads) * head_dim, p.kv_heads, head_dim, head_dim);
-      if (k_out.meets(value)) return refuse(ctx_, what, "the key output overlaps the values");
+    const Span k_out = !p.key_output ? key
+                                     : Span(p.key_output, p.tokens, static_cast<long long>(p.kv_heads) * head_dim, p.kv_heads,
+                                            head_dim, head_dim);
+    if (p.key_output && k_out.meets(value)) return refuse(ctx_, what, "the key output overlaps the values");
+    const Span caches[2] = {{p.key_cache, cache, p.kv_heads, head_dim}, {p.value_cache, cache, p.kv_heads, head_dim}};
+    for (const Span& c : caches) {
+      const char* other = c.meets(query) ? "queries" : c.meets(key) ? "keys" : c.meets(value) ? "values"
+                          : c.meets(q_out) ? "query output" : c.meets(k_out) ? "key output" : nullptr;
+      if (other) return refuse(ctx_, what, std::string("a cache overlaps the ") + other);
     }
+    if (caches_share(p.key_cache, p.value_cache, cache, p.kv_heads, head_dim))
+      return refuse(ctx_, what, "the key cache overlaps the value cache");
   }
   p.epsilon = ctx_.config().rms_norm_epsilon;
   p.status = ctx_.status_word();
@@ -305,6 +343,9 @@ Status AttentionOp::paged(cudaStream_t stream, int head_dim, AttentionParams p, 
   TK100_TRY(plane(ctx_, what, "block table", p.block_table, 4));
   TK100_TRY(range(ctx_, what, "block table row count", p.table_row_count, 1, 1 << 30));
   TK100_TRY(range(ctx_, what, "pages per row", p.max_pages, 1, 1 << 30));
+  const Span out(p.output, p.tokens, static_cast<long long>(p.q_heads) * head_dim, p.q_heads, head_dim, head_dim);
+  if (out.meets(Span(key_cache, cache, p.kv_heads, head_dim)) || out.meets(Span(value_cache, cache, p.kv_heads, head_dim)))
+    return refuse(ctx_, what, "the output overlaps the key or value cache");
   if (!p.table_rows && p.sequences > p.table_row_count)
     return refuse(ctx_, what, "the block table has fewer rows than there are sequences");
   p.page_shift = log2_of(cache.page_tokens);

@@ -49,7 +49,8 @@ SUITES = {
     "nvfp4-down": ["tests/test_gpu_nvfp4.py"],
     "page-plan": ["tests/test_gpu_paging.py"],
     "rotary-cache": ["tests/test_gpu_rotary.py"],
-    "attention": ["tests/test_gpu_attention.py", "tests/test_gpu_attention_gates.py", "tests/test_gpu_full_attention_step.py"],
+    "attention": ["tests/test_gpu_attention.py", "tests/test_gpu_attention_gates.py", "tests/test_gpu_attention_planes.py",
+                  "tests/test_gpu_full_attention_step.py"],
     "peer-exchange": ["tests/test_gpu_peer_sum.py", "tests/test_gpu_multi.py"],
     "static-entry": ["tests/test_zz_no_alloc.py"],
     "host-codecs": ["tests/test_oracle_kat.py", "tests/test_oracle_gdn.py"],

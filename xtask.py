@@ -48,7 +48,7 @@ SUITES = {
     "nvfp4-swiglu": ["tests/test_gpu_nvfp4.py"],
     "nvfp4-down": ["tests/test_gpu_nvfp4.py"],
     "page-plan": ["tests/test_gpu_paging.py"],
-    "rotary-cache": ["tests/test_gpu_rotary.py"],
+    "rotary-cache": ["tests/test_gpu_rotary.py", "tests/test_gpu_rotary_many.py"],
     "attention": ["tests/test_gpu_attention.py", "tests/test_gpu_attention_gates.py", "tests/test_gpu_attention_planes.py",
                   "tests/test_gpu_full_attention_step.py"],
     "peer-exchange": ["tests/test_gpu_peer_sum.py", "tests/test_gpu_multi.py"],

@@ -64,6 +64,31 @@ def calls(ctx):
     return Calls(ctx)
 
 
+def test_outputs_of_another_order_are_refused(ctx, calls):
+    """An output whose heads do not lie behind one another in a token's row would be filled in another order."""
+    for other in (zeros(6, 5, 128), zeros(128, 6, 5), zeros(768, 5), zeros(6, 640)):
+        for call, name in ((calls.paged, "output"), (calls.prompt, "output"), (calls.rotary, "query_output")):
+            with pytest.raises(tk.GpuError, match=name.replace("_", " ")):
+                call(**{name: other})
+    with pytest.raises(tk.GpuError, match="key output"):
+        calls.rotary(key_output=zeros(2, 5, 128))
+    assert ctx.device_status() == 0
+
+
+def test_outputs_in_rows_of_any_shape(ctx, calls):
+    """Planes with the rows' order: flat, a row a token, heads in groups, more rows than tokens."""
+    for call, name in ((calls.paged, "output"), (calls.prompt, "output"), (calls.rotary, "query_output")):
+        first = zeros(5, 6, 128)
+        call(**{name: first})
+        assert float(first.float().abs().sum()) > 0
+        for shape in ((5, 768), (5 * 768,), (30, 128), (1, 5, 6, 128), (5, 1, 768), (5, 2, 3, 128), (7, 6, 128)):
+            out = zeros(*shape)
+            call(**{name: out})
+            assert torch.equal(out.view(-1)[:5 * 768], first.view(-1)), (name, shape)
+            assert float(out.view(-1)[5 * 768:].float().abs().sum()) == 0
+    assert ctx.device_status() == 0
+
+
 def test_overlaps_are_refused(ctx, calls):
     def refused(call, text, **change):
         with pytest.raises(tk.GpuError, match=text):

@@ -407,6 +407,23 @@ def _heads(context: Context, t, name, *shape):
     return t.data_ptr(), strides, t.shape[0]
 
 
+def _head_rows(context: Context, t, name, rows, heads, head_dim):
+    """Address of a dense BF16 plane of at least `rows` rows of `heads` heads: [rows, heads, head_dim], or of another shape
+    whose values lie in that order (flat, a row or a head per row, a row's heads in groups, more dimensions in front)."""
+    found = context._heads(t, context.device, -1, heads, head_dim)
+    if found is not None and found[2] >= rows and found[1] == (heads * head_dim, head_dim, 1):
+        return found[0]
+    address = _plane(context, t, name, torch.bfloat16, rows * heads * head_dim)
+    width, values = heads * head_dim, 1
+    for extent in reversed(t.shape):
+        values *= extent
+        if values >= width:
+            break
+    if values != width and not (t.dim() == 1 or (t.dim() == 2 and t.shape[1] == head_dim)):
+        raise GpuError(5, f"[gpu.launch] {name}: shape {tuple(t.shape)} is not rows of {heads} heads of {head_dim} values")
+    return address
+
+
 def _cache(context: Context, key_cache, value_cache, kv_heads, head_dim):
     """(addresses, pages, page tokens, strides) of a cache pair ``[pages, page tokens, heads, head_dim]``."""
     key, strides, pages = _heads(context, key_cache, "key cache", -1, -1, kv_heads, head_dim)
@@ -538,8 +555,8 @@ class RotaryCacheOp:
             self._pair_axes, _plane(c, positions, "positions", torch.int32, axes * tokens), q, qs[0], qs[1], k, v,
             ks[0], ks[1], None if query_norm is None else _plane(c, query_norm, "query norm", bf16, dim),
             None if key_norm is None else _plane(c, key_norm, "key norm", bf16, dim),
-            _plane(c, query_output, "query output", bf16, tokens * self.q_heads * dim),
-            None if key_output is None else _plane(c, key_output, "key output", bf16, tokens * self.kv_heads * dim),
+            _head_rows(c, query_output, "query output", tokens, self.q_heads, dim),
+            None if key_output is None else _head_rows(c, key_output, "key output", tokens, self.kv_heads, dim),
             kc, vc, pages, page_tokens, cs[0], cs[1], cs[2], at)
 
 
@@ -564,7 +581,7 @@ class _AttentionOp:
                 raise GpuError(5, f"[gpu.launch] query and gate have different strides {qs} and {gs}")
         return (tokens, q, g, qs, _plane(c, starts, "starts", torch.int32, sequences + 1),
                 _plane(c, workspace, "workspace", torch.uint8, self._workspace_bytes),
-                _plane(c, output, "output", torch.bfloat16, tokens * self.q_heads * dim))
+                _head_rows(c, output, "output", tokens, self.q_heads, dim))
 
 
 class PagedAttentionOp(_AttentionOp):

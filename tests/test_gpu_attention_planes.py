@@ -89,6 +89,26 @@ def test_outputs_in_rows_of_any_shape(ctx, calls):
     assert ctx.device_status() == 0
 
 
+def test_positions_are_axes_by_tokens(ctx, calls):
+    query = ref.f64(calls.query)
+    positions = torch.arange(5, dtype=torch.int32, device="cuda") * 7
+    expected = ref.rotate(query, positions[None], calls.rotary_op.frequencies, None)
+    for shape in ((5,), (1, 5), (1, 1, 5)):
+        calls.rotary(positions=positions.view(shape))
+        assert bool(((ref.f64(calls.q_out) - expected).abs() <= 2.0 ** -8 * expected.abs() + 16 * 2.0 ** -18).all())
+    op = tk.RotaryCacheOp(ctx, 6, 2, 128, tk.rotary_frequencies(64, 1e4), torch.tensor([0, 1, 2, 1] * 8, dtype=torch.uint8).cuda())
+    axes = torch.stack([positions, positions * 2, positions + 3])
+    expected = ref.rotate(query, axes, op.frequencies, op.pair_axes)
+    for shape in ((3, 5), (3, 1, 5)):
+        op.launch(None, **{**calls.rotary_base, "positions": axes.view(shape)})
+        assert bool(((ref.f64(calls.q_out) - expected).abs() <= 2.0 ** -8 * expected.abs() + 16 * 2.0 ** -18).all())
+    assert ctx.device_status() == 0
+    for other in (axes.view(1, 3, 5), axes[:2].view(1, 2, 5), axes.t().contiguous(), torch.tensor(3, dtype=torch.int32, device="cuda"),
+                  torch.zeros(0, 5, dtype=torch.int32, device="cuda")):
+        with pytest.raises(tk.GpuError, match="position"):
+            op.launch(None, **{**calls.rotary_base, "positions": other})
+
+
 def test_overlaps_are_refused(ctx, calls):
     def refused(call, text, **change):
         with pytest.raises(tk.GpuError, match=text):

@@ -524,8 +524,8 @@ class RotaryCacheOp:
     def launch(self, stream, tokens, positions, query, key, value, query_norm, key_norm, query_output, key_output,
                key_cache, value_cache, slots):
         """``query`` ``[>= tokens, q_heads, head_dim]``, ``key`` and ``value`` ``[>= tokens, kv_heads, head_dim]`` with any
-        token and head strides (views of the projection's rows); ``positions`` int32 ``[axes, tokens]`` or
-        ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output`` dense or None; caches
+        token and head strides (views of the projection's rows); ``positions`` int32 ``[axes, tokens]`` (or with
+        extents of one between) or ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output`` dense or None; caches
         ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
         c, dim = self.ctx, self.head_dim
         q, qs, q_rows = _heads(c, query, "query", -1, self.q_heads, dim)
@@ -538,8 +538,8 @@ class RotaryCacheOp:
                 raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
         if q_rows < tokens or rows < tokens:
             raise GpuError(5, f"[gpu.launch] rotary: planes have fewer than {tokens} rows")
-        axes = 1 if positions.dim() == 1 else positions.shape[0]
-        if positions.shape[-1] != tokens:
+        axes = 1 if positions.dim() == 1 else positions.shape[0] if positions.dim() > 1 else 0
+        if axes == 0 or positions.shape[-1] != tokens or (positions.dim() > 2 and positions.numel() != axes * tokens):
             raise GpuError(5, f"[gpu.launch] positions: shape {tuple(positions.shape)} is not [axes, {tokens}]")
         bf16 = torch.bfloat16
         kc = vc = at = None

@@ -109,6 +109,32 @@ def test_positions_are_axes_by_tokens(ctx, calls):
             op.launch(None, **{**calls.rotary_base, "positions": other})
 
 
+def test_what_is_no_tensor_is_refused(ctx, calls):
+    """With the operators' error, whichever plane it is."""
+    for change in (dict(block_table=None), dict(block_table=7), dict(output=None), dict(query=None), dict(key_cache=None),
+                   dict(starts=None), dict(workspace=None), dict(kv_lengths=[40])):
+        with pytest.raises(tk.GpuError):
+            calls.paged(**change)
+    for change in (dict(positions=None), dict(positions=[0, 1, 2, 3, 4]), dict(slots=3), dict(query_output=None), dict(key=None)):
+        with pytest.raises(tk.GpuError):
+            calls.rotary(**change)
+    for change in (dict(frequencies=None), dict(frequencies=[1.0] * 32)):
+        with pytest.raises(tk.GpuError, match="frequencies"):
+            tk.RotaryCacheOp(ctx, 6, 2, 128, **change)
+    plan = dict(requests=1, request_rows=None, new_tokens=ints([1]), lengths=ints([0]), lengths_output=ints([0]),
+                block_table=ints([[0, 0]]), free_pages=ints([0, 1]), free_count=ints([2]), free_count_output=ints([0]),
+                starts=ints([0, 0]), kv_lengths=ints([0]), positions=ints([0]), slots=ints([0], torch.int64))
+    op = tk.PagePlanOp(ctx, 16)
+    for name in plan:
+        if name in ("requests", "request_rows"):
+            continue
+        for other in (None, 3, [0, 0]):
+            with pytest.raises(tk.GpuError):
+                op.launch(None, **{**plan, name: other})
+    op.launch(None, **plan)
+    assert ctx.device_status() == 0
+
+
 def test_overlaps_are_refused(ctx, calls):
     def refused(call, text, **change):
         with pytest.raises(tk.GpuError, match=text):

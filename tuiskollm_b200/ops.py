@@ -383,6 +383,20 @@ def _plane(context: Context, t, name, dtype, least):
     return t.data_ptr()
 
 
+def _tensor(t, name):
+    """`t`, whose extents the caller goes by."""
+    if not isinstance(t, torch.Tensor):
+        raise GpuError(5, f"[gpu.launch] {name}: a tensor is required, got {type(t).__name__}")
+    return t
+
+
+def _block_table(t):
+    """(rows, pages) of a block table."""
+    if _tensor(t, "block table").dim() != 2:
+        raise GpuError(5, f"[gpu.launch] block table: shape {tuple(t.shape)} is not [rows, pages]")
+    return t.shape
+
+
 def _heads(context: Context, t, name, *shape):
     """(address, strides, first extent) of a BF16 plane of the given shape (-1: any extent) whose last dimension is
     dense.  An extent of one has the stride of a dense plane, whatever the tensor says of it."""
@@ -452,11 +466,9 @@ class PagePlanOp:
     def _state(self, requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count,
                free_count_output):
         c = self.ctx
-        if block_table.dim() != 2:
-            raise GpuError(5, f"[gpu.launch] block table: shape {tuple(block_table.shape)} is not [rows, pages]")
-        rows, pages = block_table.shape
+        rows, pages = _block_table(block_table)
         i32 = torch.int32
-        return (rows, pages, free_pages.numel(),
+        return (rows, pages, _tensor(free_pages, "free pages").numel(),
                 None if request_rows is None else _plane(c, request_rows, "request rows", i32, requests),
                 _plane(c, lengths, "lengths", i32, rows), _plane(c, lengths_output, "length output", i32, rows),
                 _plane(c, block_table, "block table", i32, 1), _plane(c, free_pages, "free pages", i32, 1),
@@ -467,7 +479,7 @@ class PagePlanOp:
         c = self.ctx
         rows, pages, capacity, chosen, old, new, table, stack, count, left = self._state(
             requests, request_rows, lengths, lengths_output, block_table, free_pages, free_count, free_count_output)
-        tokens = slots.numel()
+        tokens = _tensor(slots, "slots").numel()
         c._native.tk100_page_plan(
             c, stream, requests, rows, pages, self.page_tokens, tokens, capacity, chosen,
             _plane(c, new_tokens, "new tokens", torch.int32, requests), old, new, table, stack, count, left,
@@ -515,7 +527,7 @@ class RotaryCacheOp:
 
     def __init__(self, context: Context, q_heads: int, kv_heads: int, head_dim: int, frequencies, pair_axes=None):
         self.ctx, self.q_heads, self.kv_heads, self.head_dim = context, q_heads, kv_heads, head_dim
-        self.rotary_dim = 2 * frequencies.numel()
+        self.rotary_dim = 2 * _tensor(frequencies, "frequencies").numel()
         self.frequencies, self.pair_axes = frequencies, pair_axes
         self._frequencies = _plane(context, frequencies, "frequencies", torch.float64, 1)
         self._pair_axes = None if pair_axes is None else _plane(context, pair_axes, "pair axes", torch.uint8,
@@ -538,7 +550,7 @@ class RotaryCacheOp:
                 raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
         if q_rows < tokens or rows < tokens:
             raise GpuError(5, f"[gpu.launch] rotary: planes have fewer than {tokens} rows")
-        axes = 1 if positions.dim() == 1 else positions.shape[0] if positions.dim() > 1 else 0
+        axes = 1 if _tensor(positions, "positions").dim() == 1 else positions.shape[0] if positions.dim() > 1 else 0
         if axes == 0 or positions.shape[-1] != tokens or (positions.dim() > 2 and positions.numel() != axes * tokens):
             raise GpuError(5, f"[gpu.launch] positions: shape {tuple(positions.shape)} is not [axes, {tokens}]")
         bf16 = torch.bfloat16
@@ -598,13 +610,12 @@ class PagedAttentionOp(_AttentionOp):
         c = self.ctx
         tokens, q, g, qs, at, work, out = self._rows(sequences, starts, query, gate, workspace, output)
         key, value, pages, page_tokens, cs = _cache(c, key_cache, value_cache, self.kv_heads, self.head_dim)
-        if block_table.dim() != 2:
-            raise GpuError(5, f"[gpu.launch] block table: shape {tuple(block_table.shape)} is not [rows, pages]")
+        rows, row_pages = _block_table(block_table)
         c._native.tk100_paged_attention(
             c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,
             _plane(c, kv_lengths, "key lengths", torch.int32, sequences), q, g, qs[0], qs[1], key, value, pages,
             page_tokens, cs[0], cs[1], cs[2], _plane(c, block_table, "block table", torch.int32, 1),
-            block_table.shape[0], block_table.shape[1],
+            rows, row_pages,
             None if request_rows is None else _plane(c, request_rows, "request rows", torch.int32, sequences),
             self.scale, work, out)
 

@@ -482,7 +482,9 @@ TK100_API tk100_status tk100_fp8_projection_static_status(tk100_stream stream, u
  *   kv_lengths    [requests]      lengths with the new tokens
  *   positions     [max_tokens]    position of every token row (0 behind the last)
  *   slots         [max_tokens]    its place in the cache (-1 behind the last)
- *   lengths_output, free_count_output: the new values; may be the planes they were read from.
+ *   lengths_output, free_count_output: the new values (rows of no request stay as they are); may be the planes
+ *   they were read from.
+ * A negative page id in a row or on the stack names no page: its tokens get slot -1, and the status word says so.
  * A step that does not fit -- a row out of range or given twice, too few free pages, more than max_tokens
  * tokens, more tokens than max_pages hold -- changes nothing: starts and kv_lengths are zero, slots -1,
  * and the status word says TK100_DEVICE_BAD_ARGUMENT.  requests <= 4096, table_rows <= 262144,
@@ -497,7 +499,8 @@ TK100_API tk100_status tk100_page_plan(tk100_ctx* ctx, tk100_stream stream, int 
 
 /* Gives the pages of requests that ended back: pushed onto the stack in request order, a request's in the
  * order of its row, whose entries stay as they are; the requests' lengths become 0.  Refused as above
- * where a row is out of range or given twice, or the stack has no room. */
+ * where a row is out of range or given twice, or the stack has no room; a negative page id is pushed like the
+ * others, and reported. */
 TK100_API tk100_status tk100_page_release(tk100_ctx* ctx, tk100_stream stream, int requests, int table_rows,
                                           int max_pages, int page_tokens, int free_capacity,
                                           const int32_t* request_rows, const int32_t* lengths,

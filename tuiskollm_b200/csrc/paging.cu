@@ -150,7 +150,9 @@ __global__ void __launch_bounds__(kThreads) page_kernel(const PageParams p) {
       const Request r = requests[request_of<true>(requests, p.requests, k)];
       int* line = p.block_table + static_cast<size_t>(r.row) * p.max_pages;
       if (RELEASE) {
-        p.free_pages[free_count + k] = line[k - r.page];
+        const int id = line[k - r.page];
+        if (id < 0) atomicOr(p.status, STATUS_BAD_ARGUMENT);
+        p.free_pages[free_count + k] = id;
       } else {
         line[((r.length + page - 1) >> shift) + (k - r.page)] = p.free_pages[free_count - 1 - k];
       }
@@ -168,7 +170,11 @@ __global__ void __launch_bounds__(kThreads) page_kernel(const PageParams p) {
         const int index = position >> shift, fresh = index - ((r.length + page - 1) >> shift);
         const int id = fresh < 0 ? p.block_table[static_cast<size_t>(r.row) * p.max_pages + index]
                                  : p.free_pages[free_count - 1 - (r.page + fresh)];
-        slot = (static_cast<long long>(id) << shift) + (position & (page - 1));
+        if (id >= 0) {
+          slot = (static_cast<long long>(id) << shift) + (position & (page - 1));
+        } else {  // no page; a negative slot alone would pass for padding
+          atomicOr(p.status, STATUS_BAD_ARGUMENT);
+        }
       }
       p.positions[t] = position;
       p.slots[t] = slot;

@@ -47,7 +47,7 @@ SUITES = {
     "gdn-recurrence": ["tests/test_gpu_gdn.py"],
     "nvfp4-swiglu": ["tests/test_gpu_nvfp4.py"],
     "nvfp4-down": ["tests/test_gpu_nvfp4.py"],
-    "page-plan": ["tests/test_gpu_paging.py"],
+    "page-plan": ["tests/test_gpu_paging.py", "tests/test_gpu_paging_bad_pages.py"],
     "rotary-cache": ["tests/test_gpu_rotary.py", "tests/test_gpu_rotary_many.py"],
     "attention": ["tests/test_gpu_attention.py", "tests/test_gpu_attention_gates.py", "tests/test_gpu_attention_planes.py",
                   "tests/test_gpu_attention_joins.py",

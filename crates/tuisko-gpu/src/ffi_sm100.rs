@@ -13,7 +13,7 @@ pub type Tk100Stream = *mut c_void;
 /// `tk100_status`: 0 ok, 1..=6 = `GpuErrorCode::{Driver, Arena, Graph, Context, Launch, Module}`.
 pub type Tk100Status = c_int;
 
-pub const TK100_ABI_VERSION: u32 = 1;
+pub const TK100_ABI_VERSION: u32 = 2;
 pub const TK100_DEVICE_WAIT_TIMEOUT: u32 = 1;
 pub const TK100_DEVICE_NONFINITE_LOGIT: u32 = 2;
 pub const TK100_DEVICE_NONFINITE_INPUT: u32 = 4;
@@ -255,16 +255,16 @@ unsafe extern "C" {
         ctx: *mut Tk100Ctx, stream: Tk100Stream, sequences: c_int, tokens: c_int,
         q_heads: c_int, kv_heads: c_int, head_dim: c_int, starts: *const i32,
         kv_lengths: *const i32, query: *const u16, gate: *const u16, query_token_stride: c_int,
-        query_head_stride: c_int, key_cache: *const u16, value_cache: *const u16, pages: c_int,
-        page_tokens: c_int, page_stride: c_int, cache_token_stride: c_int,
-        cache_head_stride: c_int, block_table: *const i32, table_rows: c_int, max_pages: c_int,
+        query_head_stride: c_int, gate_token_stride: c_int, gate_head_stride: c_int,
+        key_cache: *const u16, value_cache: *const u16, pages: c_int, page_tokens: c_int,
+        page_stride: c_int, cache_token_stride: c_int, cache_head_stride: c_int, block_table: *const i32, table_rows: c_int, max_pages: c_int,
         request_rows: *const i32, scale: f32, workspace: *mut c_void, output: *mut u16,
     ) -> Tk100Status;
     pub fn tk100_prompt_attention(
         ctx: *mut Tk100Ctx, stream: Tk100Stream, sequences: c_int, tokens: c_int,
         q_heads: c_int, kv_heads: c_int, head_dim: c_int, starts: *const i32,
         query: *const u16, gate: *const u16, query_token_stride: c_int,
-        query_head_stride: c_int, key: *const u16, value: *const u16, kv_token_stride: c_int,
-        kv_head_stride: c_int, scale: f32, workspace: *mut c_void, output: *mut u16,
+        query_head_stride: c_int, gate_token_stride: c_int, gate_head_stride: c_int,
+        key: *const u16, value: *const u16, kv_token_stride: c_int, kv_head_stride: c_int, scale: f32, workspace: *mut c_void, output: *mut u16,
     ) -> Tk100Status;
 }

@@ -527,11 +527,11 @@ impl AttentionOp {
         unsafe { ffi::tk100_attention_workspace_bytes(self.ctx.raw, rows_i32(self.heads.2)) }
     }
 
-    /// `tk100_paged_attention`; `query` and `gate` share the (token stride, head stride).
+    /// `tk100_paged_attention`; `query` and `gate` (null: none) each with their (token stride, head stride).
     #[allow(clippy::too_many_arguments)]
     pub unsafe fn launch_paged(
         &self, stream: &CudaStream, sequences: usize, tokens: usize, starts: *const i32,
-        kv_lengths: *const i32, query: *const u16, gate: *const u16, q_strides: (usize, usize),
+        kv_lengths: *const i32, query: (*const u16, usize, usize), gate: (*const u16, usize, usize),
         cache: &CachePlanes, block_table: (*const i32, usize, usize), request_rows: *const i32,
         workspace: *mut core::ffi::c_void, output: *mut u16,
     ) -> GpuResult<()> {
@@ -540,7 +540,8 @@ impl AttentionOp {
             ffi::tk100_paged_attention(
                 self.ctx.raw, stream.cu_stream().cast(), rows_i32(sequences), rows_i32(tokens),
                 rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, kv_lengths,
-                query, gate, rows_i32(q_strides.0), rows_i32(q_strides.1), cache.key, cache.value,
+                query.0, gate.0, rows_i32(query.1), rows_i32(query.2), rows_i32(gate.1),
+                rows_i32(gate.2), cache.key, cache.value,
                 rows_i32(cache.pages), rows_i32(cache.page_tokens), rows_i32(cache.page_stride),
                 rows_i32(cache.token_stride), rows_i32(cache.head_stride), block_table.0,
                 rows_i32(block_table.1), rows_i32(block_table.2), request_rows, self.scale,
@@ -549,11 +550,11 @@ impl AttentionOp {
         })
     }
 
-    /// `tk100_prompt_attention`.
+    /// `tk100_prompt_attention`; `query` and `gate` as above.
     #[allow(clippy::too_many_arguments)]
     pub unsafe fn launch_prompt(
         &self, stream: &CudaStream, sequences: usize, tokens: usize, starts: *const i32,
-        query: *const u16, gate: *const u16, q_strides: (usize, usize), key: *const u16,
+        query: (*const u16, usize, usize), gate: (*const u16, usize, usize), key: *const u16,
         value: *const u16, kv_strides: (usize, usize), workspace: *mut core::ffi::c_void,
         output: *mut u16,
     ) -> GpuResult<()> {
@@ -561,8 +562,8 @@ impl AttentionOp {
         self.ctx.check(unsafe {
             ffi::tk100_prompt_attention(
                 self.ctx.raw, stream.cu_stream().cast(), rows_i32(sequences), rows_i32(tokens),
-                rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, query, gate,
-                rows_i32(q_strides.0), rows_i32(q_strides.1), key, value, rows_i32(kv_strides.0),
+                rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, query.0, gate.0,
+                rows_i32(query.1), rows_i32(query.2), rows_i32(gate.1), rows_i32(gate.2), key, value, rows_i32(kv_strides.0),
                 rows_i32(kv_strides.1), self.scale, workspace, output,
             )
         })

@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define TK100_ABI_VERSION 1
+#define TK100_ABI_VERSION 2
 
 #if defined(__GNUC__)
 #define TK100_API __attribute__((visibility("default")))
@@ -541,8 +541,8 @@ TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_
  * its block table row (request_rows[s], or s when that is NULL), the new tokens' own included; with q new
  * tokens over k keys token i sees keys 0 .. k - q + i.  A token that sees none gets zeros.
  *   output[token][head] = softmax(scale * q . K) V, times sigmoid(gate[token][head]) when gate is given
- * (the queries' strides).  output is [tokens, q_heads, head_dim] and starts on 32 bytes; rows outside the sequences are left as
- * they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
+ * (with strides of its own: where the projection left it, next to queries rotated elsewhere).  output is [tokens,
+ * q_heads, head_dim] and starts on 32 bytes; rows outside the sequences are left as they were.  Lengths outside the planes are cut to them, and pages outside the cache read as zeros; both
  * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used,
  * whatever it is.  The output overlaps nothing that is read.  Weights times values are summed in FP32, with weights
  * of up to 2^8, in front of the division by the weights' sum; a sigmoid below 2^-126 (a gate below -87.3) counts as
@@ -552,18 +552,19 @@ TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream
                                              int q_heads, int kv_heads, int head_dim, const int32_t* starts,
                                              const int32_t* kv_lengths, const uint16_t* query,
                                              const uint16_t* gate, int query_token_stride,
-                                             int query_head_stride, const uint16_t* key_cache,
-                                             const uint16_t* value_cache, int pages, int page_tokens,
-                                             int page_stride, int cache_token_stride, int cache_head_stride,
-                                             const int32_t* block_table, int table_rows, int max_pages,
-                                             const int32_t* request_rows, float scale, void* workspace,
-                                             uint16_t* output);
+                                             int query_head_stride, int gate_token_stride, int gate_head_stride,
+                                             const uint16_t* key_cache, const uint16_t* value_cache, int pages,
+                                             int page_tokens, int page_stride, int cache_token_stride,
+                                             int cache_head_stride, const int32_t* block_table, int table_rows,
+                                             int max_pages, const int32_t* request_rows, float scale,
+                                             void* workspace, uint16_t* output);
 
 /* The same over whole prompts packed one behind the other: keys and values are rows of the same tokens. */
 TK100_API tk100_status tk100_prompt_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
                                               int q_heads, int kv_heads, int head_dim, const int32_t* starts,
                                               const uint16_t* query, const uint16_t* gate,
                                               int query_token_stride, int query_head_stride,
+                                              int gate_token_stride, int gate_head_stride,
                                               const uint16_t* key, const uint16_t* value, int kv_token_stride,
                                               int kv_head_stride, float scale, void* workspace,
                                               uint16_t* output);

@@ -13,7 +13,7 @@ import warnings
 
 from . import build as _build
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 STATUS_NAMES = {0: "ok", 1: "gpu.driver", 2: "gpu.arena", 3: "gpu.graph", 4: "gpu.context",
                 5: "gpu.launch", 6: "gpu.module"}
@@ -93,9 +93,9 @@ SIGNATURES = {
     "tk100_rotary_cache": (_i, [_vp, _vp] + [_i] * 6 + [_vp] * 4 + [_i] * 2 + [_vp] * 2 + [_i] * 2 + [_vp] * 6
                            + [_i] * 5 + [_vp]),
     "tk100_attention_workspace_bytes": (C.c_size_t, [_vp, _i]),
-    "tk100_paged_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 4 + [_i] * 2 + [_vp] * 2 + [_i] * 5
+    "tk100_paged_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 4 + [_i] * 4 + [_vp] * 2 + [_i] * 5
                               + [_vp, _i, _i, _vp, C.c_float, _vp, _vp]),
-    "tk100_prompt_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 3 + [_i] * 2 + [_vp] * 2 + [_i] * 2
+    "tk100_prompt_attention": (_i, [_vp, _vp] + [_i] * 5 + [_vp] * 3 + [_i] * 4 + [_vp] * 2 + [_i] * 2
                                + [C.c_float, _vp, _vp]),
     "tk100_fp8_projection_static": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, C.c_char_p,
                                          C.c_size_t]),

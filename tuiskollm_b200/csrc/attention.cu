@@ -475,8 +475,8 @@ __device__ __forceinline__ void store_words8(uint16_t* to, const uint32_t* w) {
 
 // Rows of a tile whose first token row is `token`.
 __device__ __forceinline__ const uint16_t* gate_row(const AttentionParams& p, int token, int head, int row) {
-  return p.gate + static_cast<size_t>(token + row / p.group) * p.query_token_stride +
-         static_cast<size_t>(head * p.group + row % p.group) * p.query_head_stride;
+  return p.gate + static_cast<size_t>(token + row / p.group) * p.gate_token_stride +
+         static_cast<size_t>(head * p.group + row % p.group) * p.gate_head_stride;
 }
 template <int D>
 __device__ __forceinline__ uint16_t* output_row(const AttentionParams& p, int token, int head, int row) {

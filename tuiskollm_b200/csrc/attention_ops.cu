@@ -270,15 +270,19 @@ Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, 
   TK100_TRY(plane(ctx_, what, "value", value, 16));
   TK100_TRY(plane(ctx_, what, "output", p->output, 32));
   TK100_TRY(plane(ctx_, what, "workspace", workspace, 16));
-  if (p->gate) TK100_TRY(plane(ctx_, what, "gate", p->gate, 16));
   TK100_TRY(stride(ctx_, what, "query token", p->query_token_stride, head_dim));
   TK100_TRY(stride(ctx_, what, "query head", p->query_head_stride, head_dim));
+  if (p->gate) {
+    TK100_TRY(plane(ctx_, what, "gate", p->gate, 16));
+    TK100_TRY(stride(ctx_, what, "gate token", p->gate_token_stride, head_dim));
+    TK100_TRY(stride(ctx_, what, "gate head", p->gate_head_stride, head_dim));
+  }
   if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse(ctx_, what, "the scale must be positive and finite");
   const Span out(p->output, p->tokens, static_cast<long long>(p->q_heads) * head_dim, p->q_heads, head_dim, head_dim);
   const Span in(query, p->tokens, p->query_token_stride, p->q_heads, p->query_head_stride, head_dim);
   if (out.meets(in)) return refuse(ctx_, what, "the output overlaps the queries");
   if (p->gate) {
-    const Span gate(p->gate, p->tokens, p->query_token_stride, p->q_heads, p->query_head_stride, head_dim);
+    const Span gate(p->gate, p->tokens, p->gate_token_stride, p->q_heads, p->gate_head_stride, head_dim);
     if (out.meets(gate)) return refuse(ctx_, what, "the output overlaps the gate");
   }
   p->group = p->q_heads / p->kv_heads;

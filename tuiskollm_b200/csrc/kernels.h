@@ -444,7 +444,7 @@ struct AttentionParams {
   int table_row_count, max_pages, page_shift, pages;
   float scale_log2;  // scale * log2(e)
   const uint16_t* gate;
-  int query_token_stride, query_head_stride;
+  int query_token_stride, query_head_stride, gate_token_stride, gate_head_stride;
   uint16_t* output;
   float* parts;        // [2 per CTA][head_dim / 4][128 rows][4]
   float2* part_stats;  // [2 per CTA][128 rows]

@@ -2051,10 +2051,11 @@ size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_dim) {
 tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens, int q_heads,
                                    int kv_heads, int head_dim, const int32_t* starts, const int32_t* kv_lengths,
                                    const uint16_t* query, const uint16_t* gate, int query_token_stride,
-                                   int query_head_stride, const uint16_t* key_cache, const uint16_t* value_cache,
-                                   int pages, int page_tokens, int page_stride, int cache_token_stride,
-                                   int cache_head_stride, const int32_t* block_table, int table_rows, int max_pages,
-                                   const int32_t* request_rows, float scale, void* workspace, uint16_t* output) {
+                                   int query_head_stride, int gate_token_stride, int gate_head_stride,
+                                   const uint16_t* key_cache, const uint16_t* value_cache, int pages, int page_tokens,
+                                   int page_stride, int cache_token_stride, int cache_head_stride,
+                                   const int32_t* block_table, int table_rows, int max_pages, const int32_t* request_rows,
+                                   float scale, void* workspace, uint16_t* output) {
   if (!ctx) return TK100_ERR_CONTEXT;
   tk100::AttentionParams p{};
   p.sequences = sequences;
@@ -2070,6 +2071,8 @@ tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequ
   p.gate = gate;
   p.query_token_stride = query_token_stride;
   p.query_head_stride = query_head_stride;
+  p.gate_token_stride = gate_token_stride;
+  p.gate_head_stride = gate_head_stride;
   p.output = output;
   return tk100::AttentionOp(*ctx->impl)
       .paged(static_cast<cudaStream_t>(stream), head_dim, p, query, key_cache, value_cache,
@@ -2079,8 +2082,9 @@ tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequ
 tk100_status tk100_prompt_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens, int q_heads,
                                     int kv_heads, int head_dim, const int32_t* starts, const uint16_t* query,
                                     const uint16_t* gate, int query_token_stride, int query_head_stride,
-                                    const uint16_t* key, const uint16_t* value, int kv_token_stride,
-                                    int kv_head_stride, float scale, void* workspace, uint16_t* output) {
+                                    int gate_token_stride, int gate_head_stride, const uint16_t* key,
+                                    const uint16_t* value, int kv_token_stride, int kv_head_stride, float scale,
+                                    void* workspace, uint16_t* output) {
   if (!ctx) return TK100_ERR_CONTEXT;
   tk100::AttentionParams p{};
   p.sequences = sequences;
@@ -2091,6 +2095,8 @@ tk100_status tk100_prompt_attention(tk100_ctx* ctx, tk100_stream stream, int seq
   p.gate = gate;
   p.query_token_stride = query_token_stride;
   p.query_head_stride = query_head_stride;
+  p.gate_token_stride = gate_token_stride;
+  p.gate_head_stride = gate_head_stride;
   p.output = output;
   return tk100::AttentionOp(*ctx->impl)
       .prompt(static_cast<cudaStream_t>(stream), head_dim, p, query, key, value, kv_token_stride, kv_head_stride, scale,

@@ -586,12 +586,10 @@ class _AttentionOp:
     def _rows(self, sequences, starts, query, gate, workspace, output):
         c, dim = self.ctx, self.head_dim
         q, qs, tokens = _heads(c, query, "query", -1, self.q_heads, dim)
-        g = None
+        g, gs = None, (0, 0)
         if gate is not None:
             g, gs, _ = _heads(c, gate, "gate", tokens, self.q_heads, dim)
-            if gs != qs:
-                raise GpuError(5, f"[gpu.launch] query and gate have different strides {qs} and {gs}")
-        return (tokens, q, g, qs, _plane(c, starts, "starts", torch.int32, sequences + 1),
+        return (tokens, q, g, (qs[0], qs[1], gs[0], gs[1]), _plane(c, starts, "starts", torch.int32, sequences + 1),
                 _plane(c, workspace, "workspace", torch.uint8, self._workspace_bytes),
                 _head_rows(c, output, "output", tokens, self.q_heads, dim))
 
@@ -602,8 +600,8 @@ class PagedAttentionOp(_AttentionOp):
     heads of 128 and up to 128 query heads per key/value head are admitted.
 
     ``launch``: ``starts`` int32 ``[sequences + 1]`` rows of ``query`` ``[tokens, q_heads, head_dim]``; ``kv_lengths`` int32
-    ``[sequences]`` keys of each, its new ones included; ``gate`` None or a plane with the query's strides whose sigmoid
-    multiplies the output; ``block_table`` int32 ``[rows, pages per row]`` with row ``request_rows[s]`` (None: s)."""
+    ``[sequences]`` keys of each, its new ones included; ``gate`` None or a plane of the query's shape, of any
+    token and head strides, whose sigmoid multiplies the output; ``block_table`` int32 ``[rows, pages per row]`` with row ``request_rows[s]`` (None: s)."""
 
     def launch(self, stream, sequences, starts, kv_lengths, query, gate, key_cache, value_cache, block_table,
                request_rows, workspace, output):
@@ -613,7 +611,7 @@ class PagedAttentionOp(_AttentionOp):
         rows, row_pages = _block_table(block_table)
         c._native.tk100_paged_attention(
             c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,
-            _plane(c, kv_lengths, "key lengths", torch.int32, sequences), q, g, qs[0], qs[1], key, value, pages,
+            _plane(c, kv_lengths, "key lengths", torch.int32, sequences), q, g, *qs, key, value, pages,
             page_tokens, cs[0], cs[1], cs[2], _plane(c, block_table, "block table", torch.int32, 1),
             rows, row_pages,
             None if request_rows is None else _plane(c, request_rows, "request rows", torch.int32, sequences),
@@ -632,7 +630,7 @@ class PromptAttentionOp(_AttentionOp):
         if vs != ks:
             raise GpuError(5, f"[gpu.launch] key and value have different strides {ks} and {vs}")
         c._native.tk100_prompt_attention(c, stream, sequences, tokens, self.q_heads, self.kv_heads, self.head_dim, at,
-                                         q, g, qs[0], qs[1], k, v, ks[0], ks[1], self.scale, work, out)
+                                         q, g, *qs, k, v, ks[0], ks[1], self.scale, work, out)
 
 
 class LmHeadOp:

@@ -50,7 +50,7 @@ SUITES = {
     "page-plan": ["tests/test_gpu_paging.py", "tests/test_gpu_paging_bad_pages.py"],
     "rotary-cache": ["tests/test_gpu_rotary.py", "tests/test_gpu_rotary_many.py"],
     "attention": ["tests/test_gpu_attention.py", "tests/test_gpu_attention_gates.py", "tests/test_gpu_attention_planes.py",
-                  "tests/test_gpu_attention_joins.py",
+                  "tests/test_gpu_attention_joins.py", "tests/test_gpu_attention_gate_planes.py",
                   "tests/test_gpu_full_attention_step.py"],
     "peer-exchange": ["tests/test_gpu_peer_sum.py", "tests/test_gpu_multi.py"],
     "static-entry": ["tests/test_zz_no_alloc.py"],

@@ -257,7 +257,8 @@ unsafe extern "C" {
         kv_lengths: *const i32, query: *const u16, gate: *const u16, query_token_stride: c_int,
         query_head_stride: c_int, gate_token_stride: c_int, gate_head_stride: c_int,
         key_cache: *const u16, value_cache: *const u16, pages: c_int, page_tokens: c_int,
-        page_stride: c_int, cache_token_stride: c_int, cache_head_stride: c_int, block_table: *const i32, table_rows: c_int, max_pages: c_int,
+        page_stride: c_int, cache_token_stride: c_int, cache_head_stride: c_int,
+        block_table: *const i32, table_rows: c_int, max_pages: c_int,
         request_rows: *const i32, scale: f32, workspace: *mut c_void, output: *mut u16,
     ) -> Tk100Status;
     pub fn tk100_prompt_attention(
@@ -265,6 +266,7 @@ unsafe extern "C" {
         q_heads: c_int, kv_heads: c_int, head_dim: c_int, starts: *const i32,
         query: *const u16, gate: *const u16, query_token_stride: c_int,
         query_head_stride: c_int, gate_token_stride: c_int, gate_head_stride: c_int,
-        key: *const u16, value: *const u16, kv_token_stride: c_int, kv_head_stride: c_int, scale: f32, workspace: *mut c_void, output: *mut u16,
+        key: *const u16, value: *const u16, kv_token_stride: c_int, kv_head_stride: c_int,
+        scale: f32, workspace: *mut c_void, output: *mut u16,
     ) -> Tk100Status;
 }

@@ -563,7 +563,8 @@ impl AttentionOp {
             ffi::tk100_prompt_attention(
                 self.ctx.raw, stream.cu_stream().cast(), rows_i32(sequences), rows_i32(tokens),
                 rows_i32(q_heads), rows_i32(kv_heads), rows_i32(head_dim), starts, query.0, gate.0,
-                rows_i32(query.1), rows_i32(query.2), rows_i32(gate.1), rows_i32(gate.2), key, value, rows_i32(kv_strides.0),
+                rows_i32(query.1), rows_i32(query.2), rows_i32(gate.1), rows_i32(gate.2), key,
+                value, rows_i32(kv_strides.0),
                 rows_i32(kv_strides.1), self.scale, workspace, output,
             )
         })

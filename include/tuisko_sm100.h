@@ -546,8 +546,9 @@ TK100_API size_t tk100_attention_workspace_bytes(const tk100_ctx* ctx, int head_
  * are reported as TK100_DEVICE_BAD_ARGUMENT.  What the cache holds behind a sequence's keys is not used,
  * whatever it is.  The output overlaps nothing that is read.  Weights times values are summed in FP32, with weights
  * of up to 2^8, in front of the division by the weights' sum; a sigmoid below 2^-126 (a gate below -87.3) counts as
- * zero.  A key or value of the sequence itself that is not finite reaches the tokens that see it, and through
- * 0 * NaN may reach those up to 127 positions in front of it. */
+ * zero.  A key or value of the sequence itself that is not finite reaches the tokens that see it; through 0 * NaN
+ * such a value may also reach tokens in front of it, up to 2 * floor(128 / (q_heads / kv_heads)) - 1 positions away
+ * (255 with a key/value head per query head). */
 TK100_API tk100_status tk100_paged_attention(tk100_ctx* ctx, tk100_stream stream, int sequences, int tokens,
                                              int q_heads, int kv_heads, int head_dim, const int32_t* starts,
                                              const int32_t* kv_lengths, const uint16_t* query,

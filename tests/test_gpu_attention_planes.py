@@ -172,3 +172,23 @@ def test_caches_in_one_plane_are_taken(ctx, calls, order):
     assert ctx.device_status() == 0
     assert torch.equal(pick(0)[0, :5], calls.k_out) and torch.equal(pick(1)[0, :5], calls.value)
     assert int(both.count_nonzero()) == int(calls.k_out.count_nonzero()) + int(calls.value.count_nonzero())
+
+
+def test_a_value_that_is_no_number_reaches_its_tile_at_most(ctx):
+    """It reaches the tokens that see it, and no token more than 2 * floor(128 / queries of a key/value head) - 1 in front
+    of it; a key that is none no token in front of it at all."""
+    for q_heads, reach in ((1, 255), (6, 41)):
+        tokens, at = 700, 511
+        query, key, value = normal(1, tokens, q_heads, 128), normal(2, tokens, 1, 128), normal(3, tokens, 1, 128)
+        op = tk.PromptAttentionOp(ctx, q_heads, 1, 128)
+        clean, out, work = torch.zeros_like(query), torch.zeros_like(query), op.workspace()
+        op.launch(None, 1, ints([0, tokens]), query, None, key, value, work, clean)
+        broken = value.clone()
+        broken[at] = float("nan")
+        op.launch(None, 1, ints([0, tokens]), query, None, key, broken, work, out)
+        assert bool(out[at:].isnan().all()) and torch.equal(out[:at - reach], clean[:at - reach])
+        broken = key.clone()
+        broken[at] = float("nan")
+        op.launch(None, 1, ints([0, tokens]), query, None, broken, value, work, out)
+        assert bool(out[at:].isnan().all()) and torch.equal(out[:at], clean[:at])
+    assert ctx.device_status() == 0

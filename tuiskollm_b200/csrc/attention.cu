@@ -277,7 +277,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& p, const Sequence
 
 // The pair's even cuts; returns the keys of a pair.
 __device__ __forceinline__ long long even_cuts(const AttentionParams& p, long long total, long long (&cuts)[2]) {
-  const long long share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), static_cast<long long>(p.min_steps) * kKeys);
+  const long long share = max(divide(total + gridDim.x / 2 - 1, gridDim.x / 2), static_cast<long long>(kKeys));
   cuts[0] = min(static_cast<long long>(blockIdx.x / 2) * share, total);
   cuts[1] = min(cuts[0] + share, total);
   return share;
@@ -502,8 +502,8 @@ __device__ __forceinline__ F32x2 gated(F32x2 v, uint32_t gate) {
   return mul2(v, f32x2(a, b));
 }
 
-// Joins the parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left, in the order of their keys.
-// Parts are [four values][128 rows][4], so that threads next to each other have rows next to each other.
+// Parts of a tile's rows that this CTA and its likes in pairs c0 .. c1 left are joined in the order of their keys.
+// A part is [four values][128 rows][4], so that threads next to each other have rows next to each other.
 __device__ __forceinline__ size_t part_slot(int k, int c0, int rank) {
   return 2 * static_cast<size_t>(2 * k + rank) + (k == c0 ? 1 : 0);
 }
@@ -512,7 +512,7 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 }
 
 // Loads past L1 that stay where they are written: left to itself the compiler moves each of them into the branch
-// that uses it, and a join of 19 parts waits for L2 60 times instead of 4.
+// that uses it, and a join of 18 parts waits for L2 60 times instead of 4.
 __device__ __forceinline__ float4 load_part(const float4* p) {
   float4 v;
   asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
@@ -567,10 +567,13 @@ __device__ __forceinline__ void join_stats(const AttentionParams& p, int c0, int
   named_barrier(1, 128);
 }
 
-// The rows: a thread has four of a row's values at PLACES places, and their loads of PARTS parts under way together.
-template <int D, int PLACES, int PARTS>
+// The rows: a thread has four of a row's values at three places, and their loads of five parts under way together (four
+// places and two parts are slower even where there are no more parts: six decoded tokens 41.6 us, not 41.1, twelve 65.3
+// and 63.9).
+template <int D>
 __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int c1, int rank, int rows, int thread, int ahead,
                                           int token, int head, const float* row_top, const float* row_scale) {
+  constexpr int PLACES = 3, PARTS = 5;
   const int places = rows * (D / 4);
 #pragma unroll 1
   for (int base = thread; base < places; base += 128 * PLACES) {
@@ -634,8 +637,6 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, int c0, int 
     }
   }
 }
-
-// ------------------------------------------------------------------------- the kernel
 
 // The same where there are many rows: a thread has one, 16 of its values at a time, and the loads of two parts of them
 // under way together.
@@ -701,6 +702,8 @@ __device__ __forceinline__ void join_tall(const AttentionParams& p, int c0, int 
     if (thread < rows) store_words8(out + 4 * quad, w);
   }
 }
+
+// ------------------------------------------------------------------------- the kernel
 
 // Barriers that both CTAs' loads or threads arrive on are the even CTA's (full, q_full, p_full, o_free); those that
 // the even CTA's MMA warp commits to are arrived on in both (empty, q_empty, s_full, pv_done, o_full).
@@ -1316,17 +1319,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ctl.last_part) {
           __threadfence();
           // row_max and row_sum have been read by their rows' threads: here they hold what the parts have in common
-          if (c1 - c0 < 8) {
-            join_stats<1>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
-          } else {
+          // What is faster, us of a launch at 24 over 4 heads of 256.  Eight lanes a row / one: 6 rows in 72 parts 33.5 / 40.1,
+          // in 18 parts 20.9 / 22.6, 48 rows 61.7 / 63.0, 72 81.8 / 82.5, 90 100.4 / 99.9, 126 121.3 / 117.1; in 4 parts 54
+          // rows 60.5 / 58.7, 90 69.8 / 65.6.  Rows by all threads / a thread each: 18 parts of 54 rows 69 / 111, of 96 97 /
+          // 107, of 108 114 / 117, of 126 127 / 118; 12 parts of 90 66.9 / 69.8, of 108 64.2 / 62.6; 6 parts of 72 57.9 / 60.9,
+          // of 90 68.8 / 64.4; 4 parts of 72 62.7 / 63.5, of 90 70.6 / 66.0; 2 parts of 54 84.8 / 90.1, of 72 90.6 / 89.8.
+          const bool many = c1 - c0 >= 8;
+          if (many && rows <= 72) {
             join_stats<8>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
-          }
-          if (rows > 48) {
-            join_tall<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
-          } else if (c1 - c0 < 2) {
-            join_rows<D, 4, 2>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           } else {
-            join_rows<D, 3, 5>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
+            join_stats<1>(p, c0, c1, rank, rows, thread, ctl.row_max[0], ctl.row_sum[0]);
+          }
+          if (rows > (many ? 96 : 72)) {
+            join_tall<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
+          } else {
+            join_rows<D>(p, c0, c1, rank, rows, thread, ahead, tile_token, it.head, ctl.row_max[0], ctl.row_sum[0]);
           }
           if (thread == 0) *ticket = 0u;
         }

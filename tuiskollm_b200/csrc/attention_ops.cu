@@ -289,10 +289,10 @@ Status AttentionOp::prepare(const char* what, int head_dim, AttentionParams* p, 
   p->half_tokens = kAttentionRows / p->group;
   p->tile_tokens = 2 * p->half_tokens;
   p->scale_log2 = scale * 1.4426950408889634f;
-  p->min_steps = 1;
   // A tile's first scores and last rows, in keys of the line: too little gives pairs with many short tiles more than
-  // their share, too much less.  256 / 384 / 512 / 640 at heads of 256, a prompt of 8192 tokens: 707 / 675 / 655 / 645 us;
-  // 128 / 176 / 224 / 300 / 400 at 128, seven packed prompts: 124 / 116 / 110 / 111 / 114.
+  // their share, too much less.  480 / 608 / 768 at heads of 256, us: a prompt of 8192 tokens 753 / 732 / 741, seven packed
+  // prompts 111 / 115 / 122, a decode batch of 32 203 / 193 / 190 (its tiles' ends cost more than this line says); 192 / 256 / 320 at
+  // 128: seven packed prompts 90 / 89 / 91, nine mixed chunks 60 / 60 / 60.  256 at heads of 256 707 for the first.
   p->tile_keys = head_dim == 256 ? 608 : 256;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   const size_t rows = 2 * static_cast<size_t>(ctx_.sm_count()) * kAttentionRows;

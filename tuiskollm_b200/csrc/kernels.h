@@ -434,7 +434,6 @@ cudaError_t launch_rotary(cudaStream_t stream, int dim, const RotaryParams& p);
 struct AttentionParams {
   int sequences, tokens, q_heads, kv_heads, group;
   int half_tokens, tile_tokens;  // tokens of the rows of one CTA, of both
-  int min_steps;               // 128-key steps that a pair takes at least
   int tile_keys;               // what a tile costs besides its keys, in keys
   const int32_t* starts;       // [sequences + 1]
   const int32_t* kv_lengths;   // null: as many keys as new tokens

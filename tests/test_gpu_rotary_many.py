@@ -1,4 +1,4 @@
-"""Rotary positions of a thousand tokens and more, where a CTA has four of them, against their 64-bit form."""
+"""Rotary positions of thousands of tokens, where a CTA may have four of them, against their 64-bit form."""
 import pytest
 import torch
 
@@ -15,9 +15,11 @@ def ctx():
     return tk.Context()
 
 
-# whole CTAs, one to three tokens in the last; more heads than a CTA takes in one round (16 x 4 of 128 values, 8 x 4 of 256)
-@pytest.mark.parametrize("tokens", [1023, 1024, 1025, 1026, 1027, 2311])
-@pytest.mark.parametrize("heads,rotary,axes", [((24, 4, 256), 64, 3), ((64, 8, 128), 128, 1), ((3, 1, 128), 48, 2), ((40, 2, 256), 256, 1)])
+# Up to 2047 tokens a CTA has one; from then on four (whole CTAs, one to three tokens in the last) where the heads of
+# queries, keys and values are one round of a CTA's at most, 64 of 128 values or 32 of 256, with norms half of one.
+@pytest.mark.parametrize("tokens", [1027, 2047, 2048, 2049, 2050, 2051])
+@pytest.mark.parametrize("heads,rotary,axes", [((24, 4, 256), 64, 3), ((48, 8, 128), 128, 1), ((56, 8, 128), 64, 1), ((3, 1, 128), 48, 2),
+                                               ((12, 2, 256), 128, 3), ((16, 8, 128), 16, 1), ((40, 2, 256), 256, 1)])
 @pytest.mark.parametrize("norm", [False, True])
 def test_rotation_and_store(ctx, tokens, heads, rotary, axes, norm):
     q_heads, kv_heads, dim = heads
@@ -48,10 +50,10 @@ def test_rotation_and_store(ctx, tokens, heads, rotary, axes, norm):
         assert bool((c[others].view(torch.uint8) == SENTINEL).all()), "slots of no token were written"
 
 
-@pytest.mark.parametrize("heads", [(6, 2, 256), (72, 2, 128)])
+@pytest.mark.parametrize("heads", [(6, 2, 256), (30, 2, 128), (72, 2, 128)])
 def test_in_place_and_replay(ctx, heads):
     q_heads, kv_heads, dim = heads
-    tokens = 1501
+    tokens = 2501
     g = torch.Generator().manual_seed(2)
     query, key = (torch.randn(tokens, h, dim, generator=g).bfloat16().cuda() for h in (q_heads, kv_heads))
     positions = torch.arange(tokens, dtype=torch.int32, device="cuda")
@@ -75,12 +77,12 @@ def test_in_place_and_replay(ctx, heads):
 
 def test_one_and_four_tokens_a_cta_agree(ctx):
     """A token's result does not depend on how many others are rotated with it."""
-    tokens = 1030
-    query, key, value = planes(tokens, 24, 4, 256, True, 4)
+    tokens, heads, dim = 2060, (14, 2), 256
+    query, key, value = planes(tokens, *heads, dim, True, 4)
     positions = torch.arange(tokens, dtype=torch.int32, device="cuda") * 177
-    op = tk.RotaryCacheOp(ctx, 24, 4, 256, tk.rotary_frequencies(64, 1e7))
-    weights = [torch.randn(256, generator=torch.Generator().manual_seed(s)).mul(0.1).bfloat16().cuda() for s in (1, 2)]
-    whole = [torch.zeros(tokens, h, 256, dtype=torch.bfloat16, device="cuda") for h in (24, 4)]
+    op = tk.RotaryCacheOp(ctx, *heads, dim, tk.rotary_frequencies(64, 1e7))
+    weights = [torch.randn(dim, generator=torch.Generator().manual_seed(s)).mul(0.1).bfloat16().cuda() for s in (1, 2)]
+    whole = [torch.zeros(tokens, h, dim, dtype=torch.bfloat16, device="cuda") for h in heads]
     op.launch(None, tokens, positions, query, key, None, *weights, *whole, None, None, None)
     part = [torch.zeros_like(t) for t in whole]
     for a in range(0, tokens, 515):

@@ -13,8 +13,17 @@
 // A CTA has TOKENS tokens: its threads form their sines and cosines once for all heads while every thread already
 // holds DEPTH heads' values; a head is DIM / 8 lanes of 16 bytes, so the partner of a lane in a rotation is R / 16
 // lanes away and comes by shuffle.  One token a CTA leaves most threads idle in the first half and has its chain of
-// loads, angles and stores to itself; four share it: 8192 tokens of 32 + 8 heads of 128 57 us with one, 48.5 with four
-// (4.1 TB/s), 777 tokens of 24 + 4 heads of 256 8.9 with one, 11 with four, so four from 1024 tokens on.
+// loads, angles and stores to itself; four share it, at half of the CTAs an SM, which pays where the loop over heads is
+// short: without norms and within one round of heads, or with norms within half of one.  us with one / with four, all with
+// cache stores:
+//                                 tokens      1024       1536       2048       4096       8192
+//   32 + 8 + 8 heads of 128             9.0/ 7.9  12.6/13.8  16.0/14.4  28.6/27.2  53.8/47.7
+//   the same with norms                10.8/10.5  15.3/18.6  19.6/19.4  35.1/36.5  66.5/63.9
+//   24 + 4 + 4 of 256, 64 turned        8.9/ 8.6  12.3/14.2  15.7/15.5  28.1/28.6  52.5/51.5
+//   the same with norms                11.5/12.1  16.1/21.4  20.2/22.5  35.9/41.6  67.1/73.3
+//   64 + 8 + 8 of 128 (two rounds)     11.8/11.7  16.1/19.9  20.3/21.4  36.4/40.4  68.6/72.6
+//   8 + 2 + 2 of 128 with norms         7.5/ 6.6  10.4/11.8  13.4/12.1  23.4/22.7  44.7/39.6
+//   8 + 1 + 1 of 256 with norms         8.8/ 8.7  12.2/15.3  15.7/15.9  27.9/29.5  53.8/51.9
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
@@ -23,13 +32,14 @@ namespace tk100 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRotaryManyTokens = 1024;
+constexpr int kDepth = 4;  // heads of a thread in one round
+constexpr int kRotaryManyTokens = 2048;
 
 template <int DIM, int TOKENS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   constexpr int LANES = DIM / 8;             // lanes of a head
   constexpr int AT_ONCE = kThreads / LANES;  // heads of a CTA side by side
-  constexpr int DEPTH = 4;                   // and one behind the other, all of them requested at once
+  constexpr int DEPTH = kDepth;              // and one behind the other, all of them requested at once
   __shared__ float2 turn[TOKENS][DIM / 2];
   __shared__ long long places[TOKENS];  // of the tokens in the cache, -1: nowhere
   pdl_wait();
@@ -182,7 +192,9 @@ cudaError_t launch(cudaStream_t stream, int dim, const RotaryParams& p) {
 }  // namespace
 
 cudaError_t launch_rotary(cudaStream_t stream, int dim, const RotaryParams& p) {
-  return p.tokens >= kRotaryManyTokens ? launch<4>(stream, dim, p) : launch<1>(stream, dim, p);
+  const int heads = p.q_heads + p.kv_heads + (p.key_cache ? p.kv_heads : 0), round = kDepth * (kThreads * 8 / dim);
+  const bool four = p.tokens >= kRotaryManyTokens && heads <= (p.query_norm || p.key_norm ? round / 2 : round);
+  return four ? launch<4>(stream, dim, p) : launch<1>(stream, dim, p);
 }
 
 }  // namespace tk100

@@ -33,12 +33,12 @@
 // and stores.  Pairs begin with such tiles, so that joins run beside whole ones.  The lengths stay on the device:
 // every CTA sums the costs up for itself, in closed form, so a captured launch follows them.
 //
-// Measured (B200 at 1.65 to 1.9 GHz), us: prompt of 8192 tokens, 24 heads over 4 of 256, gated, 645 to 703 by the clock
-// (1.17 to 1.28 PFLOP/s, 0.70 to 0.77 of cuBLAS' BF16 burst rate); seven packed prompts of up to 1777, 32 over 8 of
-// 128, 110 to 117; decode batch of 32 over up to 16384 keys 190 to 210 (849 MB: 0.62 to 0.68 of the copy rate); 512
-// tokens over 16000 keys 214 to 221; one token over 4096 keys 21.6.  A step takes 2400 cycles at heads of 256, where the MMAs take 2048, and 1600 at 128 (1024, of
-// which the exponentials take 1024 too): the chain scores -> softmax -> values of a step, with one buffer of S per
-// warpgroup, bounds both.
+// Measured (B200 at 1.65 to 1.9 GHz), us: prompt of 8192 tokens, 24 heads over 4 of 256, gated, 645 to 711 by the clock
+// (1.16 to 1.28 PFLOP/s, 0.69 to 0.77 of cuBLAS' BF16 burst rate); seven packed prompts of up to 1777, 32 over 8 of
+// 128, 110 to 117; decode batch of 32 over up to 16384 keys 190 to 214 (849 MB: 0.6 to 0.68 of the copy rate); 512
+// tokens over 16000 keys 214 to 221; one token over 4096 keys 21.  A step takes 2400 cycles at heads of 256, where the
+// MMAs take 2048, and 1600 at 128 (1024, of which the exponentials take 1024 too): the chain scores -> softmax -> values of
+// a step, with one buffer of S per warpgroup, bounds both.
 #include <cuda_fp16.h>
 
 #include <new>

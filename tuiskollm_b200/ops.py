@@ -537,8 +537,8 @@ class RotaryCacheOp:
                key_cache, value_cache, slots):
         """``query`` ``[>= tokens, q_heads, head_dim]``, ``key`` and ``value`` ``[>= tokens, kv_heads, head_dim]`` with any
         token and head strides (views of the projection's rows); ``positions`` int32 ``[axes, tokens]`` (or with
-        extents of one between) or ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output`` dense or None; caches
-        ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
+        extents of one between) or ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output``
+        dense or None; caches ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
         c, dim = self.ctx, self.head_dim
         q, qs, q_rows = _heads(c, query, "query", -1, self.q_heads, dim)
         k, ks, rows = _heads(c, key, "key", -1, self.kv_heads, dim)
@@ -601,7 +601,8 @@ class PagedAttentionOp(_AttentionOp):
 
     ``launch``: ``starts`` int32 ``[sequences + 1]`` rows of ``query`` ``[tokens, q_heads, head_dim]``; ``kv_lengths`` int32
     ``[sequences]`` keys of each, its new ones included; ``gate`` None or a plane of the query's shape, of any
-    token and head strides, whose sigmoid multiplies the output; ``block_table`` int32 ``[rows, pages per row]`` with row ``request_rows[s]`` (None: s)."""
+    token and head strides, whose sigmoid multiplies the output; ``block_table`` int32 ``[rows, pages per row]`` with
+    row ``request_rows[s]`` (None: s)."""
 
     def launch(self, stream, sequences, starts, kv_lengths, query, gate, key_cache, value_cache, block_table,
                request_rows, workspace, output):

@@ -538,7 +538,8 @@ class RotaryCacheOp:
         """``query`` ``[>= tokens, q_heads, head_dim]``, ``key`` and ``value`` ``[>= tokens, kv_heads, head_dim]`` with any
         token and head strides (views of the projection's rows); ``positions`` int32 ``[axes, tokens]`` (or with
         extents of one between) or ``[tokens]``; norms ``[head_dim]`` or None; ``query_output`` dense, ``key_output``
-        dense or None; caches ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64 ``[>= tokens]``, or None."""
+        dense or None; caches ``[pages, page tokens, kv_heads, head_dim]`` of any strides with ``slots`` int64
+        ``[>= tokens]``, or None."""
         c, dim = self.ctx, self.head_dim
         q, qs, q_rows = _heads(c, query, "query", -1, self.q_heads, dim)
         k, ks, rows = _heads(c, key, "key", -1, self.kv_heads, dim)
